@@ -1,0 +1,230 @@
+// Block-scaled 4-bit matrices: quantiser and expander (formats and layout: fp4_common.cuh).
+//
+//   mxfp4   s = 2^ceil(log2(max(amax32, 6 * 2^-126) * (1/6)))           code = e2m1(x / s)
+//   nvfp4   u = x / ts (one f32 scale ts for the tensor, or none)       s = e4m3(max(amax16(u), 6 * 2^-9) / 6)
+//           code = e2m1(u / s), both quotients rounded to f32 first
+//
+// Both kernels are bound by HBM: 2 + 17/32 bytes per bf16 value in the quantiser.  A thread owns eight consecutive
+// columns (one 16-byte load of 16-bit values, one 4-byte store of codes), a block of 32 (16) columns is four (two)
+// lanes, and a warp takes the four rows i, 32 + i, 64 + i, 96 + i of a 128-row tile over 256 columns: four independent
+// loads in flight per thread, and the scales of those rows are 16 consecutive bytes of a chunk, so one lane writes them
+// in one store where a row-wise warp would scatter single words over half-filled sectors.
+//
+// x / s with s a power of two is a product with the exact reciprocal.  For an e4m3 scale the quotient has to be the
+// correctly rounded one (a bf16 value over a 4-bit scale often lies exactly on the border of two codes, and a product
+// with the rounded reciprocal falls to either side): Markstein's correction, q0 = u r, q = q0 + (u - q0 s) r with
+// r = rn(1 / s), two FMAs per value after one division per block.
+#include "fp4_common.cuh"
+
+namespace {
+
+using namespace fp4;
+
+__device__ int g_fp4_status[4];
+
+constexpr int kQThreads = 256;
+constexpr int kQCols = 256;   // columns of a warp's pass
+
+__device__ __forceinline__ float div_by(float u, float s, float r) {
+    const float q0 = __fmul_rn(u, r);
+    return __fmaf_rn(__fmaf_rn(-q0, s, u), r, q0);
+}
+
+// Tile of this CTA: rows (tile * 128 + 8 * sub + warp) + 32 g, columns 256 * ct ...; bt = matrix of the batch.
+struct Place { int64_t bt; int64_t row; int64_t tile; int i; int64_t col; };
+__device__ __forceinline__ Place place(int64_t rows, int64_t cols) {
+    const int64_t nct = (cols + kQCols - 1) / kQCols, nrt = (rows + 127) / 128;
+    int64_t b = blockIdx.x;
+    Place p;
+    const int64_t ct = b % nct;
+    b /= nct;
+    const int sub = (int)(b & 3);
+    b >>= 2;
+    p.tile = b % nrt;
+    p.bt = b / nrt;
+    p.i = sub * 8 + (threadIdx.x >> 5);
+    p.row = p.tile * 128 + p.i;
+    p.col = ct * kQCols + (threadIdx.x & 31) * 8;
+    return p;
+}
+
+template <int FMT, typename T>
+__global__ void __launch_bounds__(kQThreads)
+fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int vec, uint8_t* __restrict__ codes,
+                    uint8_t* __restrict__ scales, int64_t rows, int64_t cols, int scaled, float ts, float inv_ts) {
+    pdl_wait();
+    pdl_launch();
+    const Place p = place(rows, cols);
+    const int lane = threadIdx.x & 31;
+    const int64_t G = groups(cols), cstride = 64 * G;
+    const T* xb = x + p.bt * bstride;
+    const int n = (int)max((int64_t)0, min((int64_t)8, cols - p.col));
+    float v[4][8];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int64_t r = p.row + 32 * g;
+        load8(xb + (r < rows ? r * ld + p.col : 0), r < rows ? n : 0, vec && r < rows, v[g]);
+    }
+    uint32_t word[4];   // this lane's group of four blocks: their scale bytes, row by row
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        if (FMT == kNvFp4 && scaled) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[g][j] = div_by(v[g][j], ts, inv_ts);
+        }
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[g][j]));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        if (FMT == kMxFp4) m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        uint32_t byte, code;
+        if (FMT == kMxFp4) {
+            byte = ue8m0_of(m, 6.f * 1.17549435e-38f, kInv6);
+            const float inv = ue8m0_inv(min(byte, 253u));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[g][j] *= inv;
+        } else {
+            byte = m >= kInfBits ? 0x7fu
+                                 : (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(fmaxf(__uint_as_float(m), 6.f / 512.f), 6.f),
+                                                                   __NV_SATFINITE, __NV_E4M3);
+            const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
+            const float s = __half2float(*reinterpret_cast<const __half*>(&hr)), r = __frcp_rn(s);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[g][j] = div_by(v[g][j], s, r);
+        }
+        code = m >= kInfBits ? 0u : e2m1x8(v[g]);   // a block that is not finite: NaN scale, zero codes
+        const int64_t r = p.row + 32 * g;
+        // columns in 8s up to the padded row end (64 bytes per group of 128 columns)
+        if (r < rows && p.col < 128 * G)
+            *reinterpret_cast<uint32_t*>(codes + (p.bt * rows + r) * cstride + p.col / 2) = code;
+        // gather the bytes of four neighbouring blocks (16 lanes of mxfp4, 8 of nvfp4) into a word
+        constexpr int kPer = FMT == kMxFp4 ? 4 : 2;
+        uint32_t w = r < rows && n > 0 ? byte << (8 * (lane / kPer & 3)) : 0u;
+        if (lane % kPer) w = 0;
+#pragma unroll
+        for (int o = 1; o < 4 * kPer; o <<= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
+        word[g] = w;
+    }
+    constexpr int kChunkCols = FMT == kMxFp4 ? 128 : 64;
+    if (lane % (kChunkCols / 8) == 0 && p.col < 128 * G) {
+        const int64_t C = FMT == kMxFp4 ? G : 2 * G, nrt = (rows + 127) / 128;
+        uint8_t* chunk = scales + ((p.bt * nrt + p.tile) * C + p.col / kChunkCols) * 512;
+        *reinterpret_cast<uint4*>(chunk + p.i * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+    }
+}
+
+template <int FMT, typename T>
+__global__ void __launch_bounds__(kQThreads)
+fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, int64_t ld,
+                      int64_t bstride, int vec, int64_t rows, int64_t cols, float ts) {
+    PDL_PROLOGUE();
+    const Place p = place(rows, cols);
+    if (p.row >= rows || p.col >= cols) return;
+    const int64_t G = groups(cols), cstride = 64 * G, nrt = (rows + 127) / 128;
+    constexpr int kChunkCols = FMT == kMxFp4 ? 128 : 64;
+    const int64_t C = FMT == kMxFp4 ? G : 2 * G;
+    const uint4 sw = ldg_nc_v4(scales + ((p.bt * nrt + p.tile) * C + p.col / kChunkCols) * 512 + p.i * 16);
+    const uint32_t w[4] = {sw.x, sw.y, sw.z, sw.w};
+    uint32_t code[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int64_t r = p.row + 32 * g;
+        code[g] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(codes + (p.bt * rows + r) * cstride + p.col / 2)) : 0u;
+    }
+    const int shift = FMT == kMxFp4 ? 8 * (int)(p.col / 32 & 3) : 8 * (int)(p.col / 16 & 3);
+    const int n = (int)min((int64_t)8, cols - p.col);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int64_t r = p.row + 32 * g;
+        if (r >= rows) break;
+        const uint32_t byte = w[g] >> shift & 0xffu;
+        float s;
+        if (FMT == kMxFp4) {
+            // 2^(byte - 127): 0 is the subnormal 2^-127, 255 is NaN
+            s = byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
+        } else {
+            const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
+            s = __half2float(*reinterpret_cast<const __half*>(&hr));
+        }
+        float v[8];
+        e2m1x8_to_f32(code[g], v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], s), ts);
+        store8(out + p.bt * bstride + r * ld + p.col, n, vec, v);
+    }
+}
+
+int64_t grid_of(int64_t batch, int64_t rows, int64_t cols) {
+    return batch * ((rows + 127) / 128) * 4 * ((cols + kQCols - 1) / kQCols);
+}
+
+bool vec_ok(const void* p, int64_t ld, int64_t bstride, int esz) {
+    return ((uintptr_t)p & 15) == 0 && ld * esz % 16 == 0 && bstride * esz % 16 == 0;
+}
+
+}  // namespace
+
+int* fp4_status_ptr() {
+    static int* cached[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    int* p = __atomic_load_n(&cached[dev], __ATOMIC_ACQUIRE);
+    if (!p) {
+        void* a = nullptr;
+        if (cudaGetSymbolAddress(&a, g_fp4_status) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return nullptr;
+        }
+        p = (int*)a;
+        __atomic_store_n(&cached[dev], p, __ATOMIC_RELEASE);
+    }
+    return p;
+}
+
+// The status words of the current device's 4-bit kernels into host[4], and zeroed if `clear`; waits for the stream.
+FB_API int fb_fp4_status(int* host, int64_t clear, cudaStream_t st) {
+    int* p = fp4_status_ptr();
+    if (!p) return (int)cudaErrorNotSupported;
+    cudaError_t e = cudaMemcpyAsync(host, p, 16, cudaMemcpyDeviceToHost, st);
+    if (e == cudaSuccess && clear) e = cudaMemsetAsync(p, 0, 16, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    return (int)e;
+}
+
+// x [batch][rows][cols] (element strides bstride, ld, 1; dtype 0 f32, 1 bf16, 2 f16) -> codes, scales (fp4_common.cuh);
+// fmt 0 mxfp4, 1 nvfp4; ts: the tensor's scale (nvfp4, 2^-100 .. 2^100; 0: none).
+FB_API int fb_fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bstride, void* codes, void* scales, int64_t batch,
+                           int64_t rows, int64_t cols, int64_t fmt, float ts, cudaStream_t st) {
+    if (batch < 1 || rows < 1 || cols < 1 || (fmt != kMxFp4 && fmt != kNvFp4) || dtype < 0 || dtype > 2 ||
+        ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15))
+        return (int)cudaErrorInvalidValue;
+    const int64_t grid = grid_of(batch, rows, cols);
+    if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const int scaled = fmt == kNvFp4 && ts != 0.f && ts != 1.f;
+    const float inv = scaled ? (float)(1.0 / (double)ts) : 1.f;
+    const int vec = vec_ok(x, ld, bstride, dtype == kF32 ? 4 : 2);
+#define FP4_Q(F, D)                                                                                                         \
+    (int)fp4_launch(fp4_quantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, g_fb_pdl != 0,      \
+                    (const Elem<D>::T*)x, ld, bstride, vec, (uint8_t*)codes, (uint8_t*)scales, rows, cols, scaled, ts, inv)
+    if (fmt == kMxFp4) return dtype == kF32 ? FP4_Q(kMxFp4, kF32) : dtype == kBf16 ? FP4_Q(kMxFp4, kBf16) : FP4_Q(kMxFp4, kF16);
+    return dtype == kF32 ? FP4_Q(kNvFp4, kF32) : dtype == kBf16 ? FP4_Q(kNvFp4, kBf16) : FP4_Q(kNvFp4, kF16);
+#undef FP4_Q
+}
+
+// codes, scales -> out [batch][rows][cols] (element strides bstride, ld, 1).
+FB_API int fb_fp4_dequantize(const void* codes, const void* scales, void* out, int64_t dtype, int64_t ld, int64_t bstride,
+                             int64_t batch, int64_t rows, int64_t cols, int64_t fmt, float ts, cudaStream_t st) {
+    if (batch < 1 || rows < 1 || cols < 1 || (fmt != kMxFp4 && fmt != kNvFp4) || dtype < 0 || dtype > 2 ||
+        ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15))
+        return (int)cudaErrorInvalidValue;
+    const int64_t grid = grid_of(batch, rows, cols);
+    if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
+    const int vec = vec_ok(out, ld, bstride, dtype == kF32 ? 4 : 2);
+    const float t = ts == 0.f ? 1.f : ts;
+#define FP4_D(F, D)                                                                                                    \
+    (int)fp4_launch(fp4_dequantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, g_fb_pdl != 0, \
+                    (const uint8_t*)codes, (const uint8_t*)scales, (Elem<D>::T*)out, ld, bstride, vec, rows, cols, t)
+    if (fmt == kMxFp4) return dtype == kF32 ? FP4_D(kMxFp4, kF32) : dtype == kBf16 ? FP4_D(kMxFp4, kBf16) : FP4_D(kMxFp4, kF16);
+    return dtype == kF32 ? FP4_D(kNvFp4, kF32) : dtype == kBf16 ? FP4_D(kNvFp4, kBf16) : FP4_D(kNvFp4, kF16);
+#undef FP4_D
+}

@@ -1,0 +1,220 @@
+// Shared by the block-scaled 4-bit operators (fp4.cu, fp4_gemm.cu, fp4_moe.cu).
+//
+// A 4-bit matrix [rows, cols] is two byte arrays:
+//   codes  [rows][64 * G], G = ceil(cols / 128): two e2m1 codes per byte, the even column in the low nibble, zero codes
+//          behind the last column.  A row is then a whole number of 64-byte groups, which is what every TMA box here
+//          starts at and what the padded 4-bit TMA form asks of a row.
+//   scales [ceil(rows / 128)][C][512], C = G (mxfp4: ue8m0 per 32 columns) or 2 G (nvfp4: e4m3 per 16 columns): byte
+//          16 i + 4 g + s of a chunk belongs to row 32 g + i of the 128 and to block s of the chunk's four: the shape
+//          that one tcgen05.cp (32x128b, broadcast to the four lane quarters) puts into tensor memory for an MMA.
+#pragma once
+#include <type_traits>
+
+#include "tc_common.cuh"
+
+enum Fp4Fmt : int { kMxFp4 = 0, kNvFp4 = 1 };
+enum Fp4Dtype : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
+
+// Device words that the bounded waits of these kernels report to (the current device's copy); null if CUDA refuses.
+int* fp4_status_ptr();
+
+// Launch with an optional cluster of `cluster` CTAs along x and, with `pdl`, programmatic serialisation against the
+// kernel before it in the stream (that kernel must be one of this file family: it waits for its own predecessor
+// before it lets its successor start).
+template <typename... KArgs, typename... Args>
+inline cudaError_t fp4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, bool pdl,
+                              Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+    if (e != cudaSuccess) (void)cudaGetLastError();   // reported to this caller, not to the next launch
+    return e;
+}
+
+// cudaFuncSetAttribute once per kernel and device.
+template <typename F>
+inline cudaError_t fp4_allow_smem(F kernel, size_t bytes, unsigned long long& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev & 1)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
+    return e;
+}
+
+namespace fp4 {
+
+constexpr float kInv6 = 1.f / 6.f;
+constexpr float kInv448 = 1.f / 448.f;
+
+__host__ __device__ __forceinline__ int64_t groups(int64_t cols) { return (cols + 127) / 128; }
+
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* gsrc, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_dst), "l"(gsrc), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Shared-memory descriptor of a 512-byte scale chunk (no swizzle, 8-row groups 128 bytes apart).
+__device__ __forceinline__ uint64_t sf_desc(uint32_t smem_addr) {
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+}
+__device__ __forceinline__ void tmem_cp_sf(uint32_t taddr, uint64_t sdesc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// ---- clusters ------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t smem_addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+// ---- codes -----------------------------------------------------------------------------------------
+// Eight f32 -> eight e2m1 codes (round to nearest, ties to even, saturating), value j in nibble j.
+__device__ __forceinline__ uint32_t e2m1x8(const float (&v)[8]) {
+    uint32_t d;
+    asm("{\n .reg .b8 b0, b1, b2, b3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+        " cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+        " mov.b32 %0, {b0, b1, b2, b3};\n}"
+        : "=r"(d) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return d;
+}
+// Eight codes -> eight f32 (exact).
+__device__ __forceinline__ void e2m1x8_to_f32(uint32_t w, float (&v)[8]) {
+    uint32_t h[4];
+    asm("{\n .reg .b8 b0, b1, b2, b3;\n mov.b32 {b0, b1, b2, b3}, %4;\n"
+        " cvt.rn.f16x2.e2m1x2 %0, b0;\n cvt.rn.f16x2.e2m1x2 %1, b1;\n cvt.rn.f16x2.e2m1x2 %2, b2;\n cvt.rn.f16x2.e2m1x2 %3, b3;\n}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
+// |x| as an integer: NaN > inf > every number, so a maximum of these keeps what a float maximum would drop.
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+constexpr uint32_t kInfBits = 0x7f800000u;
+
+// Power-of-two scale exponent byte (ue8m0) of a block: 2^ceil(log2(amax * (1 / top))), amax floored.  255 (NaN) for a
+// block that holds an infinity or a NaN.
+__device__ __forceinline__ uint32_t ue8m0_of(uint32_t amax_bits, float floor, float inv_top) {
+    if (amax_bits >= kInfBits) return 255u;
+    const uint32_t b = __float_as_uint(__fmul_rn(fmaxf(__uint_as_float(amax_bits), floor), inv_top));
+    return (b >> 23) + ((b & 0x7fffffu) != 0u);
+}
+// 1 / 2^(e - 127) for e in 1..253
+__device__ __forceinline__ float ue8m0_inv(uint32_t e) { return __uint_as_float((254u - e) << 23); }
+
+// ---- values of the three element types -----------------------------------------------------------
+template <int DT> struct Elem;
+template <> struct Elem<kF32> { using T = float; };
+template <> struct Elem<kBf16> { using T = __nv_bfloat16; };
+template <> struct Elem<kF16> { using T = __half; };
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+
+// p[0 .. 7] -> f32; `n` of them exist (the others read 0); vec: p is 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
+    if (vec && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const uint4 a = ldg_nc_v4(p), b = ldg_nc_v4(p + 4);
+            v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+            v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+        } else {
+            const uint4 a = ldg_nc_v4(p);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    v[2 * i] = bf16lo(w[i]);
+                    v[2 * i + 1] = bf16hi(w[i]);
+                } else {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    v[2 * i] = f.x;
+                    v[2 * i + 1] = f.y;
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
+    }
+}
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+// The first n of eight values to p.
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
+    if (vec && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = from_f32<T>(v[i]);
+    }
+}
+
+}  // namespace fp4

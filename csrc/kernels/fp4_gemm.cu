@@ -1,0 +1,420 @@
+// Product of two block-scaled 4-bit matrices on the 5th-generation tensor cores:
+//
+//   out[m, n] = alpha * sum_k X[m, k] W[n, k],   X, W = e2m1 codes times block scales (fp4_common.cuh)
+//
+// tcgen05.mma kind::mxf4 (ue8m0 per 32, two scales per K = 64 step) or kind::mxf4nvf4 (e4m3 per 16, four per step):
+// both operands stay packed in shared memory (128 bytes = 256 values per row, 128-byte swizzle) and the hardware
+// applies the scales, which tcgen05.cp moves from shared to tensor memory.  Nothing is expanded anywhere.
+//
+// The operand on the 128 lanes of the accumulator is called P, the other one Q (BN columns).  Many rows: P = X, so a
+// thread of the epilogue holds neighbouring outputs of one row.  Few rows (one tile of Q holds all of X): P = W, the
+// weights fill the lanes whatever the number of rows, and the K axis is split over a cluster of S CTAs whose partial
+// tiles are summed in rank order through distributed shared memory: no workspace, no atomics, the same bits every run.
+//
+// Warps: 0 producer (TMA boxes of both operands, bulk copies of the scale chunks), 1 MMA issuer, 2..9 epilogue (two per
+// lane quarter).  Without a split the CTAs are persistent and walk the tiles; the accumulator is handed to the epilogue
+// and back through two barriers.  Every wait has a clock budget; on expiry the status words say so, the tile is not
+// stored and the tensor memory is released.
+#include "fp4_common.cuh"
+
+namespace {
+
+using namespace fp4;
+
+constexpr int kBK = 256;          // values per stage row (128 bytes)
+constexpr int kGThreads = 320;
+constexpr int kEpi = 256;         // epilogue threads
+
+template <int FMT, int BN>
+struct GemmCfg {
+    static constexpr int kChunks = FMT == kMxFp4 ? 2 : 4;              // scale chunks of a stage per 128 rows
+    static constexpr int kQAtoms = (BN + 127) / 128;
+    static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
+    static constexpr int kSfa = 512 * kChunks, kSfb = kSfa * kQAtoms;
+    static constexpr int kStageBytes = (kABytes + kBBytes + kSfa + kSfb + 1023) / 1024 * 1024;
+    static constexpr int kBudget = BN <= 32 ? 113 * 1024 : 225 * 1024;  // up to 32 columns: two CTAs per SM
+    static constexpr int kStages = (kBudget - 1280) / kStageBytes;
+    static constexpr int kSfCols = 4 * kChunks * (1 + kQAtoms);        // tensor memory columns of a stage's scales
+    static constexpr int kAcc = BN < 32 ? 32 : BN;
+    static constexpr int kNeed = kAcc + 2 * kSfCols;
+    static constexpr int kTmem = kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024 + 256;
+    static_assert(kStages >= 3 && kStages * 16 + 32 <= 256, "stages");
+    static_assert((size_t)BN * 128 * 4 <= (size_t)kStages * kStageBytes, "the partial tile reuses the stages");
+};
+
+template <int FMT>
+__host__ __device__ constexpr uint32_t fp4_idesc(int N, int sf) {
+    // A, B: e2m1 (1); scale type ue8m0 (1) or ue4m3 (0); M = 128; sf: scale byte of the 32-bit word, both operands
+    return ((uint32_t)sf << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((FMT == kMxFp4 ? 1u : 0u) << 23) |
+           ((128u >> 4) << 24) | ((uint32_t)sf << 29);
+}
+template <int FMT>
+__device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+    if constexpr (FMT == kMxFp4)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                     " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                     " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
+}
+
+struct GemmArgs {
+    const uint8_t *sfp, *sfq;
+    void* out;
+    int64_t ldo;
+    int64_t P, Q, K;
+    float alpha;
+    int dtype, vec, tiles_p, tiles_q, splits, pdl;
+    int* status;
+};
+
+template <typename T, bool SWAP, int BN>
+__device__ __forceinline__ void store_direct(const GemmArgs& a, uint32_t tmem, int warp, int lane, int64_t p0, int64_t q0) {
+    // warp w of 0..7: lane quarter w & 3, column half w >> 2 (all columns in 16s)
+    const int quarter = warp & 3;
+    const int64_t p = p0 + quarter * 32 + lane;
+    T* out = reinterpret_cast<T*>(a.out);
+    constexpr int kHalf = BN >= 32 ? BN / 2 : BN;
+    if (BN < 32 && warp >= 4) return;
+    const int c0 = (warp >> 2) * kHalf;
+#pragma unroll 1
+    for (int c = c0; c < c0 + kHalf; c += 16) {
+        if (q0 + c >= a.Q) break;
+        uint32_t r[16];
+        tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c, r);
+        tmem_ld_wait();
+        if (p >= a.P) continue;
+        const int n = (int)min((int64_t)16, a.Q - (q0 + c));
+        if (SWAP) {   // lane = output column: a warp's store is 32 neighbouring outputs of row q0 + c + j
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                if (j < n) out[(q0 + c + j) * a.ldo + p] = from_f32<T>(__uint_as_float(r[j]) * a.alpha);
+        } else {
+            float v[8];
+            T* o = out + p * a.ldo + q0 + c;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * h + j]) * a.alpha;
+                if (n > 8 * h) store8(o + 8 * h, n - 8 * h, a.vec != 0, v);
+            }
+        }
+    }
+}
+
+template <typename T, bool SWAP, int BN>
+__device__ __forceinline__ void store_reduced(const GemmArgs& a, uint32_t part, int t, int rank, int64_t p0, int64_t q0) {
+    // part: this CTA's partial tile [BN][128] f32 in shared memory; ranks own the column groups of 128 lanes in turn
+    T* out = reinterpret_cast<T*>(a.out);
+    const int S = a.splits, lane = t & 127;
+    for (int c = rank * 2 + (t >> 7); c < BN; c += 2 * S) {
+        if (q0 + c >= a.Q) break;
+        float v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) v[s] = s < S ? ld_cluster(map_rank(part + (uint32_t)(c * 128 + lane) * 4, s)) : 0.f;
+        float sum = v[0];
+#pragma unroll
+        for (int s = 1; s < 8; ++s) sum += v[s];
+        const int64_t p = p0 + lane, q = q0 + c;
+        if (p < a.P) out[SWAP ? q * a.ldo + p : p * a.ldo + q] = from_f32<T>(sum * a.alpha);
+    }
+}
+
+template <int FMT, int BN, bool SWAP>
+__global__ void __launch_bounds__(kGThreads, BN <= 32 ? 2 : 1)
+fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const GemmArgs a) {
+    using C = GemmCfg<FMT, BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bars = base + C::kStages * C::kStageBytes;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (C::kStages + s); };
+    const uint32_t acc_full = bars + 16u * C::kStages, acc_empty = acc_full + 8u, tmem_slot = acc_full + 16u;
+    __shared__ int s_fail;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = a.splits, rank = S > 1 ? (int)cluster_rank() : 0;
+    const int64_t G = groups(a.K);
+    const int64_t Cch = FMT == kMxFp4 ? G : 2 * G;
+    const int nkb_all = (int)((G + 1) / 2);
+    const int kb0 = (int)((int64_t)nkb_all * rank / S), kb1 = (int)((int64_t)nkb_all * (rank + 1) / S);
+    const int n_tiles = a.tiles_p * a.tiles_q;
+    const int first = S > 1 ? blockIdx.x / S : blockIdx.x, step = S > 1 ? n_tiles : gridDim.x;
+    // tiles in bands of kBand along P, so that the CTAs in flight share operand tiles through L2
+    constexpr int kBand = 8;
+    auto tile_at = [&](int t, int64_t& p0, int64_t& q0) {
+        const int band = t / (kBand * a.tiles_q), in = t - band * kBand * a.tiles_q;
+        const int h = min(kBand, a.tiles_p - band * kBand);
+        p0 = (int64_t)(band * kBand + in % h) * 128;
+        q0 = (int64_t)(in / h) * BN;
+    };
+
+    if (threadIdx.x == 0) {
+        s_fail = 0;
+        for (int s = 0; s < C::kStages; ++s) {
+            tc::mbar_init(full(s), 1);
+            tc::mbar_init(empty(s), 1);
+        }
+        tc::mbar_init(acc_full, 1);
+        tc::mbar_init(acc_empty, kEpi / 32);
+        tc::mbar_fence_init();
+        tc::prefetch_tmap(&tmap_p);
+        tc::prefetch_tmap(&tmap_q);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    const uint32_t a_off = 0, b_off = C::kABytes, sfa_off = b_off + C::kBBytes, sfb_off = sfa_off + C::kSfa;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const int qatoms = C::kQAtoms;
+            const int64_t q_rowtiles = (a.Q + 127) / 128;
+            auto issue_p = [&](int s, int kb, int64_t p0, int nch) {
+                tc::tma_load_2d(base + s * C::kStageBytes + a_off, &tmap_p, kb * 128, (int)p0, full(s));
+                bulk_load(base + s * C::kStageBytes + sfa_off, a.sfp + ((p0 / 128) * Cch + (int64_t)kb * C::kChunks) * 512, 512 * nch, full(s));
+            };
+            auto issue_q = [&](int s, int kb, int64_t q0, int nch) {
+                tc::tma_load_2d(base + s * C::kStageBytes + b_off, &tmap_q, kb * 128, (int)q0, full(s));
+                for (int at = 0; at < qatoms; ++at)
+                    if (q0 / 128 + at < q_rowtiles)
+                        bulk_load(base + s * C::kStageBytes + sfb_off + at * C::kSfa,
+                                  a.sfq + ((q0 / 128 + at) * Cch + (int64_t)kb * C::kChunks) * 512, 512 * nch, full(s));
+            };
+            auto arm = [&](int s, int64_t q0, int nch) {
+                const int at = (int)min((int64_t)qatoms, q_rowtiles - q0 / 128);
+                tc::mbar_expect_tx(full(s), C::kABytes + C::kBBytes + 512 * nch * (1 + at));
+            };
+            auto chunks = [&](int kb) { return (int)min((int64_t)C::kChunks, Cch - (int64_t)kb * C::kChunks); };
+            int it = 0;
+            bool ok = true;
+            for (int t = first; t < n_tiles && ok; t += step) {
+                int64_t p0, q0;
+                tile_at(t, p0, q0);
+                int kb = kb0;
+                if (t == first && a.pdl) {
+                    // X is written by the kernel before this one: only W (P when swapped) may be read before the wait
+                    const int ahead = SWAP ? min(C::kStages, kb1 - kb0) : 0;
+                    for (int i = 0; i < ahead; ++i) {
+                        arm(i, q0, chunks(kb0 + i));
+                        issue_p(i, kb0 + i, p0, chunks(kb0 + i));
+                    }
+                    pdl_wait();
+                    for (int i = 0; i < ahead; ++i) issue_q(i, kb0 + i, q0, chunks(kb0 + i));
+                    kb += ahead;
+                    it += ahead;
+                }
+                for (; kb < kb1; ++kb, ++it) {
+                    const int s = it % C::kStages;
+                    if (it >= C::kStages && !tc::mbar_wait(empty(s), ((it / C::kStages) - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                    arm(s, q0, chunks(kb));
+                    issue_p(s, kb, p0, chunks(kb));
+                    issue_q(s, kb, q0, chunks(kb));
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            int it = 0, tile_no = 0;
+            bool ok = true;
+            for (int t = first; t < n_tiles && ok; t += step, ++tile_no) {
+                if (tile_no && !tc::mbar_wait(acc_empty, (tile_no - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                tc::tc_fence_after();
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int s = it % C::kStages;
+                    if (!tc::mbar_wait(full(s), (it / C::kStages) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t st = base + s * C::kStageBytes;
+                    const uint32_t sfa_t = tmem + C::kAcc + (uint32_t)(it & 1) * C::kSfCols, sfb_t = sfa_t + 4 * C::kChunks;
+                    const int steps = (int)min((int64_t)4, (a.K - (int64_t)kb * kBK + 63) / 64);
+                    const int nch = FMT == kMxFp4 ? (steps + 1) / 2 : steps;
+                    for (int c = 0; c < nch; ++c) {
+                        tmem_cp_sf(sfa_t + 4 * c, sf_desc(st + sfa_off + 512 * c));
+#pragma unroll
+                        for (int at = 0; at < C::kQAtoms; ++at)   // word c of all atoms side by side: 4 columns per 128 rows
+                            tmem_cp_sf(sfb_t + 4 * (c * C::kQAtoms + at), sf_desc(st + sfb_off + at * C::kSfa + 512 * c));
+                    }
+                    const uint64_t ad = tc::umma_desc_sw128(st + a_off), bd = tc::umma_desc_sw128(st + b_off);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (k >= steps) break;
+                        const int c = FMT == kMxFp4 ? k / 2 : k;
+                        umma_fp4<FMT>(tmem, ad + 2u * k, bd + 2u * k, fp4_idesc<FMT>(BN, FMT == kMxFp4 ? 2 * (k & 1) : 0),
+                                      sfa_t + 4 * c, sfb_t + 4 * c * C::kQAtoms, (kb > kb0 || k) ? 1u : 0u);
+                    }
+                    tc::umma_commit(empty(s));
+                }
+                tc::umma_commit(acc_full);
+            }
+        }
+    } else {
+        const int w = warp - 2;
+        // warps 2..9: TMEM lane quarter = warp & 3
+        const int quarter_warp = (warp & 3) | (w >= 4 ? 4 : 0);
+        int tile_no = 0;
+        for (int t = first; t < n_tiles; t += step, ++tile_no) {
+            int64_t p0, q0;
+            tile_at(t, p0, q0);
+            const bool done = tc::mbar_wait(acc_full, tile_no & 1, 4000000000ll);
+            tc::tc_fence_after();
+            if (!done) atomicExch(&s_fail, 1);
+            const bool go = __shfl_sync(0xffffffffu, (done && *(volatile int*)&s_fail == 0) ? 1 : 0, 0) != 0;
+            if (S > 1) {
+                // the stages are drained (every MMA of this CTA is complete): the partial tile goes into them
+                if (go) {
+                    const int quarter = quarter_warp & 3;
+                    constexpr int kHalf = BN >= 32 ? BN / 2 : BN;
+                    if (BN >= 32 || quarter_warp < 4) {
+                        const int c0 = (quarter_warp >> 2) * kHalf;
+#pragma unroll 1
+                        for (int c = c0; c < c0 + kHalf; c += 16) {
+                            uint32_t r[16];
+                            tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c, r);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + (uint32_t)((c + j) * 128 + quarter * 32 + lane) * 4), "r"(r[j]) : "memory");
+                        }
+                    }
+                }
+            } else if (go) {
+                if (a.dtype == kBf16) store_direct<__nv_bfloat16, SWAP, BN>(a, tmem, quarter_warp, lane, p0, q0);
+                else if (a.dtype == kF16) store_direct<__half, SWAP, BN>(a, tmem, quarter_warp, lane, p0, q0);
+                else store_direct<float, SWAP, BN>(a, tmem, quarter_warp, lane, p0, q0);
+            }
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);   // also after a failed wait
+            if (!go) break;
+        }
+    }
+    __syncwarp();
+    tc::tc_fence_before();
+    if (S > 1) {
+        // s_fail of every CTA is final and its partial tile is visible to the cluster
+        cluster_sync_all();
+        if (warp >= 2) {
+            int64_t p0, q0;
+            tile_at(first, p0, q0);
+            int bad = 0;
+            for (int s = 0; s < S; ++s) {
+                int f;
+                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(f) : "r"(map_rank(tc::smem_u32(&s_fail), s)) : "memory");
+                bad |= f;
+            }
+            if (!bad) {
+                const int t = threadIdx.x - 64;
+                if (a.dtype == kBf16) store_reduced<__nv_bfloat16, SWAP, BN>(a, base, t, rank, p0, q0);
+                else if (a.dtype == kF16) store_reduced<__half, SWAP, BN>(a, base, t, rank, p0, q0);
+                else store_reduced<float, SWAP, BN>(a, base, t, rank, p0, q0);
+            }
+        }
+        cluster_sync_all();   // nobody leaves while a peer still reads its tile
+    } else {
+        __syncthreads();
+    }
+    if (threadIdx.x == 0 && s_fail && a.status) { a.status[0] = FB_TIMEOUT; a.status[1] = blockIdx.x; a.status[2] = BN; a.status[3] = S; }
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, C::kTmem);
+    }
+}
+
+template <int FMT, int BN, bool SWAP>
+int launch_gemm(const GemmArgs& a, const void* pc, const void* qc, int grid, cudaStream_t st) {
+    using C = GemmCfg<FMT, BN>;
+    CUtensorMap tp, tq;
+    const uint64_t bytes = (uint64_t)(64 * groups(a.K));
+    // the row end (a multiple of 64 bytes) lies inside a 128-byte box of the last stage: what is behind it reads zero
+    int rc = fb_make_tmap_2d(&tp, pc, (uint64_t)a.P, bytes, 128, 128, 1);
+    if (!rc) rc = fb_make_tmap_2d(&tq, qc, (uint64_t)a.Q, bytes, BN, 128, 1);
+    if (rc) return rc;
+    auto k = fp4_gemm_kernel<FMT, BN, SWAP>;
+    static unsigned long long allowed = 0;
+    cudaError_t e = fp4_allow_smem(k, C::kSmem, allowed);
+    if (e != cudaSuccess) return (int)e;
+    return (int)fp4_launch(k, dim3((unsigned)grid), dim3(kGThreads), C::kSmem, st, a.splits, a.pdl != 0, tp, tq, a);
+}
+
+template <int FMT>
+int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, const uint8_t* ws, int64_t M, int64_t N, cudaStream_t st) {
+    const int sms = 148;
+    const int nkb = (int)((groups(a.K) + 1) / 2);
+    if (M <= 128) {
+        // weights on the lanes; as many K splits as fill the SMs, with at least two stages each
+        const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+        const int slots = bn <= 32 ? 2 * sms : sms;
+        a.P = N; a.Q = M; a.sfp = ws; a.sfq = xs;
+        a.tiles_p = (int)((N + 127) / 128);
+        a.tiles_q = 1;
+        int S = 1;
+        while (S < 8 && a.tiles_p * S * 2 <= slots && nkb >= 4 * S) S *= 2;
+        a.splits = S;
+        const int grid = S > 1 ? a.tiles_p * S : (a.tiles_p < slots ? a.tiles_p : slots);
+        switch (bn) {
+            case 16: return launch_gemm<FMT, 16, true>(a, wc, xc, grid, st);
+            case 32: return launch_gemm<FMT, 32, true>(a, wc, xc, grid, st);
+            case 64: return launch_gemm<FMT, 64, true>(a, wc, xc, grid, st);
+            default: return launch_gemm<FMT, 128, true>(a, wc, xc, grid, st);
+        }
+    }
+    a.P = M; a.Q = N; a.sfp = xs; a.sfq = ws;
+    a.tiles_p = (int)((M + 127) / 128);
+    const int64_t t256 = (int64_t)a.tiles_p * ((N + 255) / 256), t128 = (int64_t)a.tiles_p * ((N + 127) / 128);
+    // tiles of 256 columns unless the narrower ones fill the last wave better
+    const bool wide = (t256 + sms - 1) / sms * 2 <= (t128 + sms - 1) / sms;
+    a.tiles_q = (int)((N + (wide ? 255 : 127)) / (wide ? 256 : 128));
+    const int64_t tiles = wide ? t256 : t128;
+    if (tiles > 0x3fffffff) return (int)cudaErrorInvalidValue;
+    int S = 1;
+    while (S < 8 && tiles * S * 2 <= sms && nkb >= 4 * S) S *= 2;
+    a.splits = S;
+    const int grid = S > 1 ? (int)tiles * S : (int)(tiles < sms ? tiles : sms);
+    if (wide) return launch_gemm<FMT, 256, false>(a, xc, wc, grid, st);
+    return launch_gemm<FMT, 128, false>(a, xc, wc, grid, st);
+}
+
+}  // namespace
+
+FB_API int fb_fp4_quantize(const void*, int64_t, int64_t, int64_t, void*, void*, int64_t, int64_t, int64_t, int64_t, float, cudaStream_t);
+
+static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, void* out, int64_t dtype, int64_t ldo, int64_t M,
+                      int64_t N, int64_t K, int64_t fmt, float alpha, int pdl, cudaStream_t st) {
+    if (M < 1 || N < 1 || K < 1 || M > 0x7fffff00ll || N > 0x7fffff00ll || K > 0x3fffff00ll || ldo < N || dtype < 0 || dtype > 2 ||
+        (fmt != kMxFp4 && fmt != kNvFp4) || (((uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws) & 15))
+        return (int)cudaErrorInvalidValue;
+    GemmArgs a = {};
+    a.out = out; a.ldo = ldo; a.K = K; a.alpha = alpha; a.dtype = (int)dtype; a.pdl = pdl;
+    const int esz = dtype == kF32 ? 4 : 2;
+    a.vec = ((uintptr_t)out & 15) == 0 && ldo * esz % 16 == 0;
+    a.status = fp4_status_ptr();
+    if (!a.status) return (int)cudaErrorNotSupported;
+    return fmt == kMxFp4 ? gemm_fmt<kMxFp4>(a, xc, (const uint8_t*)xs, wc, (const uint8_t*)ws, M, N, st)
+                         : gemm_fmt<kNvFp4>(a, xc, (const uint8_t*)xs, wc, (const uint8_t*)ws, M, N, st);
+}
+
+// out[M, N] (row stride ldo, dtype 0 f32, 1 bf16, 2 f16) = alpha * X W^T of two 4-bit matrices of one format with K columns.
+FB_API int fb_fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, void* out, int64_t dtype, int64_t ldo,
+                         int64_t M, int64_t N, int64_t K, int64_t fmt, float alpha, cudaStream_t st) {
+    return fp4_matmul(xc, xs, wc, ws, out, dtype, ldo, M, N, K, fmt, alpha, 0, st);
+}
+
+// The same with the rows of x [M, K] (dtype xdt, row stride ldx) quantised first, into `work`: codes
+// [M][64 ceil(K / 128)], then (at the next multiple of 512) the scale chunks.  Two launches; the product's prologue and its
+// first weight tiles overlap the quantiser.
+FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, const void* wc, const void* ws, void* out,
+                         int64_t dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t fmt, float xts, float alpha,
+                         cudaStream_t st) {
+    if (M < 1 || K < 1 || ((uintptr_t)work & 15)) return (int)cudaErrorInvalidValue;
+    uint8_t* codes = (uint8_t*)work;
+    uint8_t* scales = codes + (M * 64 * groups(K) + 511) / 512 * 512;
+    const int rc = fb_fp4_quantize(x, xdt, ldx, 0, codes, scales, 1, M, K, fmt, xts, st);
+    if (rc) return rc;
+    return fp4_matmul(codes, scales, wc, ws, out, dtype, ldo, M, N, K, fmt, alpha, 1, st);
+}

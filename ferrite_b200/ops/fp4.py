@@ -1,0 +1,261 @@
+"""Block-scaled 4-bit matrices on the device: quantiser, expander and products
+(``csrc/kernels/fp4.cu``, ``fp4_gemm.cu``).
+
+A value is an e2m1 code times the scale of its block of consecutive columns:
+
+* ``"mxfp4"``: blocks of 32, the scale a power of two (ue8m0): ``2^ceil(log2(amax / 6))``, the form of the expert weights
+  (``ops/quant.py::quant_fp4_weight``);
+* ``"nvfp4"``: blocks of 16, the scale an e4m3 number (``amax / 6`` rounded, ``ops/quant.py::fp4_act_roundtrip`` with
+  ``scale="e4m3"``), and optionally one f32 ``tensor_scale`` by which the values are divided first.
+
+A block that holds an infinity or a NaN gets the NaN scale: all of its values, and every product that meets it, read NaN.
+
+All functions launch on the current stream of their operands' device, allocate with torch's allocator (nothing is kept
+between calls, so calls may overlap on several streams and be captured) and raise ``ValueError`` / ``TypeError`` for
+arguments they do not take and ``KernelError`` when CUDA refuses a launch.  A wait inside a kernel that ran out is
+reported by :func:`check`.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _lib
+from .quant import e2m1_unpack
+
+FORMATS = {"mxfp4": 0, "nvfp4": 1}
+BLOCK = {"mxfp4": 32, "nvfp4": 16}
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class Fp4Tensor:
+    """A 4-bit tensor ``[..., rows, cols]``: ``codes`` [..., rows, 64 * ceil(cols / 128)] uint8 (the even column in the low
+    nibble, zero codes behind the last column) and ``scales`` [..., ceil(rows / 128), C, 512] uint8 with C =
+    ceil(cols / 128) (mxfp4) or twice that (nvfp4): byte ``16 i + 4 g + s`` of a chunk is the scale of row ``32 g + i`` and
+    block ``s`` of the chunk's four.  Scale bytes of rows and blocks that do not exist are never NaN codes.
+
+    ``tensor_scale`` (a float, nvfp4 only) multiplies every value."""
+
+    __slots__ = ("codes", "scales", "fmt", "shape", "tensor_scale")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str, shape, tensor_scale: Optional[float] = None):
+        if fmt not in FORMATS:
+            raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
+        shape = tuple(shape)
+        if len(shape) < 2 or shape[-1] < 1 or min(shape) < 0:
+            raise ValueError(f"a 4-bit tensor has a shape [..., rows, cols >= 1], got {shape}")
+        if tensor_scale is not None:
+            _check_scale(tensor_scale, fmt)
+        g = (shape[-1] + 127) // 128
+        c = g if fmt == "mxfp4" else 2 * g
+        if tuple(codes.shape) != (*shape[:-1], 64 * g) or tuple(scales.shape) != (*shape[:-2], (shape[-2] + 127) // 128, c, 512):
+            raise ValueError(f"codes {tuple(codes.shape)} / scales {tuple(scales.shape)} do not belong to a {fmt} tensor of shape {shape}")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("codes and scales are uint8")
+        if codes.device != scales.device:
+            raise ValueError("codes and scales are on different devices")
+        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 32 or scales.data_ptr() % 16:
+            raise ValueError("codes and scales are contiguous, codes on a 32-byte and scales on a 16-byte boundary")
+        self.codes, self.scales, self.fmt, self.shape, self.tensor_scale = codes, scales, fmt, shape, tensor_scale
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def __repr__(self) -> str:
+        return f"Fp4Tensor({self.fmt}, shape={self.shape}, tensor_scale={self.tensor_scale}, device={self.device})"
+
+    @staticmethod
+    def from_rows(packed: torch.Tensor, scale: torch.Tensor, fmt: str = "mxfp4", tensor_scale: Optional[float] = None) -> "Fp4Tensor":
+        """From checkpoint order: ``packed`` [..., rows, cols / 2] codes (cols a whole number of blocks) and ``scale`` bytes
+        [..., rows, cols / block], as ``ops/quant.py::quant_fp4_weight`` returns them.  Copies; done once at load time."""
+        if fmt not in FORMATS:
+            raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
+        rows, cols = packed.shape[-2], 2 * packed.shape[-1]
+        if tuple(scale.shape) != (*packed.shape[:-1], cols // BLOCK[fmt]) or cols % BLOCK[fmt]:
+            raise ValueError(f"packed {tuple(packed.shape)} and scale {tuple(scale.shape)} do not match for {fmt}")
+        if packed.dtype != torch.uint8 or scale.dtype != torch.uint8:
+            raise TypeError("packed codes and scale bytes are uint8")
+        g = (cols + 127) // 128
+        codes = torch.nn.functional.pad(packed, (0, 64 * g - cols // 2)).contiguous()
+        return Fp4Tensor(codes, pack_scales(scale, 128 * g // BLOCK[fmt]), fmt, (*packed.shape[:-1], cols), tensor_scale)
+
+
+def pack_scales(scale: torch.Tensor, blocks: Optional[int] = None) -> torch.Tensor:
+    """Scale bytes [..., rows, n] in row order -> chunks [..., ceil(rows / 128), ceil(blocks / 4), 512]; missing bytes are 0
+    (a valid exponent, and a zero in e4m3)."""
+    rows, n = scale.shape[-2:]
+    blocks = max(n, blocks or 0)
+    s = torch.nn.functional.pad(scale, (0, blocks - n + -blocks % 4, 0, -rows % 128))
+    lead = s.shape[:-2]
+    s = s.reshape(*lead, s.shape[-2] // 128, 4, 32, s.shape[-1] // 4, 4)
+    k = len(lead)
+    out = s.permute(*range(k), k, k + 3, k + 2, k + 1, k + 4)
+    return out.reshape(*lead, s.shape[k], s.shape[k + 3], 512).contiguous()
+
+
+def unpack_scales(chunks: torch.Tensor, rows: int, blocks: int) -> torch.Tensor:
+    """The inverse of :func:`pack_scales`: bytes [..., rows, blocks]."""
+    lead = chunks.shape[:-3]
+    k = len(lead)
+    s = chunks.reshape(*lead, chunks.shape[k], chunks.shape[k + 1], 32, 4, 4).permute(*range(k), k, k + 3, k + 2, k + 1, k + 4)
+    return s.reshape(*lead, chunks.shape[k] * 128, -1)[..., :rows, :blocks]
+
+
+def _check_scale(ts: float, fmt: str) -> None:
+    if fmt != "nvfp4":
+        raise ValueError("tensor_scale belongs to nvfp4")
+    if not (isinstance(ts, (int, float)) and 2.0 ** -100 <= ts <= 2.0 ** 100):
+        raise ValueError(f"tensor_scale is a number in [2^-100, 2^100], got {ts!r}")
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    if torch.cuda.current_device() == device.index:
+        _lib.lib().call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _lib.lib().call(name, *args)
+
+
+def _matrix(x: torch.Tensor, what: str) -> Tuple[int, int, int, int, int]:
+    """(batch, rows, cols, batch stride, row stride) of a tensor whose leading dimensions form one stride."""
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{what} is float32, bfloat16 or float16, got {x.dtype}")
+    if not x.is_cuda:
+        raise ValueError(f"{what} is not on a CUDA device")
+    if x.dim() < 2:
+        raise ValueError(f"{what} has a shape [..., rows, cols], got {tuple(x.shape)}")
+    rows, cols = x.shape[-2:]
+    if cols < 1:
+        raise ValueError(f"{what} has no columns")
+    ld = x.stride(-2) if rows > 1 else cols
+    if (cols > 1 and x.stride(-1) != 1) or ld < cols:
+        raise ValueError(f"{what} has rows of consecutive values that do not overlap, got strides {x.stride()}")
+    if x.dim() == 2:
+        return 1, rows, cols, 0, ld
+    if x.numel() == 0:
+        return 0, rows, cols, 0, ld
+    batch, bs = 1, rows * ld
+    for n, s in zip(reversed(x.shape[:-2]), reversed(x.stride()[:-2])):   # innermost first
+        if n == 1:
+            continue
+        if batch == 1:
+            bs = s
+        elif s != bs * batch:
+            raise ValueError(f"the leading dimensions of {what} have no common stride: {tuple(x.shape)} {x.stride()}")
+        batch *= n
+    return batch, rows, cols, bs, ld
+
+
+def quantize(x: torch.Tensor, fmt: str = "mxfp4", tensor_scale: Optional[float] = None) -> Fp4Tensor:
+    """Quantise ``x`` [..., rows, cols] (f32, bf16 or f16; rows may be strided) along its last dimension."""
+    if fmt not in FORMATS:
+        raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
+    if tensor_scale is not None:
+        _check_scale(tensor_scale, fmt)
+    batch, rows, cols, bs, ld = _matrix(x, "x")
+    g = (cols + 127) // 128
+    codes = torch.empty(*x.shape[:-1], 64 * g, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(*x.shape[:-2], (rows + 127) // 128, g if fmt == "mxfp4" else 2 * g, 512, dtype=torch.uint8, device=x.device)
+    if batch * rows:
+        _call(x.device, "fb_fp4_quantize", x, _DTYPES[x.dtype], ld, bs, codes, scales, batch, rows, cols, FORMATS[fmt],
+              float(tensor_scale or 0.0))
+    return Fp4Tensor(codes, scales, fmt, x.shape, tensor_scale)
+
+
+def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.device, what: str = "out") -> torch.Tensor:
+    if out is None:
+        if dtype not in _DTYPES:
+            raise TypeError(f"{what} is float32, bfloat16 or float16, got {dtype}")
+        return torch.empty(shape, dtype=dtype, device=device)
+    if tuple(out.shape) != tuple(shape) or out.device != device:
+        raise ValueError(f"{what} must be {tuple(shape)} on {device}, got {tuple(out.shape)} on {out.device}")
+    return out
+
+
+def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values of ``q``, rounded once to ``dtype`` (or into ``out``, whose rows may be strided)."""
+    if not q.codes.is_cuda:
+        raise ValueError("q is not on a CUDA device")
+    out = _out(out, q.shape, dtype, q.device)
+    if out.numel():
+        batch, rows, cols, bs, ld = _matrix(out, "out")
+        _call(q.device, "fb_fp4_dequantize", q.codes, q.scales, out, _DTYPES[out.dtype], ld, bs, batch, rows, cols,
+              FORMATS[q.fmt], float(q.tensor_scale or 0.0))
+    return out
+
+
+def _product_out(out, M: int, N: int, dtype, device):
+    out = _out(out, (M, N), dtype, device)
+    _, _, _, _, ldo = _matrix(out, "out") if out.numel() else (0, 0, 0, 0, N)
+    return out, ldo
+
+
+def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x @ w.T`` of two 4-bit matrices [M, K] and [N, K] of one format: products of the values they stand for, summed in
+    f32 and rounded once."""
+    if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"matmul takes [M, K] and [N, K], got {x.shape} and {w.shape}")
+    if x.fmt != w.fmt:
+        raise ValueError(f"matmul takes two tensors of one format, got {x.fmt} and {w.fmt}")
+    if not x.codes.is_cuda or x.device != w.device:
+        raise ValueError(f"matmul takes tensors of one CUDA device, got {x.device} and {w.device}")
+    M, N, K = x.shape[0], w.shape[0], x.shape[1]
+    out, ldo = _product_out(out, M, N, out_dtype, x.device)
+    if M and N:
+        alpha = float(x.tensor_scale or 1.0) * float(w.tensor_scale or 1.0)
+        _call(x.device, "fb_fp4_matmul", x.codes, x.scales, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
+              FORMATS[x.fmt], alpha)
+    return out
+
+
+def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
+           x_scale: Optional[float] = None) -> torch.Tensor:
+    """``quantize(x, w.fmt, x_scale) @ w.T`` for ``x`` [M, K] (f32, bf16, f16) and 4-bit weights [N, K], in one call.
+    ``out_dtype`` defaults to x's."""
+    if x.dim() != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
+        raise ValueError(f"linear takes [M, K] and 4-bit [N, K], got {tuple(x.shape)} and {w.shape}")
+    if x_scale is not None:
+        _check_scale(x_scale, w.fmt)
+    _, M, K, _, ldx = _matrix(x, "x")
+    if x.device != w.device:
+        raise ValueError(f"x is on {x.device}, w on {w.device}")
+    N = w.shape[0]
+    out, ldo = _product_out(out, M, N, out_dtype or x.dtype, x.device)
+    if M and N:
+        g = (K + 127) // 128
+        work = torch.empty((M * 64 * g + 511) // 512 * 512 + (M + 127) // 128 * (g if w.fmt == "mxfp4" else 2 * g) * 512,
+                           dtype=torch.uint8, device=x.device)
+        alpha = float(x_scale or 1.0) * float(w.tensor_scale or 1.0)
+        _call(x.device, "fb_fp4_linear", x, _DTYPES[x.dtype], ldx, work, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
+              FORMATS[w.fmt], float(x_scale or 0.0), alpha)
+    return out
+
+
+def check(device=None) -> None:
+    """Raise ``KernelError`` if a wait inside one of this module's kernels on ``device`` (default: the current one) ran
+    out since the last check.  Waits for the current stream."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    host = (ctypes.c_int * 4)()
+    with torch.cuda.device(dev):
+        _lib.lib().call("fb_fp4_status", ctypes.cast(host, ctypes.POINTER(ctypes.c_int)), 1)
+    if host[0]:
+        raise _lib.KernelError(f"a wait of a 4-bit kernel ran out (block {host[1]}, {host[2]}, {host[3]}): its output is not valid")
+
+
+def reference_dequantize(q: Fp4Tensor) -> torch.Tensor:
+    """The values of ``q`` as f64, in plain torch (CPU or GPU): the statement that the kernels are tested against."""
+    from .quant import e2m1_decode, ue8m0_decode
+    rows, cols = q.shape[-2:]
+    v = e2m1_decode(e2m1_unpack(q.codes)).double()
+    b = BLOCK[q.fmt]
+    s = unpack_scales(q.scales, rows, v.shape[-1] // b)
+    if q.fmt == "mxfp4":
+        f = torch.where(s == 255, torch.full((), math.nan, dtype=torch.float64, device=s.device), ue8m0_decode(s).double())
+        f = torch.where(s == 0, torch.full((), 2.0 ** -127, dtype=torch.float64, device=s.device), f)
+    else:
+        f = s.contiguous().view(torch.float8_e4m3fn).double()
+    return (v.unflatten(-1, (-1, b)) * f.unsqueeze(-1)).flatten(-2)[..., :cols] * (q.tensor_scale or 1.0)

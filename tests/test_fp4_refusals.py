@@ -1,0 +1,92 @@
+"""CPU: what the 4-bit operators refuse, and the layout of their scale chunks."""
+import pytest
+import torch
+
+from ferrite_b200.ops import fp4
+from ferrite_b200.ops import quant as Q
+
+
+def test_scale_chunks_round_trip_and_place():
+    s = torch.randint(0, 255, (3, 200, 7), dtype=torch.uint8)
+    c = fp4.pack_scales(s)
+    assert c.shape == (3, 2, 2, 512)
+    assert torch.equal(fp4.unpack_scales(c, 200, 7), s)
+    for r, b in ((0, 0), (33, 5), (127, 3), (199, 6)):
+        assert c[1, r // 128, b // 4, r % 32 * 16 + r % 128 // 32 * 4 + b % 4] == s[1, r, b]
+
+
+def test_from_rows_is_the_checkpoint_codec():
+    w = torch.randn(130, 192)
+    packed, scale = Q.quant_fp4_weight(w)
+    t = fp4.Fp4Tensor.from_rows(packed, scale)
+    assert t.codes.shape == (130, 128) and (t.codes[:, 96:] == 0).all()
+    assert torch.equal(fp4.reference_dequantize(t).float(), Q.dequant_fp4_weight(packed, scale))
+
+
+def _t(rows=4, cols=64, fmt="mxfp4", lead=()):
+    g = (cols + 127) // 128
+    c = g if fmt == "mxfp4" else 2 * g
+    return fp4.Fp4Tensor(torch.zeros(*lead, rows, 64 * g, dtype=torch.uint8),
+                         torch.zeros(*lead, (rows + 127) // 128, c, 512, dtype=torch.uint8), fmt, (*lead, rows, cols))
+
+
+def test_a_tensor_s_parts_have_to_belong_together():
+    codes, scales = torch.zeros(4, 64, dtype=torch.uint8), torch.zeros(1, 1, 512, dtype=torch.uint8)
+    fp4.Fp4Tensor(codes, scales, "mxfp4", (4, 128))
+    for bad in [(codes, scales, "mxfp8", (4, 128)), (codes, scales, "mxfp4", (4, 129)), (codes, scales, "nvfp4", (4, 128)),
+                (codes, scales, "mxfp4", (128,)), (codes, scales, "mxfp4", (4, 0)), (codes[:3], scales, "mxfp4", (4, 128)),
+                (codes, scales, "mxfp4", (4, 128), 2.0)]:
+        with pytest.raises(ValueError):
+            fp4.Fp4Tensor(*bad)
+    with pytest.raises(TypeError):
+        fp4.Fp4Tensor(codes.int(), scales, "mxfp4", (4, 128))
+    with pytest.raises(ValueError):   # not contiguous
+        fp4.Fp4Tensor(torch.zeros(4, 128, dtype=torch.uint8)[:, ::2], scales, "mxfp4", (4, 128))
+    with pytest.raises(ValueError):   # not aligned
+        fp4.Fp4Tensor(torch.zeros(257, dtype=torch.uint8)[1:].view(4, 64), scales, "mxfp4", (4, 128))
+
+
+def test_refusals_before_any_launch():
+    x = torch.zeros(4, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp4.quantize(x)
+    with pytest.raises(ValueError, match="fmt"):
+        fp4.quantize(x, "int4")
+    with pytest.raises(TypeError):
+        fp4.quantize(x.double())
+    for ts in (0.0, -1.0, float("nan"), float("inf"), 2.0 ** -101, "1"):
+        with pytest.raises(ValueError, match="tensor_scale"):
+            fp4.quantize(x, "nvfp4", tensor_scale=ts)
+    with pytest.raises(ValueError, match="nvfp4"):
+        fp4.quantize(x, "mxfp4", tensor_scale=1.0)
+    with pytest.raises(ValueError, match="CUDA"):
+        fp4.dequantize(_t())
+    with pytest.raises(ValueError, match=r"\[M, K\]"):
+        fp4.matmul(_t(4, 64), _t(4, 96))
+    with pytest.raises(ValueError, match="one format"):
+        fp4.matmul(_t(4, 64), _t(4, 64, "nvfp4"))
+    with pytest.raises(ValueError, match="CUDA"):
+        fp4.matmul(_t(), _t())
+    with pytest.raises(ValueError, match=r"\[M, K\]"):
+        fp4.linear(torch.zeros(2, 4, 64), _t())
+    with pytest.raises(ValueError, match="CUDA"):
+        fp4.linear(x, _t())
+
+
+@pytest.mark.parametrize("x", [torch.zeros(4, 64).t(), torch.zeros(4, 64)[:, ::2], torch.zeros(1, 64).expand(4, 64),
+                               torch.zeros(64), torch.zeros(4, 0)])
+def test_layouts_that_are_refused(x, monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    with pytest.raises(ValueError):
+        fp4._matrix(x, "x")
+
+
+def test_layouts_that_are_taken(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    b = torch.zeros(6, 5, 40, 100)
+    assert fp4._matrix(b, "x") == (30, 40, 100, 4000, 100)
+    assert fp4._matrix(b[:, :, :8, :60], "x") == (30, 8, 60, 4000, 100)
+    assert fp4._matrix(b[2:3, 1:2], "x")[:3] == (1, 40, 100)
+    assert fp4._matrix(b[:, 2], "x") == (6, 40, 100, 20000, 100)
+    with pytest.raises(ValueError, match="common stride"):
+        fp4._matrix(b[:, :3], "x")
