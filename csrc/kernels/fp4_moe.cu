@@ -1,0 +1,693 @@
+// A whole layer of 4-bit experts for a few tokens (1..32) in two kernels.
+//
+//   p = score(logits), chosen = top-k of p + bias (ties to the lower index), w = scale * p / sum(chosen p)
+//   g, u = W13[e] . e4m3(x)                            e4m3(.): power-of-two scale per 32 values
+//   h[e, t] = e4m3(silu(min(g, limit)) * clamp(u, -limit, limit) * w[t, e])
+//   y[t] = sum over chosen e of W2[e] . h[e, t]
+//
+// The layer is bound by streaming the chosen experts' weights (17/32 byte per value) once.  Nothing is dequantised in
+// registers: tcgen05.mma kind::mxf8f6f4.block_scale multiplies e2m1 weights with e4m3 activations and applies both
+// scale vectors; the padded 4-bit form that it wants in shared memory (16 codes in 8 bytes, 8 bytes of gap) is what a TMA
+// box of the 4-bit element type writes, so weight bytes go from HBM to the tensor core without passing a register.
+// The weights are the operand on the 128 lanes, ALL tokens (padded to 16 or 32) are the columns, for every expert that any
+// token chose: columns of tokens that did not choose the expert cost no bytes, and are dropped (gate | up) or zero (down).
+//
+// Kernel 1 (gate_up): persistent clusters of S CTAs.  Every CTA routes all tokens by itself (a warp per token; the logits
+// are a few KB in L2, and a separate routing launch costs more), quantises its K range of x into shared memory once, and
+// walks the (expert, 128 rows of I) tiles of its cluster, each CTA over 1/S of K.  The S partial sums of a 32-row
+// quarter meet in the CTA that owns the quarter (pushed through distributed shared memory, summed in rank order), which
+// applies SwiGLU and quantises: 32 rows of a lane quarter are exactly one block of h.  h is stored in the swizzled
+// operand form, so kernel 2 fetches it with plain bulk copies.
+// Kernel 2 (down): a cluster of S CTAs per 128 rows of the output; the (expert, 128 columns of I) blocks of all chosen
+// experts are one long K axis, split over the cluster, accumulated in ONE accumulator: the sum over experts costs
+// nothing.  Partials are summed in rank order.  No atomics anywhere: the same bits every run.
+// Kernel 2 is launched with programmatic serialisation: it routes again and starts its weight stream while kernel 1
+// drains, and waits only before it reads h.
+#include "fp4_common.cuh"
+
+namespace {
+
+using namespace fp4;
+
+constexpr int kMaxE = 512, kMaxTok = 32, kMaxTopk = 32;
+constexpr int kMThreads = 320;
+
+enum Score : int { kSqrtSoftplus = 0, kSigmoid = 1, kSoftmax = 2 };
+
+struct MoeArgs {
+    const void* x;
+    int64_t ldx;
+    const float *logits, *bias;
+    int64_t ldl;
+    const uint8_t *s13, *s2;
+    void* out;
+    int64_t ldo;
+    uint8_t *h, *hs;          // [active][nit][BN * 128] operand tiles, [active][nit][512] scale chunks
+    float scale, limit;
+    int xdt, odt, accumulate, T, E, topk, D, I, score, norm;
+    int g1, nit, S;           // 128-column groups of D, 128-row tiles of I, cluster size
+    int* status;
+};
+
+struct Route {
+    uint32_t mask[kMaxE];                     // tokens that chose the expert
+    float wt[kMaxTok * kMaxTopk];
+    uint16_t sel[kMaxTok * kMaxTopk];
+    uint16_t act[kMaxE];                      // chosen experts, ascending
+    int n_act;
+};
+
+__device__ __forceinline__ uint32_t order_key(float v) {   // larger float -> larger key; NaN below every number; 0 is free
+    if (v != v) return 1u;
+    const uint32_t u = __float_as_uint(v);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__device__ __forceinline__ float score_of(float z, int score, float mx, float inv_sum) {
+    if (score == kSigmoid) return 1.f / (1.f + expf(-z));
+    if (score == kSoftmax) return expf(z - mx) * inv_sum;
+    return sqrtf(fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
+}
+
+// All tokens' choices into r; the whole block takes part (ends with a block barrier).
+__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    for (int e = threadIdx.x; e < kMaxE; e += blockDim.x) r.mask[e] = 0u;
+    __syncthreads();
+    for (int t = warp; t < a.T; t += nw) {
+        const float* lg = a.logits + t * a.ldl;
+        float z[kMaxE / 32];
+#pragma unroll
+        for (int j = 0; j < kMaxE / 32; ++j) z[j] = lane + 32 * j < a.E ? __ldg(lg + lane + 32 * j) : -INFINITY;
+        float mx = 0.f, inv_sum = 1.f;
+        if (a.score == kSoftmax) {
+            mx = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < kMaxE / 32; ++j) mx = fmaxf(mx, z[j]);
+            mx = warp_max(mx);
+            if (mx == -INFINITY) mx = 0.f;
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < kMaxE / 32; ++j) s += lane + 32 * j < a.E ? expf(z[j] - mx) : 0.f;
+            inv_sum = 1.f / warp_sum(s);
+        }
+        uint32_t key[kMaxE / 32];
+#pragma unroll
+        for (int j = 0; j < kMaxE / 32; ++j) {
+            const int e = lane + 32 * j;
+            // every score grows with its logit: without a bias the logit itself decides, exactly
+            key[j] = e >= a.E ? 0u : order_key(a.bias ? score_of(z[j], a.score, mx, inv_sum) + __ldg(a.bias + e) : z[j]);
+        }
+        int mine = 0;
+        for (int k = 0; k < a.topk; ++k) {
+            uint32_t best = 0;
+            int bj = 0;
+#pragma unroll
+            for (int j = 0; j < kMaxE / 32; ++j)
+                if (key[j] > best) { best = key[j]; bj = j; }
+            const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+            const uint32_t cand = best == top ? (uint32_t)(lane + 32 * bj) : 0xffffffffu;
+            const int e = (int)__reduce_min_sync(0xffffffffu, cand);
+            if (lane == k) mine = e;
+#pragma unroll
+            for (int j = 0; j < kMaxE / 32; ++j)
+                if (e == lane + 32 * j) key[j] = 0u;
+        }
+        float p = lane < a.topk ? score_of(__ldg(lg + mine), a.score, mx, inv_sum) : 0.f;
+        if (a.norm) p = p / (warp_sum(p) + 1e-20f);
+        if (lane < a.topk) {
+            r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
+            r.wt[t * kMaxTopk + lane] = p * a.scale;
+            atomicOr(&r.mask[mine], 1u << t);
+        }
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int n = 0;
+        for (int e0 = 0; e0 < a.E; e0 += 32) {
+            const bool on = e0 + lane < a.E && r.mask[e0 + lane] != 0u;
+            const uint32_t b = __ballot_sync(0xffffffffu, on);
+            if (on) r.act[n + __popc(b & ((1u << lane) - 1u))] = (uint16_t)(e0 + lane);
+            n += __popc(b);
+        }
+        if (lane == 0) r.n_act = n;
+    }
+    __syncthreads();
+}
+
+// kind::mxf8f6f4: A e2m1 (5), B e4m3 (0), ue8m0 scales, M = 128
+__host__ __device__ constexpr uint32_t moe_idesc(int N, int sf) {
+    return ((uint32_t)sf << 4) | (5u << 7) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | ((uint32_t)sf << 29);
+}
+__device__ __forceinline__ void umma_w4a8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, long long budget = 2000000000ll) {
+    const long long t0 = clock64();
+    for (;;) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if (clock64() - t0 > budget) return false;
+    }
+}
+
+template <int BN>
+struct UpCfg {
+    static constexpr int kA = 128 * 128;                       // padded 4-bit tile
+    static constexpr int kStage = 2 * kA + 1024;               // gate, up, their scale chunks
+    static constexpr int kXBlock = BN * 128 + 512;             // one 128-column block of x and its scale chunk
+    static constexpr int kTmem = BN == 16 ? 128 : 256;
+    static constexpr int kAccSet = 2 * BN;                     // gate | up columns of one accumulator set
+    static constexpr int kSf = 2 * kAccSet;                    // scales: 2 x (gate 4, up 4, x 4)
+    static constexpr int kBars = 256;
+};
+// shared memory of kernel 1: x blocks | receive slots | stages | barriers
+template <int BN>
+__host__ __device__ constexpr size_t up_recv_bytes(int S) { return S == 1 ? 0 : (size_t)(S - 1) * (S >= 4 ? 1 : 4 / S) * 2 * BN * 128; }
+template <int BN>
+__host__ __device__ constexpr size_t up_fixed(int nkb, int S) {
+    return ((size_t)nkb * UpCfg<BN>::kXBlock + up_recv_bytes<BN>(S) + 1023) / 1024 * 1024 + 1024 + UpCfg<BN>::kBars;
+}
+
+template <int BN, typename TX>
+__global__ void __launch_bounds__(kMThreads, 1)
+fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_tail, const MoeArgs a, int stages) {
+    using C = UpCfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Route R;
+    __shared__ int s_fail;
+    const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* base_g = smem_raw + (base - tc::smem_u32(smem_raw));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = a.S, rank = S > 1 ? (int)cluster_rank() : 0;
+    const int kb0 = a.g1 * rank / S, kb1 = a.g1 * (rank + 1) / S, nkb = kb1 - kb0;
+    const int nkb_max = (a.g1 + S - 1) / S;
+    const uint32_t xsf_off = (uint32_t)nkb_max * BN * 128;
+    const uint32_t recv_off = (uint32_t)nkb_max * C::kXBlock;
+    const uint32_t st_off = (uint32_t)((recv_off + up_recv_bytes<BN>(S) + 1023) / 1024 * 1024);
+    const uint32_t bars = base + st_off + (uint32_t)stages * C::kStage;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (stages + s); };
+    const uint32_t acc_full = bars + 16u * stages, acc_empty = acc_full + 16u, recv_full = acc_empty + 16u, recv_free = recv_full + 32u,
+                   tmem_slot = recv_free + 32u;
+
+    pdl_wait();
+    pdl_launch();
+    if (threadIdx.x == 0) {
+        s_fail = 0;
+        for (int s = 0; s < stages; ++s) {
+            tc::mbar_init(full(s), 1);
+            tc::mbar_init(empty(s), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(acc_full + 8u * i, 1);
+            tc::mbar_init(acc_empty + 8u * i, 4);
+        }
+        for (int q = 0; q < 4; ++q) {
+            tc::mbar_init(recv_full + 8u * q, S > 1 ? S - 1 : 1);
+            tc::mbar_init(recv_free + 8u * q, 1);
+        }
+        tc::mbar_fence_init();
+        tc::prefetch_tmap(&tmap_w);
+        tc::prefetch_tmap(&tmap_tail);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
+    route_all(a, R);
+    tc::tc_fence_before();
+    if (S > 1) cluster_sync_all(); else __syncthreads();
+    tc::tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+    const int items = R.n_act * a.nit;
+    const int first = blockIdx.x / S, step = gridDim.x / S;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int it = 0;
+            bool ok = true;
+            for (int item = first; item < items && ok; item += step) {
+                const int e = R.act[item / a.nit], j = item % a.nit;
+                const int rows = min(128, a.I - j * 128), boxes = rows == 128 ? 0 : (rows + 31) / 32;
+                const int row_g = (e * 2) * a.I + j * 128, row_u = row_g + a.I;
+                const uint8_t* sg = a.s13 + (((int64_t)e * 2) * a.nit + j) * a.g1 * 512;
+                const uint8_t* su = sg + (int64_t)a.nit * a.g1 * 512;
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int s = it % stages;
+                    if (it >= stages && !tc::mbar_wait(empty(s), ((it / stages) - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                    const uint32_t st = base + st_off + (uint32_t)s * C::kStage;
+                    // the barrier counts the packed bytes: 64 per row of 128 codes
+                    tc::mbar_expect_tx(full(s), 2 * (boxes ? boxes * 32 * 64 : 128 * 64) + 1024);
+                    if (!boxes) {
+                        tc::tma_load_2d(st, &tmap_w, kb * 128, row_g, full(s));
+                        tc::tma_load_2d(st + C::kA, &tmap_w, kb * 128, row_u, full(s));
+                    } else {
+                        for (int b = 0; b < boxes; ++b) {
+                            tc::tma_load_2d(st + b * 32 * 128, &tmap_tail, kb * 128, row_g + 32 * b, full(s));
+                            tc::tma_load_2d(st + C::kA + b * 32 * 128, &tmap_tail, kb * 128, row_u + 32 * b, full(s));
+                        }
+                    }
+                    bulk_load(st + 2 * C::kA, sg + (int64_t)kb * 512, 512, full(s));
+                    bulk_load(st + 2 * C::kA + 512, su + (int64_t)kb * 512, 512, full(s));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- warps 1..9: this CTA's K range of x, quantised, in operand form ----
+        const TX* x = reinterpret_cast<const TX*>(a.x);
+        const bool vec = ((uintptr_t)x & 15) == 0 && a.ldx * (int64_t)sizeof(TX) % 16 == 0;
+        const int per_row = nkb * 16;    // 8-value units
+        const int units = a.T * per_row;
+        const int tid = threadIdx.x - 32;
+        for (int u0 = 0; u0 < units; u0 += kMThreads - 32) {
+            const int u = u0 + tid;
+            const int t = u < units ? u / per_row : 0, c = u < units ? u % per_row : 0;
+            const int col = kb0 * 128 + c * 8;
+            float v[8];
+            load8(x + t * a.ldx + min(col, a.D - 1), u < units ? max(0, min(8, a.D - col)) : 0, vec && u < units, v);
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            if (u < units) {
+                const uint32_t sb = ue8m0_of(m, 1e-4f, kInv448);
+                const float inv = sb == 255u ? 0.f : ue8m0_inv(sb);
+                uint32_t w[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                    w[i] = lo | hi << 16;
+                }
+                if (sb == 255u) w[0] = w[1] = 0u;
+                const int kb = c >> 4, u16 = c & 15;      // 8-byte unit of the 128-byte row
+                *reinterpret_cast<uint2*>(base_g + (size_t)kb * BN * 128 + t * 128 + (((u16 >> 1) ^ (t & 7)) << 4) + (u16 & 1) * 8) = make_uint2(w[0], w[1]);
+                if ((c & 3) == 0) base_g[xsf_off + kb * 512 + t * 16 + (u16 >> 2)] = (uint8_t)sb;
+            }
+        }
+        fence_proxy_async();
+        asm volatile("bar.sync 1, 288;" ::: "memory");
+        if (warp == 1) {
+            if (lane == 0) {
+                int it = 0, no = 0;
+                bool ok = true;
+                for (int item = first; item < items && ok; item += step, ++no) {
+                    const int buf = no & 1;
+                    if (no >= 2 && !tc::mbar_wait(acc_empty + 8u * buf, ((no >> 1) - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                    tc::tc_fence_after();
+                    const uint32_t dg = tmem + (uint32_t)buf * C::kAccSet, du = dg + BN;
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        const int s = it % stages;
+                        if (!tc::mbar_wait(full(s), (it / stages) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                        tc::tc_fence_after();
+                        const uint32_t st = base + st_off + (uint32_t)s * C::kStage;
+                        const uint32_t sf = tmem + C::kSf + (uint32_t)(it & 1) * 12;
+                        tmem_cp_sf(sf, sf_desc(st + 2 * C::kA));
+                        tmem_cp_sf(sf + 4, sf_desc(st + 2 * C::kA + 512));
+                        tmem_cp_sf(sf + 8, sf_desc(base + xsf_off + kb * 512));
+                        const uint64_t gd = tc::umma_desc_sw128(st), ud = tc::umma_desc_sw128(st + C::kA);
+                        const uint64_t xd = tc::umma_desc_sw128(base + (uint32_t)kb * BN * 128);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            umma_w4a8(dg, gd + 2u * k, xd + 2u * k, moe_idesc(BN, k), sf, sf + 8, (kb | k) ? 1u : 0u);
+                            umma_w4a8(du, ud + 2u * k, xd + 2u * k, moe_idesc(BN, k), sf + 4, sf + 8, (kb | k) ? 1u : 0u);
+                        }
+                        tc::umma_commit(empty(s));
+                    }
+                    tc::umma_commit(acc_full + 8u * buf);
+                }
+            }
+            __syncwarp();
+        } else if (warp < 6) {
+            const int q = warp & 3;
+            const int owner = S == 1 ? 0 : S == 2 ? q >> 1 : q;
+            const int slot_q = S == 2 ? q & 1 : 0;            // the owner's slots: its quarters one after the other
+            const uint32_t slots = base + recv_off + (uint32_t)(slot_q * (S - 1)) * 2 * BN * 128;
+            int no = 0;
+            for (int item = first; item < items; item += step, ++no) {
+                const int ai = item / a.nit, j = item % a.nit, buf = no & 1, e = R.act[ai];
+                const bool done = tc::mbar_wait(acc_full + 8u * buf, (no >> 1) & 1, 4000000000ll);
+                tc::tc_fence_after();
+                if (!done) atomicExch(&s_fail, 1);
+                bool go = __shfl_sync(0xffffffffu, (done && *(volatile int*)&s_fail == 0) ? 1 : 0, 0) != 0;
+                float v[2 * BN];
+                if (go) {
+#pragma unroll
+                    for (int c = 0; c < 2 * BN; c += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::kAccSet + c), r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[c + i] = __uint_as_float(r[i]);
+                    }
+                }
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty + 8u * buf);
+                if (!go) break;
+                if (S > 1) {
+                    if (rank != owner) {
+                        if (no && !wait_cluster(recv_free + 8u * q, (no - 1) & 1)) { atomicExch(&s_fail, 1); break; }
+                        const int src = rank < owner ? rank : rank - 1;
+                        const uint32_t dst = map_rank(slots + (uint32_t)src * 2 * BN * 128 + lane * 4, owner);
+#pragma unroll
+                        for (int c = 0; c < 2 * BN; ++c) st_cluster(dst + c * 128, v[c]);
+                        __syncwarp();
+                        if (lane == 0) arrive_cluster(map_rank(recv_full + 8u * q, owner));
+                        continue;
+                    }
+                    if (!wait_cluster(recv_full + 8u * q, no & 1)) { atomicExch(&s_fail, 1); break; }
+#pragma unroll
+                    for (int c = 0; c < 2 * BN; ++c) {
+                        float sum = 0.f;
+                        for (int s = 0; s < S; ++s) {   // rank order
+                            float p = v[c];
+                            if (s != rank)
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p) : "r"(slots + (uint32_t)(s < rank ? s : s - 1) * 2 * BN * 128 + c * 128 + lane * 4) : "memory");
+                            sum = s ? sum + p : p;
+                        }
+                        v[c] = sum;
+                    }
+                    __syncwarp();
+                    if (lane < S && lane != rank) arrive_cluster(map_rank(recv_free + 8u * q, lane));
+                }
+                // SwiGLU and the block quantiser: lane = row of I, this warp's 32 rows are one block
+                const uint32_t mask = R.mask[e];
+                float wv = 0.f;
+                if (lane < a.T)
+                    for (int k = 0; k < a.topk; ++k)
+                        if (R.sel[lane * kMaxTopk + k] == e) wv = R.wt[lane * kMaxTopk + k];
+                const bool real = j * 128 + q * 32 < a.I;
+                const int64_t tile = (int64_t)ai * a.nit + j;
+                uint8_t* ht = a.h + tile * (BN * 128);
+                uint8_t* hs = a.hs + tile * 512;
+                const int c16 = q * 2 + (lane >> 4);
+#pragma unroll
+                for (int t = 0; t < BN; ++t) {
+                    if (t < a.T) {
+                        const float w = __shfl_sync(0xffffffffu, wv, t);
+                        uint32_t byte = 0, sb = 127;
+                        if (real && (mask >> t & 1)) {
+                            const float g = fminf(v[t], a.limit), u = fminf(fmaxf(v[BN + t], -a.limit), a.limit);
+                            // fminf drops a NaN: put it back
+                            const float hv = (v[t] != v[t] || v[BN + t] != v[BN + t]) ? __uint_as_float(0x7fc00000u) : g / (1.f + expf(-g)) * u * w;
+                            const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(hv));
+                            sb = ue8m0_of(m, 1e-4f, kInv448);
+                            byte = sb == 255u ? 0u : __nv_cvt_float_to_fp8(hv * ue8m0_inv(sb), __NV_SATFINITE, __NV_E4M3);
+                        }
+                        ht[t * 128 + ((c16 ^ (t & 7)) << 4) + (lane & 15)] = (uint8_t)byte;
+                        if (lane == 0) hs[t * 16 + q] = (uint8_t)sb;
+                    }
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc::tc_fence_before();
+    if (S > 1) cluster_sync_all(); else __syncthreads();   // no CTA leaves while a peer may still write to it
+    if (threadIdx.x == 0 && s_fail && a.status) { a.status[0] = FB_TIMEOUT; a.status[1] = blockIdx.x; a.status[2] = 1000 + BN; a.status[3] = S; }
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, C::kTmem);
+    }
+}
+
+template <int BN>
+struct DownCfg {
+    static constexpr int kA = 128 * 128;
+    static constexpr int kStage = kA + BN * 128 + 1024;         // weights, h tile, both scale chunks
+    static constexpr int kStages = (104 * 1024 - 1024 - 256) / kStage;   // two CTAs per SM, each with 9 KB of tables
+    static constexpr int kTmem = 64;                            // BN accumulator columns + 2 x 8 of scales
+    static constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 256;
+    static_assert((size_t)BN * 128 * 4 <= (size_t)kStages * kStage && kStages * 16 + 16 <= 256, "smem");
+};
+
+template <int BN, typename TO>
+__global__ void __launch_bounds__(kMThreads, 2)
+fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a) {
+    using C = DownCfg<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Route R;
+    __shared__ int s_fail;
+    const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bars = base + C::kStages * C::kStage;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (C::kStages + s); };
+    const uint32_t acc_full = bars + 16u * C::kStages, tmem_slot = acc_full + 8u;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = a.S, rank = S > 1 ? (int)cluster_rank() : 0;
+    const int tile = blockIdx.x / S, d0 = tile * 128, ntd = (a.D + 127) / 128;
+    pdl_launch();
+    if (threadIdx.x == 0) {
+        s_fail = 0;
+        for (int s = 0; s < C::kStages; ++s) {
+            tc::mbar_init(full(s), 1);
+            tc::mbar_init(empty(s), 1);
+        }
+        tc::mbar_init(acc_full, 1);
+        tc::mbar_fence_init();
+        tc::prefetch_tmap(&tmap_w);
+    }
+    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
+    // the logits were complete before kernel 1 started, the weights are never written: both may be read before the wait
+    route_all(a, R);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    const int64_t units = (int64_t)R.n_act * a.nit;
+    const int u0 = (int)(units * rank / S), u1 = (int)(units * (rank + 1) / S);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto arm_w = [&](int s, int u) {
+                const int ai = u / a.nit, kb = u % a.nit, e = R.act[ai];
+                const uint32_t st = base + (uint32_t)s * C::kStage;
+                tc::mbar_expect_tx(full(s), 128 * 64 + 512 + BN * 128 + 512);
+                tc::tma_load_2d(st, &tmap_w, kb * 128, e * a.D + d0, full(s));
+                bulk_load(st + C::kA + BN * 128, a.s2 + (((int64_t)e * ntd + tile) * a.nit + kb) * 512, 512, full(s));
+            };
+            auto load_h = [&](int s, int u) {
+                const uint32_t st = base + (uint32_t)s * C::kStage;
+                bulk_load(st + C::kA, a.h + (int64_t)u * (BN * 128), BN * 128, full(s));
+                bulk_load(st + C::kA + BN * 128 + 512, a.hs + (int64_t)u * 512, 512, full(s));
+            };
+            const int ahead = min(C::kStages, u1 - u0);
+            for (int i = 0; i < ahead; ++i) arm_w(i, u0 + i);
+            pdl_wait();
+            for (int i = 0; i < ahead; ++i) load_h(i, u0 + i);
+            for (int it = ahead; it < u1 - u0; ++it) {
+                const int s = it % C::kStages;
+                if (!tc::mbar_wait(empty(s), ((it / C::kStages) - 1) & 1)) { atomicExch(&s_fail, 1); break; }
+                arm_w(s, u0 + it);
+                load_h(s, u0 + it);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            for (int it = 0; it < u1 - u0; ++it) {
+                const int s = it % C::kStages;
+                if (!tc::mbar_wait(full(s), (it / C::kStages) & 1)) { atomicExch(&s_fail, 1); break; }
+                tc::tc_fence_after();
+                const uint32_t st = base + (uint32_t)s * C::kStage;
+                const uint32_t sf = tmem + 32 + (uint32_t)(it & 1) * 8;
+                tmem_cp_sf(sf, sf_desc(st + C::kA + BN * 128));
+                tmem_cp_sf(sf + 4, sf_desc(st + C::kA + BN * 128 + 512));
+                const uint64_t wd = tc::umma_desc_sw128(st), hd = tc::umma_desc_sw128(st + C::kA);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    umma_w4a8(tmem, wd + 2u * k, hd + 2u * k, moe_idesc(BN, k), sf, sf + 4, (it | k) ? 1u : 0u);
+                tc::umma_commit(empty(s));
+            }
+            tc::umma_commit(acc_full);
+        }
+    } else if (warp < 6) {
+        const int q = warp & 3;
+        const bool done = tc::mbar_wait(acc_full, 0, 4000000000ll);
+        tc::tc_fence_after();
+        if (!done) atomicExch(&s_fail, 1);
+        const bool go = __shfl_sync(0xffffffffu, (done && *(volatile int*)&s_fail == 0) ? 1 : 0, 0) != 0;
+        if (go) {
+            // the stages are drained: the partial tile [BN][128] goes into them (a rank without blocks has none: zeros)
+#pragma unroll
+            for (int c = 0; c < BN; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + (uint32_t)((c + i) * 128 + q * 32 + lane) * 4), "r"(u1 > u0 ? r[i] : 0u) : "memory");
+            }
+        }
+        tc::tc_fence_before();
+    }
+    __syncwarp();
+    if (S > 1) cluster_sync_all(); else __syncthreads();
+    if (warp >= 2) {
+        int bad = 0;
+        for (int s = 0; s < S; ++s) {
+            int f;
+            asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(f) : "r"(S > 1 ? map_rank(tc::smem_u32(&s_fail), s) : tc::smem_u32(&s_fail)) : "memory");
+            bad |= f;
+        }
+        const int t = threadIdx.x - 64, l = t & 127;
+        TO* out = reinterpret_cast<TO*>(a.out);
+        for (int c = rank * 2 + (t >> 7); c < a.T && !bad; c += 2 * S) {
+            const uint32_t at = base + (uint32_t)(c * 128 + l) * 4;
+            float p[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) p[s] = s < S ? ld_cluster(S > 1 ? map_rank(at, s) : at) : 0.f;
+            float sum = p[0];
+#pragma unroll
+            for (int s = 1; s < 8; ++s) sum += p[s];
+            if (d0 + l < a.D) {
+                TO* o = out + c * a.ldo + d0 + l;
+                if (a.accumulate) sum += to_f32(*o);
+                *o = from_f32<TO>(sum);
+            }
+        }
+    }
+    __syncwarp();
+    if (S > 1) cluster_sync_all(); else __syncthreads();
+    if (threadIdx.x == 0 && s_fail && a.status) { a.status[0] = FB_TIMEOUT; a.status[1] = blockIdx.x; a.status[2] = 2000 + BN; a.status[3] = S; }
+    if (warp == 1) {
+        tc::tc_fence_after();
+        tc::tmem_dealloc(tmem, C::kTmem);
+    }
+}
+
+// Tensor map of 4-bit codes [rows][cols] (cols a multiple of 128), boxes of 128 codes x box_rows in the padded form.
+int make_tmap_u4(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeFn fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || !p)
+            return (int)cudaErrorNotSupported;
+        fn = (EncodeFn)p;
+    }
+    if (((uintptr_t)base & 31) || cols % 128) return (int)cudaErrorInvalidValue;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {cols / 2};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(base), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
+constexpr int kSms = 148;
+constexpr size_t kSmemMax = 227 * 1024 - 16 * 1024;   // dynamic part: the routing tables are static
+
+template <int BN>
+int pick_up_cluster(int g1, int64_t items, int* stages) {
+    // Rounds of the persistent clusters times the share of K that a CTA takes, over the cluster sizes whose x blocks leave
+    // room for three stages; with fewer than four (66 KB of weights in flight per SM) the stream is slower.  The smallest
+    // cluster among near equals.
+    int best = 0;
+    double cost = 0;
+    for (int S = 1; S <= 8 && S <= g1; S *= 2) {
+        const size_t fixed = up_fixed<BN>((g1 + S - 1) / S, S);
+        if (fixed + 3 * (size_t)UpCfg<BN>::kStage > kSmemMax) continue;
+        const int n = (int)((kSmemMax - fixed) / UpCfg<BN>::kStage);
+        const int64_t nc = kSms / S;
+        const double c = (double)((items + nc - 1) / nc) * ((g1 + S - 1) / S) * (n < 4 ? 1.15 : 1.0);
+        if (!best || c < cost * 0.97) { best = S; cost = c; *stages = n > 8 ? 8 : n; }
+    }
+    return best;
+}
+
+template <int BN, typename TX>
+int launch_up(MoeArgs a, const void* w13, cudaStream_t st) {
+    CUtensorMap tw, tt;
+    int rc = make_tmap_u4(&tw, w13, (uint64_t)a.E * 2 * a.I, (uint64_t)a.g1 * 128, 128);
+    if (!rc) rc = make_tmap_u4(&tt, w13, (uint64_t)a.E * 2 * a.I, (uint64_t)a.g1 * 128, 32);
+    if (rc) return rc;
+    int stages = 0;
+    const int64_t pairs = (int64_t)a.T * a.topk, items = (pairs < a.E ? pairs : a.E) * a.nit;
+    a.S = pick_up_cluster<BN>(a.g1, items, &stages);
+    if (!a.S) return (int)cudaErrorInvalidValue;
+    const size_t smem = up_fixed<BN>((a.g1 + a.S - 1) / a.S, a.S) + (size_t)stages * UpCfg<BN>::kStage;
+    auto k = fp4_moe_up_kernel<BN, TX>;
+    static unsigned long long allowed = 0;
+    cudaError_t e = fp4_allow_smem(k, kSmemMax, allowed);
+    if (e != cudaSuccess) return (int)e;
+    int64_t nc = kSms / a.S;
+    if (items < nc) nc = items;
+    return (int)fp4_launch(k, dim3((unsigned)(nc * a.S)), dim3(kMThreads), smem, st, a.S, g_fb_pdl != 0, tw, tt, a, stages);
+}
+
+template <int BN, typename TO>
+int launch_down(MoeArgs a, const void* w2, cudaStream_t st) {
+    CUtensorMap tw;
+    const int rc = make_tmap_u4(&tw, w2, (uint64_t)a.E * a.D, (uint64_t)a.nit * 128, 128);
+    if (rc) return rc;
+    auto k = fp4_moe_down_kernel<BN, TO>;
+    static unsigned long long allowed = 0;
+    cudaError_t e = fp4_allow_smem(k, DownCfg<BN>::kSmem, allowed);
+    if (e != cudaSuccess) return (int)e;
+    const int tiles = (a.D + 127) / 128;
+    const int64_t pairs = (int64_t)a.T * a.topk, units = (pairs < a.E ? pairs : a.E) * a.nit;
+    // two CTAs per SM: as many K splits as fill them, with a few blocks each
+    int S = 2 * kSms / tiles;
+    S = S > 8 ? 8 : S < 1 ? 1 : S;
+    while (S > 1 && units < 2 * S) --S;
+    a.S = S;
+    return (int)fp4_launch(k, dim3((unsigned)(tiles * S)), dim3(kMThreads), DownCfg<BN>::kSmem, st, S, true, tw, a);
+}
+
+template <int BN>
+int moe_bn(const MoeArgs& a, const void* w13, const void* w2, cudaStream_t st) {
+    int rc = a.xdt == kF32 ? launch_up<BN, float>(a, w13, st) : a.xdt == kBf16 ? launch_up<BN, __nv_bfloat16>(a, w13, st)
+                                                                              : launch_up<BN, __half>(a, w13, st);
+    if (rc) return rc;
+    return a.odt == kF32 ? launch_down<BN, float>(a, w2, st) : a.odt == kBf16 ? launch_down<BN, __nv_bfloat16>(a, w2, st)
+                                                                             : launch_down<BN, __half>(a, w2, st);
+}
+
+}  // namespace
+
+// x [T, D] (dtype xdt, row stride ldx), logits f32 [T, E] (row stride ldl), bias f32 [E] or null; w13 codes / s13 scales of
+// [E, 2, I, D] mxfp4 (gate, up), w2 / s2 of [E, D, I]; out [T, D] (dtype odt, row stride ldo; accumulate: added to);
+// score 0 sqrt(softplus), 1 sigmoid, 2 softmax; norm: the chosen scores are divided by their sum; limit: SwiGLU clamp
+// (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: min(E, T topk) ceil(I / 128) (BN 128 + 512)
+// bytes, BN = 16 up to 16 tokens, else 32.
+FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logits, int64_t ldl, const float* bias, const void* w13,
+                      const void* s13, const void* w2, const void* s2, void* out, int64_t odt, int64_t ldo, int64_t accumulate,
+                      void* work, int64_t T, int64_t E, int64_t topk, int64_t D, int64_t I, int64_t score, int64_t norm, float scale,
+                      float limit, cudaStream_t st) {
+    if (T < 1 || T > kMaxTok || E < 1 || E > kMaxE || topk < 1 || topk > kMaxTopk || topk > E || D < 1 || I < 32 || I % 32 || ldx < D ||
+        ldo < D || ldl < E || score < 0 || score > 2 || xdt < 0 || xdt > 2 || odt < 0 || odt > 2 || E * 2 * I > 0x7fffff00ll ||
+        E * D > 0x7fffff00ll || D > 0x3fffff || (((uintptr_t)w13 | (uintptr_t)w2) & 31) ||
+        (((uintptr_t)s13 | (uintptr_t)s2 | (uintptr_t)work) & 15))
+        return (int)cudaErrorInvalidValue;
+    MoeArgs a = {};
+    a.x = x; a.ldx = ldx; a.logits = logits; a.bias = bias; a.ldl = ldl;
+    a.s13 = (const uint8_t*)s13; a.s2 = (const uint8_t*)s2; a.out = out; a.ldo = ldo;
+    a.scale = scale; a.limit = limit; a.xdt = (int)xdt; a.odt = (int)odt; a.accumulate = accumulate != 0;
+    a.T = (int)T; a.E = (int)E; a.topk = (int)topk; a.D = (int)D; a.I = (int)I; a.score = (int)score; a.norm = norm != 0;
+    a.g1 = (int)groups(D); a.nit = (int)((I + 127) / 128);
+    a.status = fp4_status_ptr();
+    if (!a.status) return (int)cudaErrorNotSupported;
+    const int64_t bn = T <= 16 ? 16 : 32, pairs = T * topk < E ? T * topk : E;
+    a.hs = (uint8_t*)work;                       // scale chunks, then operand tiles: both 16-byte aligned
+    a.h = a.hs + pairs * a.nit * 512;
+    return bn == 16 ? moe_bn<16>(a, w13, w2, st) : moe_bn<32>(a, w13, w2, st);
+}

@@ -1,5 +1,5 @@
-"""Block-scaled 4-bit matrices on the device: quantiser, expander and products
-(``csrc/kernels/fp4.cu``, ``fp4_gemm.cu``).
+"""Block-scaled 4-bit matrices on the device: quantiser, expander, products and an expert layer for a few tokens
+(``csrc/kernels/fp4.cu``, ``fp4_gemm.cu``, ``fp4_moe.cu``).
 
 A value is an e2m1 code times the scale of its block of consecutive columns:
 
@@ -232,6 +232,63 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
         alpha = float(x_scale or 1.0) * float(w.tensor_scale or 1.0)
         _call(x.device, "fb_fp4_linear", x, _DTYPES[x.dtype], ldx, work, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
               FORMATS[w.fmt], float(x_scale or 0.0), alpha)
+    return out
+
+
+SCORES = {"sqrtsoftplus": 0, "sigmoid": 1, "softmax": 2}
+MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOPK, MOE_MAX_DIM = 32, 512, 32, 8192
+
+
+def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, topk: int, *, bias: Optional[torch.Tensor] = None,
+        score: str = "sqrtsoftplus", norm: bool = True, scale: float = 1.0, limit: float = 0.0,
+        out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+    """The routed experts of a layer for up to 32 tokens, in two kernels.
+
+    ``x`` [T, D] (f32, bf16, f16), ``logits`` [T, E] f32 of the router, ``w13`` mxfp4 [E, 2, I, D] (gate, up), ``w2`` mxfp4
+    [E, D, I] (I a multiple of 32).  Every token takes the ``topk`` experts of largest ``score(logits) + bias`` (ties and
+    equal logits to the lower index; NaN below every number; without a bias the logits decide), weighted by
+    ``scale * score``, with ``norm`` divided by the sum of the chosen scores.  Activations meet the weights as e4m3 with a
+    power-of-two scale per 32 values (``ops/quant.py::fp8_act_roundtrip``): x before the gate and up products, and
+    ``silu(min(g, limit)) * clamp(u, -limit, limit) * weight`` before the down product (``limit`` 0: no clamp).  The
+    result, summed in f32, is rounded once to ``out_dtype`` (default: x's) or, with ``accumulate``, added to ``out``."""
+    if score not in SCORES:
+        raise ValueError(f"score must be one of {sorted(SCORES)}, got {score!r}")
+    if w13.fmt != "mxfp4" or w2.fmt != "mxfp4":
+        raise ValueError("moe takes mxfp4 experts")
+    if len(w13.shape) != 4 or w13.shape[1] != 2 or len(w2.shape) != 3:
+        raise ValueError(f"moe takes w13 [E, 2, I, D] and w2 [E, D, I], got {w13.shape} and {w2.shape}")
+    E, _, I, D = w13.shape
+    if w2.shape != (E, D, I):
+        raise ValueError(f"w13 {w13.shape} asks for w2 {(E, D, I)}, got {w2.shape}")
+    if I % 32 or I < 32:
+        raise ValueError(f"moe takes experts of a multiple of 32 columns, got {I}")
+    if x.dim() != 2 or x.shape[1] != D:
+        raise ValueError(f"x must be [T, {D}], got {tuple(x.shape)}")
+    T = x.shape[0]
+    if T > MOE_MAX_TOKENS or not 1 <= E <= MOE_MAX_EXPERTS or not 1 <= topk <= min(E, MOE_MAX_TOPK):
+        raise ValueError(f"moe takes up to {MOE_MAX_TOKENS} tokens, {MOE_MAX_EXPERTS} experts and topk {MOE_MAX_TOPK}, "
+                         f"got {T}, {E}, {topk}")
+    if D > MOE_MAX_DIM:
+        raise ValueError(f"moe takes rows of up to {MOE_MAX_DIM} values, got {D}")
+    if not (limit >= 0.0) or not math.isfinite(scale):
+        raise ValueError(f"limit must not be negative and scale must be finite, got {limit}, {scale}")
+    if logits.dtype != torch.float32 or tuple(logits.shape) != (T, E) or (E > 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < E):
+        raise ValueError(f"logits must be f32 {(T, E)} with rows of consecutive values, got {logits.dtype} {tuple(logits.shape)} {logits.stride()}")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be contiguous f32 {(E,)}, got {bias.dtype} {tuple(bias.shape)}")
+    if accumulate and out is None:
+        raise ValueError("accumulate needs out")
+    dev = w13.device
+    if any(t is not None and t.device != dev for t in (x, logits, bias, w2.codes)):
+        raise ValueError("moe takes tensors of one device")
+    _, _, _, _, ldx = _matrix(x, "x")
+    out, ldo = _product_out(out, T, D, out_dtype or x.dtype, dev)
+    if T:
+        nit = (I + 127) // 128
+        work = torch.empty(min(E, T * topk) * nit * ((16 if T <= 16 else 32) * 128 + 512), dtype=torch.uint8, device=dev)
+        _call(dev, "fb_fp4_moe", x, _DTYPES[x.dtype], ldx, logits, logits.stride(0) if T > 1 else E, bias, w13.codes, w13.scales,
+              w2.codes, w2.scales, out, _DTYPES[out.dtype], ldo, int(accumulate), work, T, E, topk, D, I, SCORES[score], int(norm),
+              float(scale), float(limit) if limit else math.inf)
     return out
 
 

@@ -90,3 +90,43 @@ def test_layouts_that_are_taken(monkeypatch):
     assert fp4._matrix(b[:, 2], "x") == (6, 40, 100, 20000, 100)
     with pytest.raises(ValueError, match="common stride"):
         fp4._matrix(b[:, :3], "x")
+
+
+def _moe_args(T=2, E=4, I=64, D=128):
+    return [torch.zeros(T, D), torch.zeros(T, E), _t(I, D, lead=(E, 2)), _t(D, I, lead=(E,)), 2]
+
+
+@pytest.mark.parametrize("change,match", [
+    (lambda a, k: k.update(score="tanh"), "score"),
+    (lambda a, k: a.__setitem__(2, _t(64, 128, "nvfp4", (4, 2))), "mxfp4"),
+    (lambda a, k: a.__setitem__(2, _t(64, 128, lead=(4,))), "w13"),
+    (lambda a, k: a.__setitem__(3, _t(64, 128, lead=(4,))), "w2"),
+    (lambda a, k: a.__setitem__(0, torch.zeros(2, 127)), r"\[T, 128\]"),
+    (lambda a, k: a.__setitem__(4, 5), "topk"),
+    (lambda a, k: a.__setitem__(4, 0), "topk"),
+    (lambda a, k: a.__setitem__(1, torch.zeros(2, 5)), "logits"),
+    (lambda a, k: a.__setitem__(1, torch.zeros(2, 4).bfloat16()), "logits"),
+    (lambda a, k: a.__setitem__(1, torch.zeros(4, 2).t()), "logits"),
+    (lambda a, k: k.update(bias=torch.zeros(3)), "bias"),
+    (lambda a, k: k.update(limit=-1.0), "limit"),
+    (lambda a, k: k.update(limit=float("nan")), "limit"),
+    (lambda a, k: k.update(scale=float("inf")), "scale"),
+    (lambda a, k: k.update(accumulate=True), "out"),
+    (lambda a, k: None, "CUDA"),
+])
+def test_moe_refusals(change, match):
+    a, k = _moe_args(), {}
+    change(a, k)
+    with pytest.raises(ValueError, match=match):
+        fp4.moe(*a, **k)
+
+
+def test_moe_limits():
+    with pytest.raises(ValueError, match="32 tokens"):
+        fp4.moe(*_moe_args(T=33))
+    with pytest.raises(ValueError, match="multiple of 32"):
+        fp4.moe(*_moe_args(I=48))
+    with pytest.raises(ValueError, match="512 experts"):
+        fp4.moe(*_moe_args(E=513, I=32, D=32))
+    with pytest.raises(ValueError, match="up to 8192"):
+        fp4.moe(*_moe_args(E=2, I=32, D=8193))
