@@ -23,6 +23,7 @@
 // nothing.  Partials are summed in rank order.  No atomics anywhere: the same bits every run.
 // Kernel 2 is launched with programmatic serialisation: it routes again and starts its weight stream while kernel 1
 // drains, and waits only before it reads h.
+#include <stdlib.h>
 #include "fp4_common.cuh"
 
 namespace {
@@ -42,7 +43,7 @@ struct MoeArgs {
     const uint8_t *s13, *s2;
     void* out;
     int64_t ldo;
-    uint8_t *h, *hs;          // [active][nit][BN * 128] operand tiles, [active][nit][512] scale chunks
+    uint8_t *h, *hs;          // [active][nit][BN * 128] operand tiles, [active][nit][512] their scale chunks
     float scale, limit;
     int xdt, odt, accumulate, T, E, topk, D, I, score, norm;
     int g1, nit, S;           // 128-column groups of D, 128-row tiles of I, cluster size
@@ -54,6 +55,7 @@ struct Route {
     float wt[kMaxTok * kMaxTopk];
     uint16_t sel[kMaxTok * kMaxTopk];
     uint16_t act[kMaxE];                      // chosen experts, ascending
+    float mx[kMaxTok], inv[kMaxTok];          // softmax: largest logit, 1 / sum
     int n_act;
 };
 
@@ -69,36 +71,46 @@ __device__ __forceinline__ float score_of(float z, int score, float mx, float in
     return sqrtf(fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
 }
 
-// All tokens' choices into r; the whole block takes part (ends with a block barrier).
-__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    for (int e = threadIdx.x; e < kMaxE; e += blockDim.x) r.mask[e] = 0u;
-    __syncthreads();
-    for (int t = warp; t < a.T; t += nw) {
-        const float* lg = a.logits + t * a.ldl;
-        float z[kMaxE / 32];
-#pragma unroll
-        for (int j = 0; j < kMaxE / 32; ++j) z[j] = lane + 32 * j < a.E ? __ldg(lg + lane + 32 * j) : -INFINITY;
-        float mx = 0.f, inv_sum = 1.f;
-        if (a.score == kSoftmax) {
-            mx = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < kMaxE / 32; ++j) mx = fmaxf(mx, z[j]);
+// All tokens' choices into r, by the first `nthreads` threads of the block (barrier 2 among them; no barrier at the end).
+// keys: T * E words of scratch.
+// Everything here is a rolled loop: the code runs once per CTA, and straight-line code that runs once costs its
+// instruction fetches (a version unrolled over the 16 scores of a lane took 30 us, this one about 3).
+__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, uint32_t* keys, const int nthreads) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = nthreads >> 5;
+    auto sync = [&]() { asm volatile("bar.sync 2, %0;" ::"r"(nthreads) : "memory"); };
+    for (int e = threadIdx.x; e < kMaxE; e += nthreads) r.mask[e] = 0u;
+    if (a.score == kSoftmax) {
+        for (int t = warp; t < a.T; t += nw) {
+            const float* lg = a.logits + t * a.ldl;
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll 1
+            for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, __ldg(lg + e));
             mx = warp_max(mx);
             if (mx == -INFINITY) mx = 0.f;
-            float s = 0.f;
-#pragma unroll
-            for (int j = 0; j < kMaxE / 32; ++j) s += lane + 32 * j < a.E ? expf(z[j] - mx) : 0.f;
-            inv_sum = 1.f / warp_sum(s);
+#pragma unroll 1
+            for (int e = lane; e < a.E; e += 32) sum += expf(__ldg(lg + e) - mx);
+            sum = warp_sum(sum);
+            if (lane == 0) { r.mx[t] = mx; r.inv[t] = 1.f / sum; }
         }
+        sync();
+    }
+    const int total = a.T * a.E;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < total; i += nthreads) {
+        const int t = i / a.E, e = i - t * a.E;
+        const float z = __ldg(a.logits + t * a.ldl + e);
+        // every score grows with its logit: without a bias the logit itself decides, exactly
+        keys[i] = order_key(a.bias ? score_of(z, a.score, r.mx[t], r.inv[t]) + __ldg(a.bias + e) : z);
+    }
+    sync();
+#pragma unroll 1
+    for (int t = warp; t < a.T; t += nw) {
+        const float* lg = a.logits + t * a.ldl;
         uint32_t key[kMaxE / 32];
 #pragma unroll
-        for (int j = 0; j < kMaxE / 32; ++j) {
-            const int e = lane + 32 * j;
-            // every score grows with its logit: without a bias the logit itself decides, exactly
-            key[j] = e >= a.E ? 0u : order_key(a.bias ? score_of(z[j], a.score, mx, inv_sum) + __ldg(a.bias + e) : z[j]);
-        }
+        for (int j = 0; j < kMaxE / 32; ++j) key[j] = lane + 32 * j < a.E ? keys[t * a.E + lane + 32 * j] : 0u;
         int mine = 0;
+#pragma unroll 1
         for (int k = 0; k < a.topk; ++k) {
             uint32_t best = 0;
             int bj = 0;
@@ -113,7 +125,7 @@ __device__ __forceinline__ void route_all(const MoeArgs& a, Route& r) {
             for (int j = 0; j < kMaxE / 32; ++j)
                 if (e == lane + 32 * j) key[j] = 0u;
         }
-        float p = lane < a.topk ? score_of(__ldg(lg + mine), a.score, mx, inv_sum) : 0.f;
+        float p = lane < a.topk ? score_of(__ldg(lg + mine), a.score, r.mx[t], r.inv[t]) : 0.f;
         if (a.norm) p = p / (warp_sum(p) + 1e-20f);
         if (lane < a.topk) {
             r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
@@ -121,9 +133,10 @@ __device__ __forceinline__ void route_all(const MoeArgs& a, Route& r) {
             atomicOr(&r.mask[mine], 1u << t);
         }
     }
-    __syncthreads();
+    sync();
     if (warp == 0) {
         int n = 0;
+#pragma unroll 1
         for (int e0 = 0; e0 < a.E; e0 += 32) {
             const bool on = e0 + lane < a.E && r.mask[e0 + lane] != 0u;
             const uint32_t b = __ballot_sync(0xffffffffu, on);
@@ -132,7 +145,7 @@ __device__ __forceinline__ void route_all(const MoeArgs& a, Route& r) {
         }
         if (lane == 0) r.n_act = n;
     }
-    __syncthreads();
+    fence_proxy_async();   // the scratch becomes the target of TMA copies
 }
 
 // kind::mxf8f6f4: A e2m1 (5), B e4m3 (0), ue8m0 scales, M = 128
@@ -144,6 +157,12 @@ __device__ __forceinline__ void umma_w4a8(uint32_t d, uint64_t a, uint64_t b, ui
                  " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
 }
+__device__ __forceinline__ void tmem_ld1(uint32_t taddr, float& v) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(v) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_ld4(uint32_t taddr, float (&v)[4]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(taddr) : "memory");
+}
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) {
     asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
@@ -154,7 +173,7 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, long
     const long long t0 = clock64();
     for (;;) {
         uint32_t ok;
-        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
         if (clock64() - t0 > budget) return false;
@@ -163,21 +182,27 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, long
 
 template <int BN>
 struct UpCfg {
-    static constexpr int kA = 128 * 128;                       // padded 4-bit tile
-    static constexpr int kStage = 2 * kA + 1024;               // gate, up, their scale chunks
-    static constexpr int kXBlock = BN * 128 + 512;             // one 128-column block of x and its scale chunk
-    static constexpr int kTmem = BN == 16 ? 128 : 256;
+    static constexpr int kA = 128 * 128;                       // padded 4-bit tile: one matrix, 128 columns
+    static constexpr int kStage = kA + 512;                    // and its scale chunk (kept apart: tiles start on 1024 bytes)
     static constexpr int kAccSet = 2 * BN;                     // gate | up columns of one accumulator set
-    static constexpr int kSf = 2 * kAccSet;                    // scales: 2 x (gate 4, up 4, x 4)
-    static constexpr int kBars = 256;
+    static constexpr int kSfW = 2 * kAccSet, kSfX = kSfW + 8;  // scales: 2 x 4 columns of weights, 4 per block of x (an
+                                                               // MMA takes its scales from a multiple of four columns)
+    static constexpr int kTmem = 512;
+    static constexpr int kBars = 512;
+    static constexpr int kMaxKb = 64;                          // 128-column blocks of x per CTA
+    static_assert(kSfX + 4 * kMaxKb <= kTmem, "tensor memory");
 };
-// shared memory of kernel 1: x blocks | receive slots | stages | barriers
+constexpr int kRouteThreads = 160;   // of kernel 1: the others quantise x meanwhile
+
+// Shared memory of kernel 1: x blocks | their scale chunks | receive slots | stages | stage scales | barriers
 template <int BN>
 __host__ __device__ constexpr size_t up_recv_bytes(int S) { return S == 1 ? 0 : (size_t)(S - 1) * (S >= 4 ? 1 : 4 / S) * 2 * BN * 128; }
 template <int BN>
-__host__ __device__ constexpr size_t up_fixed(int nkb, int S) {
-    return ((size_t)nkb * UpCfg<BN>::kXBlock + up_recv_bytes<BN>(S) + 1023) / 1024 * 1024 + 1024 + UpCfg<BN>::kBars;
+__host__ __device__ constexpr size_t up_front(int nkb, int S) {
+    return ((size_t)nkb * (BN * 128 + 512) + up_recv_bytes<BN>(S) + 1023) / 1024 * 1024;
 }
+template <int BN>
+__host__ __device__ constexpr size_t up_fixed(int nkb, int S) { return up_front<BN>(nkb, S) + 1024 + UpCfg<BN>::kBars; }
 
 template <int BN, typename TX>
 __global__ void __launch_bounds__(kMThreads, 1)
@@ -193,9 +218,10 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const int kb0 = a.g1 * rank / S, kb1 = a.g1 * (rank + 1) / S, nkb = kb1 - kb0;
     const int nkb_max = (a.g1 + S - 1) / S;
     const uint32_t xsf_off = (uint32_t)nkb_max * BN * 128;
-    const uint32_t recv_off = (uint32_t)nkb_max * C::kXBlock;
-    const uint32_t st_off = (uint32_t)((recv_off + up_recv_bytes<BN>(S) + 1023) / 1024 * 1024);
-    const uint32_t bars = base + st_off + (uint32_t)stages * C::kStage;
+    const uint32_t recv_off = xsf_off + (uint32_t)nkb_max * 512;
+    const uint32_t st_off = (uint32_t)up_front<BN>(nkb_max, S);
+    const uint32_t sf_off = st_off + (uint32_t)stages * C::kA;
+    const uint32_t bars = base + sf_off + (uint32_t)stages * 512;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (stages + s); };
     const uint32_t acc_full = bars + 16u * stages, acc_empty = acc_full + 16u, recv_full = acc_empty + 16u, recv_free = recv_full + 32u,
@@ -203,76 +229,41 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
 
     pdl_wait();
     pdl_launch();
-    if (threadIdx.x == 0) {
-        s_fail = 0;
-        for (int s = 0; s < stages; ++s) {
-            tc::mbar_init(full(s), 1);
-            tc::mbar_init(empty(s), 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(acc_full + 8u * i, 1);
-            tc::mbar_init(acc_empty + 8u * i, 4);
-        }
-        for (int q = 0; q < 4; ++q) {
-            tc::mbar_init(recv_full + 8u * q, S > 1 ? S - 1 : 1);
-            tc::mbar_init(recv_free + 8u * q, 1);
-        }
-        tc::mbar_fence_init();
-        tc::prefetch_tmap(&tmap_w);
-        tc::prefetch_tmap(&tmap_tail);
-    }
-    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
-    route_all(a, R);
-    tc::tc_fence_before();
-    if (S > 1) cluster_sync_all(); else __syncthreads();
-    tc::tc_fence_after();
-    uint32_t tmem;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
-
-    const int items = R.n_act * a.nit;
-    const int first = blockIdx.x / S, step = gridDim.x / S;
-
-    if (warp == 0) {
+    if (warp == 9) {
         if (lane == 0) {
-            int it = 0;
-            bool ok = true;
-            for (int item = first; item < items && ok; item += step) {
-                const int e = R.act[item / a.nit], j = item % a.nit;
-                const int rows = min(128, a.I - j * 128), boxes = rows == 128 ? 0 : (rows + 31) / 32;
-                const int row_g = (e * 2) * a.I + j * 128, row_u = row_g + a.I;
-                const uint8_t* sg = a.s13 + (((int64_t)e * 2) * a.nit + j) * a.g1 * 512;
-                const uint8_t* su = sg + (int64_t)a.nit * a.g1 * 512;
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % stages;
-                    if (it >= stages && !tc::mbar_wait(empty(s), ((it / stages) - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
-                    const uint32_t st = base + st_off + (uint32_t)s * C::kStage;
-                    // the barrier counts the packed bytes: 64 per row of 128 codes
-                    tc::mbar_expect_tx(full(s), 2 * (boxes ? boxes * 32 * 64 : 128 * 64) + 1024);
-                    if (!boxes) {
-                        tc::tma_load_2d(st, &tmap_w, kb * 128, row_g, full(s));
-                        tc::tma_load_2d(st + C::kA, &tmap_w, kb * 128, row_u, full(s));
-                    } else {
-                        for (int b = 0; b < boxes; ++b) {
-                            tc::tma_load_2d(st + b * 32 * 128, &tmap_tail, kb * 128, row_g + 32 * b, full(s));
-                            tc::tma_load_2d(st + C::kA + b * 32 * 128, &tmap_tail, kb * 128, row_u + 32 * b, full(s));
-                        }
-                    }
-                    bulk_load(st + 2 * C::kA, sg + (int64_t)kb * 512, 512, full(s));
-                    bulk_load(st + 2 * C::kA + 512, su + (int64_t)kb * 512, 512, full(s));
-                }
+            s_fail = 0;
+            for (int s = 0; s < stages; ++s) {
+                tc::mbar_init(full(s), 1);
+                tc::mbar_init(empty(s), 1);
             }
+            for (int i = 0; i < 2; ++i) {
+                tc::mbar_init(acc_full + 8u * i, 1);
+                tc::mbar_init(acc_empty + 8u * i, 4);
+            }
+            for (int q = 0; q < 4; ++q) {
+                tc::mbar_init(recv_full + 8u * q, S > 1 ? S - 1 : 1);
+                tc::mbar_init(recv_free + 8u * q, 1);
+            }
+            tc::mbar_fence_init();
+            tc::prefetch_tmap(&tmap_w);
+            tc::prefetch_tmap(&tmap_tail);
         }
         __syncwarp();
+        tc::tmem_alloc(tmem_slot, C::kTmem);
+    }
+    if (threadIdx.x < kRouteThreads) {
+        route_all(a, R, reinterpret_cast<uint32_t*>(base_g + st_off), kRouteThreads);
     } else {
-        // ---- warps 1..9: this CTA's K range of x, quantised, in operand form ----
+        // ---- this CTA's K range of x, quantised, in operand form ----
         const TX* x = reinterpret_cast<const TX*>(a.x);
         const bool vec = ((uintptr_t)x & 15) == 0 && a.ldx * (int64_t)sizeof(TX) % 16 == 0;
         const int per_row = nkb * 16;    // 8-value units
         const int units = a.T * per_row;
-        const int tid = threadIdx.x - 32;
-        for (int u0 = 0; u0 < units; u0 += kMThreads - 32) {
+        const int tid = threadIdx.x - kRouteThreads;
+#pragma unroll 1
+        for (int u0 = 0; u0 < units; u0 += kMThreads - kRouteThreads) {
             const int u = u0 + tid;
-            const int t = u < units ? u / per_row : 0, c = u < units ? u % per_row : 0;
+            const int t = u < units ? u / per_row : 0, c = u < units ? u - t * per_row : 0;
             const int col = kb0 * 128 + c * 8;
             float v[8];
             load8(x + t * a.ldx + min(col, a.D - 1), u < units ? max(0, min(8, a.D - col)) : 0, vec && u < units, v);
@@ -298,120 +289,163 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             }
         }
         fence_proxy_async();
-        asm volatile("bar.sync 1, 288;" ::: "memory");
-        if (warp == 1) {
-            if (lane == 0) {
-                int it = 0, no = 0;
-                bool ok = true;
-                for (int item = first; item < items && ok; item += step, ++no) {
-                    const int buf = no & 1;
-                    if (no >= 2 && !tc::mbar_wait(acc_empty + 8u * buf, ((no >> 1) - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
-                    tc::tc_fence_after();
-                    const uint32_t dg = tmem + (uint32_t)buf * C::kAccSet, du = dg + BN;
-                    for (int kb = 0; kb < nkb; ++kb, ++it) {
-                        const int s = it % stages;
-                        if (!tc::mbar_wait(full(s), (it / stages) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
-                        tc::tc_fence_after();
-                        const uint32_t st = base + st_off + (uint32_t)s * C::kStage;
-                        const uint32_t sf = tmem + C::kSf + (uint32_t)(it & 1) * 12;
-                        tmem_cp_sf(sf, sf_desc(st + 2 * C::kA));
-                        tmem_cp_sf(sf + 4, sf_desc(st + 2 * C::kA + 512));
-                        tmem_cp_sf(sf + 8, sf_desc(base + xsf_off + kb * 512));
-                        const uint64_t gd = tc::umma_desc_sw128(st), ud = tc::umma_desc_sw128(st + C::kA);
-                        const uint64_t xd = tc::umma_desc_sw128(base + (uint32_t)kb * BN * 128);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            umma_w4a8(dg, gd + 2u * k, xd + 2u * k, moe_idesc(BN, k), sf, sf + 8, (kb | k) ? 1u : 0u);
-                            umma_w4a8(du, ud + 2u * k, xd + 2u * k, moe_idesc(BN, k), sf + 4, sf + 8, (kb | k) ? 1u : 0u);
-                        }
-                        tc::umma_commit(empty(s));
+    }
+    __syncwarp();
+    tc::tc_fence_before();
+    if (S > 1) cluster_sync_all(); else __syncthreads();
+    tc::tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+
+    const int items = R.n_act * a.nit;
+    const int first = blockIdx.x / S, step = gridDim.x / S;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int s = 0, round = 0;     // stage and how often the ring went round (no divisions on this thread's path)
+            bool ok = true;
+            for (int item = first; item < items && ok; item += step) {
+                const int e = R.act[item / a.nit], j = item % a.nit;
+                const int rows = min(128, a.I - j * 128), boxes = rows == 128 ? 0 : (rows + 31) / 32;
+                int row = (e * 2) * a.I + j * 128;
+                const uint8_t* sf = a.s13 + (((int64_t)e * 2) * a.nit + j) * a.g1 * 512 + kb0 * 512;
+                // the barrier counts the packed bytes: 64 per row of 128 codes
+                const uint32_t bytes = (boxes ? boxes * 32 * 64 : 128 * 64) + 512;
+                for (int m = 0; m < 2 && ok; ++m, row += a.I, sf += (int64_t)a.nit * a.g1 * 512) {   // gate, up
+                    const uint8_t* f = sf;
+                    for (int kb = kb0; kb < kb1; ++kb, f += 512) {
+                        if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                        const uint32_t st = base + st_off + (uint32_t)s * C::kA;
+                        tc::mbar_expect_tx(full(s), bytes);
+                        if (!boxes) tc::tma_load_2d(st, &tmap_w, kb * 128, row, full(s));
+                        else
+                            for (int b = 0; b < boxes; ++b) tc::tma_load_2d(st + b * 32 * 128, &tmap_tail, kb * 128, row + 32 * b, full(s));
+                        bulk_load(base + sf_off + s * 512, f, 512, full(s));
+                        if (++s == stages) { s = 0; ++round; }
                     }
-                    tc::umma_commit(acc_full + 8u * buf);
                 }
             }
-            __syncwarp();
-        } else if (warp < 6) {
-            const int q = warp & 3;
-            const int owner = S == 1 ? 0 : S == 2 ? q >> 1 : q;
-            const int slot_q = S == 2 ? q & 1 : 0;            // the owner's slots: its quarters one after the other
-            const uint32_t slots = base + recv_off + (uint32_t)(slot_q * (S - 1)) * 2 * BN * 128;
-            int no = 0;
-            for (int item = first; item < items; item += step, ++no) {
-                const int ai = item / a.nit, j = item % a.nit, buf = no & 1, e = R.act[ai];
-                const bool done = tc::mbar_wait(acc_full + 8u * buf, (no >> 1) & 1, 4000000000ll);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // x's scales stay in tensor memory
+            for (int kb = 0; kb < nkb; ++kb) tmem_cp_sf(tmem + C::kSfX + 4 * kb, sf_desc(base + xsf_off + kb * 512));
+            int s = 0, par = 0, it = 0, no = 0;
+            bool ok = true;
+            for (int item = first; item < items && ok; item += step, ++no) {
+                const int buf = no & 1;
+                if (no >= 2 && !tc::mbar_wait(acc_empty + 8u * buf, ((no >> 1) - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
                 tc::tc_fence_after();
-                if (!done) atomicExch(&s_fail, 1);
-                bool go = __shfl_sync(0xffffffffu, (done && *(volatile int*)&s_fail == 0) ? 1 : 0, 0) != 0;
-                float v[2 * BN];
-                if (go) {
+                // all of the gate product, then all of up: a change of accumulator costs about 140 clocks, an MMA 57
+                for (int m = 0; m < 2 && ok; ++m) {
+                    const uint32_t d = tmem + (uint32_t)(buf * C::kAccSet + m * BN);
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        if (!tc::mbar_wait(full(s), par)) { atomicExch(&s_fail, 1); ok = false; break; }
+                        tc::tc_fence_after();
+                        const uint32_t sf = tmem + C::kSfW + (uint32_t)(it & 1) * 4;
+                        tmem_cp_sf(sf, sf_desc(base + sf_off + s * 512));
+                        const uint64_t wd = tc::umma_desc_sw128(base + st_off + (uint32_t)s * C::kA);
+                        const uint64_t xd = tc::umma_desc_sw128(base + (uint32_t)kb * BN * 128);
 #pragma unroll
-                    for (int c = 0; c < 2 * BN; c += 16) {
-                        uint32_t r[16];
-                        tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::kAccSet + c), r);
-                        tmem_ld_wait();
+                        for (int k = 0; k < 4; ++k)
+                            umma_w4a8(d, wd + 2u * k, xd + 2u * k, moe_idesc(BN, k), sf, tmem + C::kSfX + 4 * kb, (kb | k) ? 1u : 0u);
+                        tc::umma_commit(empty(s));
+                        if (++s == stages) { s = 0; par ^= 1; }
+                    }
+                }
+                tc::umma_commit(acc_full + 8u * buf);
+            }
+        }
+    } else if (warp < 6) {
+        const int q = warp & 3;
+        const int owner = S == 1 ? 0 : S == 2 ? q >> 1 : q;
+        const int slot_q = S == 2 ? q & 1 : 0;            // the owner's slots: its quarters one after the other
+        const uint32_t slots = base + recv_off + (uint32_t)(slot_q * (S - 1)) * 2 * BN * 128;
+        int no = 0;
+        for (int item = first; item < items; item += step, ++no) {
+            const int ai = item / a.nit, j = item % a.nit, buf = no & 1, e = R.act[ai];
+            const bool done = tc::mbar_wait(acc_full + 8u * buf, (no >> 1) & 1, 4000000000ll);
+            tc::tc_fence_after();
+            if (!done) atomicExch(&s_fail, 1);
+            const bool go = __shfl_sync(0xffffffffu, (done && *(volatile int*)&s_fail == 0) ? 1 : 0, 0) != 0;
+            if (!go) break;
+            const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::kAccSet);
+            if (S > 1 && rank != owner) {
+                if (no && !wait_cluster(recv_free + 8u * q, (no - 1) & 1)) { atomicExch(&s_fail, 1); break; }
+                const int src = rank < owner ? rank : rank - 1;
+                const uint32_t dst = map_rank(slots + (uint32_t)src * 2 * BN * 128 + lane * 4, owner);
+#pragma unroll 1
+                for (int t = 0; t < a.T; t += 4) {   // four tokens' gate and up columns; the columns behind T are padding
+                    float g[4], u[4];
+                    tmem_ld4(acc + t, g);
+                    tmem_ld4(acc + BN + t, u);
+                    tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[c + i] = __uint_as_float(r[i]);
+                    for (int i = 0; i < 4; ++i) {
+                        st_cluster(dst + (t + i) * 128, g[i]);
+                        st_cluster(dst + (BN + t + i) * 128, u[i]);
                     }
                 }
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty + 8u * buf);
-                if (!go) break;
-                if (S > 1) {
-                    if (rank != owner) {
-                        if (no && !wait_cluster(recv_free + 8u * q, (no - 1) & 1)) { atomicExch(&s_fail, 1); break; }
-                        const int src = rank < owner ? rank : rank - 1;
-                        const uint32_t dst = map_rank(slots + (uint32_t)src * 2 * BN * 128 + lane * 4, owner);
-#pragma unroll
-                        for (int c = 0; c < 2 * BN; ++c) st_cluster(dst + c * 128, v[c]);
-                        __syncwarp();
-                        if (lane == 0) arrive_cluster(map_rank(recv_full + 8u * q, owner));
-                        continue;
-                    }
-                    if (!wait_cluster(recv_full + 8u * q, no & 1)) { atomicExch(&s_fail, 1); break; }
-#pragma unroll
-                    for (int c = 0; c < 2 * BN; ++c) {
-                        float sum = 0.f;
-                        for (int s = 0; s < S; ++s) {   // rank order
-                            float p = v[c];
-                            if (s != rank)
-                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p) : "r"(slots + (uint32_t)(s < rank ? s : s - 1) * 2 * BN * 128 + c * 128 + lane * 4) : "memory");
-                            sum = s ? sum + p : p;
-                        }
-                        v[c] = sum;
-                    }
-                    __syncwarp();
-                    if (lane < S && lane != rank) arrive_cluster(map_rank(recv_free + 8u * q, lane));
+                if (lane == 0) {
+                    mbar_arrive(acc_empty + 8u * buf);
+                    arrive_cluster(map_rank(recv_full + 8u * q, owner));
                 }
-                // SwiGLU and the block quantiser: lane = row of I, this warp's 32 rows are one block
-                const uint32_t mask = R.mask[e];
-                float wv = 0.f;
-                if (lane < a.T)
-                    for (int k = 0; k < a.topk; ++k)
-                        if (R.sel[lane * kMaxTopk + k] == e) wv = R.wt[lane * kMaxTopk + k];
-                const bool real = j * 128 + q * 32 < a.I;
-                const int64_t tile = (int64_t)ai * a.nit + j;
-                uint8_t* ht = a.h + tile * (BN * 128);
-                uint8_t* hs = a.hs + tile * 512;
-                const int c16 = q * 2 + (lane >> 4);
-#pragma unroll
-                for (int t = 0; t < BN; ++t) {
-                    if (t < a.T) {
-                        const float w = __shfl_sync(0xffffffffu, wv, t);
-                        uint32_t byte = 0, sb = 127;
-                        if (real && (mask >> t & 1)) {
-                            const float g = fminf(v[t], a.limit), u = fminf(fmaxf(v[BN + t], -a.limit), a.limit);
-                            // fminf drops a NaN: put it back
-                            const float hv = (v[t] != v[t] || v[BN + t] != v[BN + t]) ? __uint_as_float(0x7fc00000u) : g / (1.f + expf(-g)) * u * w;
-                            const uint32_t m = __reduce_max_sync(0xffffffffu, abs_bits(hv));
-                            sb = ue8m0_of(m, 1e-4f, kInv448);
-                            byte = sb == 255u ? 0u : __nv_cvt_float_to_fp8(hv * ue8m0_inv(sb), __NV_SATFINITE, __NV_E4M3);
-                        }
-                        ht[t * 128 + ((c16 ^ (t & 7)) << 4) + (lane & 15)] = (uint8_t)byte;
-                        if (lane == 0) hs[t * 16 + q] = (uint8_t)sb;
-                    }
-                }
+                continue;
             }
+            if (S > 1 && !wait_cluster(recv_full + 8u * q, no & 1)) { atomicExch(&s_fail, 1); break; }
+            // sums of the S parts in rank order, SwiGLU and the block quantiser: lane = row of I, 32 rows = one block
+            const uint32_t mask = R.mask[e];
+            float wv = 0.f;
+            if (lane < a.T)
+                for (int k = 0; k < a.topk; ++k)
+                    if (R.sel[lane * kMaxTopk + k] == e) wv = R.wt[lane * kMaxTopk + k];
+            const bool real = j * 128 + q * 32 < a.I;
+            const int64_t tile = (int64_t)ai * a.nit + j;
+            uint8_t* ht = a.h + tile * (BN * 128);
+            uint8_t* hs = a.hs + tile * 512;
+            const int c16 = q * 2 + (lane >> 4);
+#pragma unroll 1
+            for (int t = 0; t < a.T; ++t) {
+                uint32_t byte = 0, sb = 127;
+                if (real && (mask >> t & 1)) {
+                    float g, u;
+                    tmem_ld1(acc + t, g);
+                    tmem_ld1(acc + BN + t, u);
+                    tmem_ld_wait();
+                    if (S > 1) {
+                        const uint32_t at = slots + t * 128 + lane * 4;
+                        float gs = 0.f, us = 0.f;
+#pragma unroll 1
+                        for (int s = 0; s < S; ++s) {
+                            float pg = g, pu = u;
+                            if (s != rank) {
+                                const uint32_t p = at + (uint32_t)(s < rank ? s : s - 1) * 2 * BN * 128;
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(pg) : "r"(p) : "memory");
+                                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(pu) : "r"(p + BN * 128) : "memory");
+                            }
+                            gs = s ? gs + pg : pg;
+                            us = s ? us + pu : pu;
+                        }
+                        g = gs;
+                        u = us;
+                    }
+                    const float w = __shfl_sync(0xffffffffu, wv, t);
+                    const bool nan = g != g || u != u;      // fminf and fmaxf drop a NaN: put it back
+                    g = fminf(g, a.limit);
+                    u = fminf(fmaxf(u, -a.limit), a.limit);
+                    const float hv = nan ? __uint_as_float(0x7fc00000u) : g / (1.f + expf(-g)) * u * w;
+                    sb = ue8m0_of(__reduce_max_sync(0xffffffffu, abs_bits(hv)), 1e-4f, kInv448);
+                    byte = sb == 255u ? 0u : __nv_cvt_float_to_fp8(hv * ue8m0_inv(sb), __NV_SATFINITE, __NV_E4M3);
+                }
+                ht[t * 128 + ((c16 ^ (t & 7)) << 4) + (lane & 15)] = (uint8_t)byte;
+                if (lane == 0) hs[t * 16 + q] = (uint8_t)sb;
+            }
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty + 8u * buf);
+            if (S > 1 && lane < S && lane != rank) arrive_cluster(map_rank(recv_free + 8u * q, lane));
         }
     }
     __syncwarp();
@@ -462,7 +496,7 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
     }
     if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
     // the logits were complete before kernel 1 started, the weights are never written: both may be read before the wait
-    route_all(a, R);
+    route_all(a, R, reinterpret_cast<uint32_t*>(smem_raw + (base - tc::smem_u32(smem_raw))), kMThreads);
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -473,12 +507,16 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
 
     if (warp == 0) {
         if (lane == 0) {
-            auto arm_w = [&](int s, int u) {
-                const int ai = u / a.nit, kb = u % a.nit, e = R.act[ai];
+            int ai = u0 / a.nit, kb = u0 - ai * a.nit, e = ai < R.n_act ? R.act[ai] : 0;
+            auto arm_w = [&](int s) {   // the next block in order
                 const uint32_t st = base + (uint32_t)s * C::kStage;
                 tc::mbar_expect_tx(full(s), 128 * 64 + 512 + BN * 128 + 512);
                 tc::tma_load_2d(st, &tmap_w, kb * 128, e * a.D + d0, full(s));
                 bulk_load(st + C::kA + BN * 128, a.s2 + (((int64_t)e * ntd + tile) * a.nit + kb) * 512, 512, full(s));
+                if (++kb == a.nit) {
+                    kb = 0;
+                    if (++ai < R.n_act) e = R.act[ai];
+                }
             };
             auto load_h = [&](int s, int u) {
                 const uint32_t st = base + (uint32_t)s * C::kStage;
@@ -486,21 +524,22 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
                 bulk_load(st + C::kA + BN * 128 + 512, a.hs + (int64_t)u * 512, 512, full(s));
             };
             const int ahead = min(C::kStages, u1 - u0);
-            for (int i = 0; i < ahead; ++i) arm_w(i, u0 + i);
+            for (int i = 0; i < ahead; ++i) arm_w(i);
             pdl_wait();
             for (int i = 0; i < ahead; ++i) load_h(i, u0 + i);
-            for (int it = ahead; it < u1 - u0; ++it) {
-                const int s = it % C::kStages;
-                if (!tc::mbar_wait(empty(s), ((it / C::kStages) - 1) & 1)) { atomicExch(&s_fail, 1); break; }
-                arm_w(s, u0 + it);
-                load_h(s, u0 + it);
+            int s = 0, par = 0;
+            for (int u = u0 + ahead; u < u1; ++u) {
+                if (!tc::mbar_wait(empty(s), par)) { atomicExch(&s_fail, 1); break; }
+                arm_w(s);
+                load_h(s, u);
+                if (++s == C::kStages) { s = 0; par ^= 1; }
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
+            int s = 0, par = 0;
             for (int it = 0; it < u1 - u0; ++it) {
-                const int s = it % C::kStages;
-                if (!tc::mbar_wait(full(s), (it / C::kStages) & 1)) { atomicExch(&s_fail, 1); break; }
+                if (!tc::mbar_wait(full(s), par)) { atomicExch(&s_fail, 1); break; }
                 tc::tc_fence_after();
                 const uint32_t st = base + (uint32_t)s * C::kStage;
                 const uint32_t sf = tmem + 32 + (uint32_t)(it & 1) * 8;
@@ -511,6 +550,7 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
                 for (int k = 0; k < 4; ++k)
                     umma_w4a8(tmem, wd + 2u * k, hd + 2u * k, moe_idesc(BN, k), sf, sf + 4, (it | k) ? 1u : 0u);
                 tc::umma_commit(empty(s));
+                if (++s == C::kStages) { s = 0; par ^= 1; }
             }
             tc::umma_commit(acc_full);
         }
@@ -547,7 +587,7 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
         TO* out = reinterpret_cast<TO*>(a.out);
         for (int c = rank * 2 + (t >> 7); c < a.T && !bad; c += 2 * S) {
             const uint32_t at = base + (uint32_t)(c * 128 + l) * 4;
-            float p[8];
+            float p[8];   // all ranks' loads in flight, then the sum in rank order
 #pragma unroll
             for (int s = 0; s < 8; ++s) p[s] = s < S ? ld_cluster(S > 1 ? map_rank(at, s) : at) : 0.f;
             float sum = p[0];
@@ -594,22 +634,51 @@ int make_tmap_u4(CUtensorMap* map, const void* base, uint64_t rows, uint64_t col
 }
 
 constexpr int kSms = 148;
-constexpr size_t kSmemMax = 227 * 1024 - 16 * 1024;   // dynamic part: the routing tables are static
+constexpr size_t kSmemMax = 227 * 1024 - 10 * 1024;   // dynamic part: the routing tables are static
 
-template <int BN>
-int pick_up_cluster(int g1, int64_t items, int* stages) {
-    // Rounds of the persistent clusters times the share of K that a CTA takes, over the cluster sizes whose x blocks leave
-    // room for three stages; with fewer than four (66 KB of weights in flight per SM) the stream is slower.  The smallest
-    // cluster among near equals.
+// Clusters of S CTAs that the device holds at once (a cluster stays inside a GPC, and GPCs lose SMs to odd sizes: 33
+// clusters of 4 at one CTA per SM, not 37).  A property of the device and of the kernel's resources.
+template <typename F>
+int resident_clusters(F kernel, int S, size_t smem, int per_sm, int* cache /* [9] */) {
+    if (S == 1) return kSms * per_sm;
+    int n = __atomic_load_n(&cache[S], __ATOMIC_RELAXED);
+    if (n) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(S * kSms));
+    cfg.blockDim = dim3(kMThreads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)S;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+        (void)cudaGetLastError();
+        n = 1;
+    }
+    __atomic_store_n(&cache[S], n, __ATOMIC_RELAXED);
+    return n;
+}
+
+template <int BN, typename F>
+int pick_up_cluster(F kernel, int g1, int64_t items, int* stages, int* clusters, int* cache) {
+    // Clocks of the longest-running cluster, over the cluster sizes whose x blocks leave room for four stages: per 128-column
+    // block of a matrix 300 (four MMAs of 57 and a scale copy), or its bytes' share of HBM if more than 119 CTAs stream;
+    // per tile about 1500 in the epilogue that the next tile does not hide, and 2000 more for the exchange of a split.
     int best = 0;
     double cost = 0;
     for (int S = 1; S <= 8 && S <= g1; S *= 2) {
-        const size_t fixed = up_fixed<BN>((g1 + S - 1) / S, S);
-        if (fixed + 3 * (size_t)UpCfg<BN>::kStage > kSmemMax) continue;
-        const int n = (int)((kSmemMax - fixed) / UpCfg<BN>::kStage);
-        const int64_t nc = kSms / S;
-        const double c = (double)((items + nc - 1) / nc) * ((g1 + S - 1) / S) * (n < 4 ? 1.15 : 1.0);
-        if (!best || c < cost * 0.97) { best = S; cost = c; *stages = n > 8 ? 8 : n; }
+        const int nkb = (g1 + S - 1) / S;
+        const size_t fixed = up_fixed<BN>(nkb, S);
+        if (nkb > UpCfg<BN>::kMaxKb || fixed + 4 * (size_t)UpCfg<BN>::kStage > kSmemMax) continue;
+        int n = (int)((kSmemMax - fixed) / UpCfg<BN>::kStage);
+        n = n > 12 ? 12 : n;
+        const int64_t nc = resident_clusters(kernel, S, kSmemMax, 1, cache);
+        const int64_t active = (items < nc ? items : nc) * S;
+        const double block = active * 2.52 > 300 ? active * 2.52 : 300.0;
+        const double c = (double)((items + nc - 1) / nc) * (2 * nkb * block + 1500 + (S > 1 ? 2000 : 0));
+        if (!best || c < cost) { best = S; cost = c; *stages = n; *clusters = (int)(items < nc ? items : nc); }
     }
     return best;
 }
@@ -620,18 +689,17 @@ int launch_up(MoeArgs a, const void* w13, cudaStream_t st) {
     int rc = make_tmap_u4(&tw, w13, (uint64_t)a.E * 2 * a.I, (uint64_t)a.g1 * 128, 128);
     if (!rc) rc = make_tmap_u4(&tt, w13, (uint64_t)a.E * 2 * a.I, (uint64_t)a.g1 * 128, 32);
     if (rc) return rc;
-    int stages = 0;
-    const int64_t pairs = (int64_t)a.T * a.topk, items = (pairs < a.E ? pairs : a.E) * a.nit;
-    a.S = pick_up_cluster<BN>(a.g1, items, &stages);
-    if (!a.S) return (int)cudaErrorInvalidValue;
-    const size_t smem = up_fixed<BN>((a.g1 + a.S - 1) / a.S, a.S) + (size_t)stages * UpCfg<BN>::kStage;
     auto k = fp4_moe_up_kernel<BN, TX>;
     static unsigned long long allowed = 0;
+    static int resident[9] = {};
     cudaError_t e = fp4_allow_smem(k, kSmemMax, allowed);
     if (e != cudaSuccess) return (int)e;
-    int64_t nc = kSms / a.S;
-    if (items < nc) nc = items;
-    return (int)fp4_launch(k, dim3((unsigned)(nc * a.S)), dim3(kMThreads), smem, st, a.S, g_fb_pdl != 0, tw, tt, a, stages);
+    int stages = 0, clusters = 0;
+    const int64_t pairs = (int64_t)a.T * a.topk, items = (pairs < a.E ? pairs : a.E) * a.nit;
+    a.S = pick_up_cluster<BN>(k, a.g1, items, &stages, &clusters, resident);
+    if (!a.S) return (int)cudaErrorInvalidValue;
+    const size_t smem = up_fixed<BN>((a.g1 + a.S - 1) / a.S, a.S) + (size_t)stages * UpCfg<BN>::kStage;
+    return (int)fp4_launch(k, dim3((unsigned)(clusters * a.S)), dim3(kMThreads), smem, st, a.S, g_fb_pdl != 0, tw, tt, a, stages);
 }
 
 template <int BN, typename TO>
@@ -645,10 +713,11 @@ int launch_down(MoeArgs a, const void* w2, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
     const int tiles = (a.D + 127) / 128;
     const int64_t pairs = (int64_t)a.T * a.topk, units = (pairs < a.E ? pairs : a.E) * a.nit;
-    // two CTAs per SM: as many K splits as fill them, with a few blocks each
-    int S = 2 * kSms / tiles;
-    S = S > 8 ? 8 : S < 1 ? 1 : S;
-    while (S > 1 && units < 2 * S) --S;
+    // as many K splits as keep all clusters resident at two CTAs per SM, with two blocks each at least
+    static int resident[9] = {};
+    int S = 1;
+    for (int c = 2; c <= 8; ++c)
+        if (units >= 2 * c && tiles <= resident_clusters(k, c, DownCfg<BN>::kSmem, 2, resident)) S = c;
     a.S = S;
     return (int)fp4_launch(k, dim3((unsigned)(tiles * S)), dim3(kMThreads), DownCfg<BN>::kSmem, st, S, true, tw, a);
 }
@@ -667,7 +736,7 @@ int moe_bn(const MoeArgs& a, const void* w13, const void* w2, cudaStream_t st) {
 // x [T, D] (dtype xdt, row stride ldx), logits f32 [T, E] (row stride ldl), bias f32 [E] or null; w13 codes / s13 scales of
 // [E, 2, I, D] mxfp4 (gate, up), w2 / s2 of [E, D, I]; out [T, D] (dtype odt, row stride ldo; accumulate: added to);
 // score 0 sqrt(softplus), 1 sigmoid, 2 softmax; norm: the chosen scores are divided by their sum; limit: SwiGLU clamp
-// (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: min(E, T topk) ceil(I / 128) (BN 128 + 512)
+// (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: min(E, T topk) ceil(I / 128) (128 BN + 512)
 // bytes, BN = 16 up to 16 tokens, else 32.
 FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logits, int64_t ldl, const float* bias, const void* w13,
                       const void* s13, const void* w2, const void* s2, void* out, int64_t odt, int64_t ldo, int64_t accumulate,
