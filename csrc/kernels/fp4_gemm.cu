@@ -173,7 +173,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     const uint32_t a_off = 0, b_off = C::kABytes, sfa_off = b_off + C::kBBytes, sfb_off = sfa_off + C::kSfa;
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             const int qatoms = C::kQAtoms;
             const int64_t q_rowtiles = (a.Q + 127) / 128;
             auto issue_p = [&](int s, int kb, int64_t p0, int nch) {
@@ -220,7 +220,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             int it = 0, tile_no = 0;
             bool ok = true;
             for (int t = first; t < n_tiles && ok; t += step, ++tile_no) {

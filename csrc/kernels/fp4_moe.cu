@@ -301,7 +301,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const int first = blockIdx.x / S, step = gridDim.x / S;
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             int s = 0, round = 0;     // stage and how often the ring went round (no divisions on this thread's path)
             bool ok = true;
             for (int item = first; item < items && ok; item += step) {
@@ -327,7 +327,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             // x's scales stay in tensor memory
             for (int kb = 0; kb < nkb; ++kb) tmem_cp_sf(tmem + C::kSfX + 4 * kb, sf_desc(base + xsf_off + kb * 512));
             int s = 0, par = 0, it = 0, no = 0;
@@ -506,7 +506,7 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
     const int u0 = (int)(units * rank / S), u1 = (int)(units * (rank + 1) / S);
 
     if (warp == 0) {
-        if (lane == 0) {
+        if (elect_one()) {
             int ai = u0 / a.nit, kb = u0 - ai * a.nit, e = ai < R.n_act ? R.act[ai] : 0;
             auto arm_w = [&](int s) {   // the next block in order
                 const uint32_t st = base + (uint32_t)s * C::kStage;
@@ -536,7 +536,7 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             int s = 0, par = 0;
             for (int it = 0; it < u1 - u0; ++it) {
                 if (!tc::mbar_wait(full(s), par)) { atomicExch(&s_fail, 1); break; }
