@@ -52,8 +52,7 @@ template <int FMT, typename T>
 __global__ void __launch_bounds__(kQThreads)
 fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int vec, uint8_t* __restrict__ codes,
                     uint8_t* __restrict__ scales, int64_t rows, int64_t cols, int scaled, float ts, float inv_ts) {
-    pdl_wait();
-    pdl_launch();
+    pdl_launch();   // (launched plainly: its own predecessor is complete)
     const Place p = place(rows, cols);
     const int lane = threadIdx.x & 31;
     const int64_t G = groups(cols), cstride = 64 * G;
@@ -117,7 +116,6 @@ template <int FMT, typename T>
 __global__ void __launch_bounds__(kQThreads)
 fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, int64_t ld,
                       int64_t bstride, int vec, int64_t rows, int64_t cols, float ts) {
-    PDL_PROLOGUE();
     const Place p = place(rows, cols);
     if (p.row >= rows || p.col >= cols) return;
     const int64_t G = groups(cols), cstride = 64 * G, nrt = (rows + 127) / 128;
@@ -204,7 +202,7 @@ FB_API int fb_fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bst
     const float inv = scaled ? (float)(1.0 / (double)ts) : 1.f;
     const int vec = vec_ok(x, ld, bstride, dtype == kF32 ? 4 : 2);
 #define FP4_Q(F, D)                                                                                                         \
-    (int)fp4_launch(fp4_quantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, g_fb_pdl != 0,      \
+    (int)fp4_launch(fp4_quantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, false,      \
                     (const Elem<D>::T*)x, ld, bstride, vec, (uint8_t*)codes, (uint8_t*)scales, rows, cols, scaled, ts, inv)
     if (fmt == kMxFp4) return dtype == kF32 ? FP4_Q(kMxFp4, kF32) : dtype == kBf16 ? FP4_Q(kMxFp4, kBf16) : FP4_Q(kMxFp4, kF16);
     return dtype == kF32 ? FP4_Q(kNvFp4, kF32) : dtype == kBf16 ? FP4_Q(kNvFp4, kBf16) : FP4_Q(kNvFp4, kF16);
@@ -222,7 +220,7 @@ FB_API int fb_fp4_dequantize(const void* codes, const void* scales, void* out, i
     const int vec = vec_ok(out, ld, bstride, dtype == kF32 ? 4 : 2);
     const float t = ts == 0.f ? 1.f : ts;
 #define FP4_D(F, D)                                                                                                    \
-    (int)fp4_launch(fp4_dequantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, g_fb_pdl != 0, \
+    (int)fp4_launch(fp4_dequantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, false, \
                     (const uint8_t*)codes, (const uint8_t*)scales, (Elem<D>::T*)out, ld, bstride, vec, rows, cols, t)
     if (fmt == kMxFp4) return dtype == kF32 ? FP4_D(kMxFp4, kF32) : dtype == kBf16 ? FP4_D(kMxFp4, kBf16) : FP4_D(kMxFp4, kF16);
     return dtype == kF32 ? FP4_D(kNvFp4, kF32) : dtype == kBf16 ? FP4_D(kNvFp4, kBf16) : FP4_D(kNvFp4, kF16);

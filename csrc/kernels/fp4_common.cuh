@@ -19,8 +19,8 @@ enum Fp4Dtype : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 int* fp4_status_ptr();
 
 // Launch with an optional cluster of `cluster` CTAs along x and, with `pdl`, programmatic serialisation against the
-// kernel before it in the stream (that kernel must be one of this file family: it waits for its own predecessor
-// before it lets its successor start).
+// kernel before it in the stream (always one of this file family that was launched plainly: when it runs, everything
+// before it is complete, so its successor may read what IT does not write before the wait).
 template <typename... KArgs, typename... Args>
 inline cudaError_t fp4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, bool pdl,
                               Args&&... args) {

@@ -21,8 +21,8 @@
 // Kernel 2 (down): a cluster of S CTAs per 128 rows of the output; the (expert, 128 columns of I) blocks of all chosen
 // experts are one long K axis, split over the cluster, accumulated in ONE accumulator: the sum over experts costs
 // nothing.  Partials are summed in rank order.  No atomics anywhere: the same bits every run.
-// Kernel 2 is launched with programmatic serialisation: it routes again and starts its weight stream while kernel 1
-// drains, and waits only before it reads h.
+// Kernel 2 is launched with programmatic serialisation: its CTAs set up on SMs that kernel 1 has left and wait for the
+// list of chosen experts, which kernel 1 leaves behind (routing again there cost 4 us at the head of kernel 2).
 #include <stdlib.h>
 #include "fp4_common.cuh"
 
@@ -31,7 +31,8 @@ namespace {
 using namespace fp4;
 
 constexpr int kMaxE = 512, kMaxTok = 32, kMaxTopk = 32;
-constexpr int kMThreads = 320;
+constexpr int kUpThreads = 640, kRouteThreads = 256;   // kernel 1: warps 0..7 route, the others quantise x meanwhile
+constexpr int kDownThreads = 320;
 
 enum Score : int { kSqrtSoftplus = 0, kSigmoid = 1, kSoftmax = 2 };
 
@@ -44,6 +45,7 @@ struct MoeArgs {
     void* out;
     int64_t ldo;
     uint8_t *h, *hs;          // [active][nit][BN * 128] operand tiles, [active][nit][512] their scale chunks
+    int* list;                // number of chosen experts, then the experts, ascending
     float scale, limit;
     int xdt, odt, accumulate, T, E, topk, D, I, score, norm;
     int g1, nit, S;           // 128-column groups of D, 128-row tiles of I, cluster size
@@ -55,7 +57,6 @@ struct Route {
     float wt[kMaxTok * kMaxTopk];
     uint16_t sel[kMaxTok * kMaxTopk];
     uint16_t act[kMaxE];                      // chosen experts, ascending
-    float mx[kMaxTok], inv[kMaxTok];          // softmax: largest logit, 1 / sum
     int n_act;
 };
 
@@ -71,44 +72,60 @@ __device__ __forceinline__ float score_of(float z, int score, float mx, float in
     return sqrtf(fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
 }
 
-// All tokens' choices into r, by the first `nthreads` threads of the block (barrier 2 among them; no barrier at the end).
-// keys: T * E words of scratch.
-// Everything here is a rolled loop: the code runs once per CTA, and straight-line code that runs once costs its
-// instruction fetches (a version unrolled over the 16 scores of a lane took 30 us, this one about 3).
-__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, uint32_t* keys, const int nthreads) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = nthreads >> 5;
-    auto sync = [&]() { asm volatile("bar.sync 2, %0;" ::"r"(nthreads) : "memory"); };
-    for (int e = threadIdx.x; e < kMaxE; e += nthreads) r.mask[e] = 0u;
-    if (a.score == kSoftmax) {
-        for (int t = warp; t < a.T; t += nw) {
-            const float* lg = a.logits + t * a.ldl;
-            float mx = -INFINITY, sum = 0.f;
-#pragma unroll 1
-            for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, __ldg(lg + e));
-            mx = warp_max(mx);
-            if (mx == -INFINITY) mx = 0.f;
-#pragma unroll 1
-            for (int e = lane; e < a.E; e += 32) sum += expf(__ldg(lg + e) - mx);
-            sum = warp_sum(sum);
-            if (lane == 0) { r.mx[t] = mx; r.inv[t] = 1.f / sum; }
-        }
-        sync();
-    }
+// All tokens' choices into r, by the first kRouteThreads threads of the block (barrier 2 among them; none at the end).
+// keys: (T + 1) * E words of scratch.  Loops are rolled except for loads: the code runs once per CTA, and straight-line
+// code that runs once costs its instruction fetches (unrolled over the 16 scores of a lane it took 30 us for one token).
+__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, uint32_t* keys) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int nw = kRouteThreads / 32;
+    auto sync = [&]() { asm volatile("bar.sync 2, %0;" ::"n"(kRouteThreads) : "memory"); };
     const int total = a.T * a.E;
+    float* lg = reinterpret_cast<float*>(keys);     // logits, then in their place the keys
+    float* bias = lg + total;
 #pragma unroll 1
-    for (int i = threadIdx.x; i < total; i += nthreads) {
-        const int t = i / a.E, e = i - t * a.E;
-        const float z = __ldg(a.logits + t * a.ldl + e);
-        // every score grows with its logit: without a bias the logit itself decides, exactly
-        keys[i] = order_key(a.bias ? score_of(z, a.score, r.mx[t], r.inv[t]) + __ldg(a.bias + e) : z);
+    for (int i0 = threadIdx.x; i0 < total; i0 += 8 * kRouteThreads) {   // eight loads in flight
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + j * kRouteThreads, t = i / a.E;
+            z[j] = i < total ? __ldg(a.logits + t * a.ldl + (i - t * a.E)) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (i0 + j * kRouteThreads < total) lg[i0 + j * kRouteThreads] = z[j];
+    }
+    for (int e = threadIdx.x; e < kMaxE; e += kRouteThreads) {
+        r.mask[e] = 0u;
+        if (e < a.E && a.bias) bias[e] = __ldg(a.bias + e);
     }
     sync();
 #pragma unroll 1
     for (int t = warp; t < a.T; t += nw) {
-        const float* lg = a.logits + t * a.ldl;
+        float* row = lg + t * a.E;
+        float mx = 0.f, inv = 1.f;
+        if (a.score == kSoftmax) {
+            mx = -INFINITY;
+#pragma unroll 1
+            for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, row[e]);
+            mx = warp_max(mx);
+            if (mx == -INFINITY) mx = 0.f;
+            float sum = 0.f;
+#pragma unroll 1
+            for (int e = lane; e < a.E; e += 32) sum += expf(row[e] - mx);
+            inv = 1.f / warp_sum(sum);
+        }
+        // every score grows with its logit: without a bias the logit itself decides, exactly
+        if (a.bias) {
+#pragma unroll 1
+            for (int e = lane; e < a.E; e += 32) keys[t * a.E + e] = order_key(score_of(row[e], a.score, mx, inv) + bias[e]);
+        }
+        __syncwarp();
         uint32_t key[kMaxE / 32];
 #pragma unroll
-        for (int j = 0; j < kMaxE / 32; ++j) key[j] = lane + 32 * j < a.E ? keys[t * a.E + lane + 32 * j] : 0u;
+        for (int j = 0; j < kMaxE / 32; ++j) {
+            const int e = lane + 32 * j;
+            key[j] = e >= a.E ? 0u : a.bias ? keys[t * a.E + e] : order_key(row[e]);
+        }
         int mine = 0;
 #pragma unroll 1
         for (int k = 0; k < a.topk; ++k) {
@@ -125,7 +142,7 @@ __device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, uint32_t* 
             for (int j = 0; j < kMaxE / 32; ++j)
                 if (e == lane + 32 * j) key[j] = 0u;
         }
-        float p = lane < a.topk ? score_of(__ldg(lg + mine), a.score, r.mx[t], r.inv[t]) : 0.f;
+        float p = lane < a.topk ? score_of(__ldg(a.logits + t * a.ldl + mine), a.score, mx, inv) : 0.f;
         if (a.norm) p = p / (warp_sum(p) + 1e-20f);
         if (lane < a.topk) {
             r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
@@ -144,6 +161,11 @@ __device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, uint32_t* 
             n += __popc(b);
         }
         if (lane == 0) r.n_act = n;
+        __syncwarp();
+        if (blockIdx.x == 0) {   // for kernel 2
+            for (int i = lane; i < n; i += 32) a.list[1 + i] = r.act[i];
+            if (lane == 0) a.list[0] = n;
+        }
     }
     fence_proxy_async();   // the scratch becomes the target of TMA copies
 }
@@ -192,7 +214,6 @@ struct UpCfg {
     static constexpr int kMaxKb = 64;                          // 128-column blocks of x per CTA
     static_assert(kSfX + 4 * kMaxKb <= kTmem, "tensor memory");
 };
-constexpr int kRouteThreads = 160;   // of kernel 1: the others quantise x meanwhile
 
 // Shared memory of kernel 1: x blocks | their scale chunks | receive slots | stages | stage scales | barriers
 template <int BN>
@@ -205,7 +226,7 @@ template <int BN>
 __host__ __device__ constexpr size_t up_fixed(int nkb, int S) { return up_front<BN>(nkb, S) + 1024 + UpCfg<BN>::kBars; }
 
 template <int BN, typename TX>
-__global__ void __launch_bounds__(kMThreads, 1)
+__global__ void __launch_bounds__(kUpThreads, 1)
 fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_tail, const MoeArgs a, int stages) {
     using C = UpCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -227,7 +248,6 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const uint32_t acc_full = bars + 16u * stages, acc_empty = acc_full + 16u, recv_full = acc_empty + 16u, recv_free = recv_full + 32u,
                    tmem_slot = recv_free + 32u;
 
-    pdl_wait();
     pdl_launch();
     if (warp == 9) {
         if (lane == 0) {
@@ -252,7 +272,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         tc::tmem_alloc(tmem_slot, C::kTmem);
     }
     if (threadIdx.x < kRouteThreads) {
-        route_all(a, R, reinterpret_cast<uint32_t*>(base_g + st_off), kRouteThreads);
+        route_all(a, R, reinterpret_cast<uint32_t*>(base_g + st_off));
     } else {
         // ---- this CTA's K range of x, quantised, in operand form ----
         const TX* x = reinterpret_cast<const TX*>(a.x);
@@ -260,32 +280,40 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         const int per_row = nkb * 16;    // 8-value units
         const int units = a.T * per_row;
         const int tid = threadIdx.x - kRouteThreads;
+        constexpr int kN = kUpThreads - kRouteThreads, kBatch = 4;
 #pragma unroll 1
-        for (int u0 = 0; u0 < units; u0 += kMThreads - kRouteThreads) {
-            const int u = u0 + tid;
-            const int t = u < units ? u / per_row : 0, c = u < units ? u - t * per_row : 0;
-            const int col = kb0 * 128 + c * 8;
-            float v[8];
-            load8(x + t * a.ldx + min(col, a.D - 1), u < units ? max(0, min(8, a.D - col)) : 0, vec && u < units, v);
-            uint32_t m = 0;
+        for (int u0 = 0; u0 < units; u0 += kBatch * kN) {   // four loads in flight per thread
+            float v[kBatch][8];
+            int at[kBatch], sat[kBatch];   // where the unit and (from a block's first lane) its scale go; -1: nowhere
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-            if (u < units) {
+            for (int b = 0; b < kBatch; ++b) {
+                const int u = u0 + b * kN + tid;
+                const int t = u < units ? u / per_row : 0, c = u < units ? u - t * per_row : 0;
+                const int col = kb0 * 128 + c * 8, kb = c >> 4, u16 = c & 15;      // u16: 8-byte unit of the 128-byte row
+                load8(x + t * a.ldx + min(col, a.D - 1), u < units ? max(0, min(8, a.D - col)) : 0, vec && u < units, v[b]);
+                at[b] = u < units ? kb * (BN * 128) + t * 128 + (((u16 >> 1) ^ (t & 7)) << 4) + (u16 & 1) * 8 : -1;
+                sat[b] = (c & 3) == 0 ? (int)xsf_off + kb * 512 + t * 16 + (u16 >> 2) : -1;
+            }
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[b][i]));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 const uint32_t sb = ue8m0_of(m, 1e-4f, kInv448);
                 const float inv = sb == 255u ? 0.f : ue8m0_inv(sb);
                 uint32_t w[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-                    w[i] = lo | hi << 16;
+                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i] * inv, v[b][4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i + 2] * inv, v[b][4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                    w[i] = sb == 255u ? 0u : lo | hi << 16;
                 }
-                if (sb == 255u) w[0] = w[1] = 0u;
-                const int kb = c >> 4, u16 = c & 15;      // 8-byte unit of the 128-byte row
-                *reinterpret_cast<uint2*>(base_g + (size_t)kb * BN * 128 + t * 128 + (((u16 >> 1) ^ (t & 7)) << 4) + (u16 & 1) * 8) = make_uint2(w[0], w[1]);
-                if ((c & 3) == 0) base_g[xsf_off + kb * 512 + t * 16 + (u16 >> 2)] = (uint8_t)sb;
+                if (at[b] >= 0) {
+                    *reinterpret_cast<uint2*>(base_g + at[b]) = make_uint2(w[0], w[1]);
+                    if (sat[b] >= 0) base_g[sat[b]] = (uint8_t)sb;
+                }
             }
         }
         fence_proxy_async();
@@ -462,18 +490,19 @@ template <int BN>
 struct DownCfg {
     static constexpr int kA = 128 * 128;
     static constexpr int kStage = kA + BN * 128 + 1024;         // weights, h tile, both scale chunks
-    static constexpr int kStages = (104 * 1024 - 1024 - 256) / kStage;   // two CTAs per SM, each with 9 KB of tables
+    static constexpr int kStages = (111 * 1024 - 1024 - 256) / kStage;   // two CTAs per SM, each with 1 KB of static tables
     static constexpr int kTmem = 64;                            // BN accumulator columns + 2 x 8 of scales
     static constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 256;
     static_assert((size_t)BN * 128 * 4 <= (size_t)kStages * kStage && kStages * 16 + 16 <= 256, "smem");
 };
 
 template <int BN, typename TO>
-__global__ void __launch_bounds__(kMThreads, 2)
+__global__ void __launch_bounds__(kDownThreads, 2)
 fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a) {
     using C = DownCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ Route R;
+    __shared__ uint16_t s_act[kMaxE];
+    __shared__ int s_n;
     __shared__ int s_fail;
     const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = base + C::kStages * C::kStage;
@@ -495,19 +524,24 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
         tc::prefetch_tmap(&tmap_w);
     }
     if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
-    // the logits were complete before kernel 1 started, the weights are never written: both may be read before the wait
-    route_all(a, R, reinterpret_cast<uint32_t*>(smem_raw + (base - tc::smem_u32(smem_raw))), kMThreads);
+    pdl_wait();   // everything below reads what kernel 1 wrote
+    if (warp >= 2) {
+        const volatile int* list = a.list;   // (a read-only load might move above the wait)
+        const int n = list[0];
+        for (int i = threadIdx.x - 64; i < n; i += kDownThreads - 64) s_act[i] = (uint16_t)list[1 + i];
+        if (threadIdx.x == 64) s_n = n;
+    }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
-    const int64_t units = (int64_t)R.n_act * a.nit;
+    const int64_t units = (int64_t)s_n * a.nit;
     const int u0 = (int)(units * rank / S), u1 = (int)(units * (rank + 1) / S);
 
     if (warp == 0) {
         if (elect_one()) {
-            int ai = u0 / a.nit, kb = u0 - ai * a.nit, e = ai < R.n_act ? R.act[ai] : 0;
+            int ai = u0 / a.nit, kb = u0 - ai * a.nit, e = ai < s_n ? s_act[ai] : 0;
             auto arm_w = [&](int s) {   // the next block in order
                 const uint32_t st = base + (uint32_t)s * C::kStage;
                 tc::mbar_expect_tx(full(s), 128 * 64 + 512 + BN * 128 + 512);
@@ -515,7 +549,7 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
                 bulk_load(st + C::kA + BN * 128, a.s2 + (((int64_t)e * ntd + tile) * a.nit + kb) * 512, 512, full(s));
                 if (++kb == a.nit) {
                     kb = 0;
-                    if (++ai < R.n_act) e = R.act[ai];
+                    if (++ai < s_n) e = s_act[ai];
                 }
             };
             auto load_h = [&](int s, int u) {
@@ -523,16 +557,12 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
                 bulk_load(st + C::kA, a.h + (int64_t)u * (BN * 128), BN * 128, full(s));
                 bulk_load(st + C::kA + BN * 128 + 512, a.hs + (int64_t)u * 512, 512, full(s));
             };
-            const int ahead = min(C::kStages, u1 - u0);
-            for (int i = 0; i < ahead; ++i) arm_w(i);
-            pdl_wait();
-            for (int i = 0; i < ahead; ++i) load_h(i, u0 + i);
-            int s = 0, par = 0;
-            for (int u = u0 + ahead; u < u1; ++u) {
-                if (!tc::mbar_wait(empty(s), par)) { atomicExch(&s_fail, 1); break; }
+            int s = 0, round = 0;
+            for (int u = u0; u < u1; ++u) {
+                if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); break; }
                 arm_w(s);
                 load_h(s, u);
-                if (++s == C::kStages) { s = 0; par ^= 1; }
+                if (++s == C::kStages) { s = 0; ++round; }
             }
         }
     } else if (warp == 1) {
@@ -639,13 +669,13 @@ constexpr size_t kSmemMax = 227 * 1024 - 10 * 1024;   // dynamic part: the routi
 // Clusters of S CTAs that the device holds at once (a cluster stays inside a GPC, and GPCs lose SMs to odd sizes: 33
 // clusters of 4 at one CTA per SM, not 37).  A property of the device and of the kernel's resources.
 template <typename F>
-int resident_clusters(F kernel, int S, size_t smem, int per_sm, int* cache /* [9] */) {
+int resident_clusters(F kernel, int S, int threads, size_t smem, int per_sm, int* cache /* [9] */) {
     if (S == 1) return kSms * per_sm;
     int n = __atomic_load_n(&cache[S], __ATOMIC_RELAXED);
     if (n) return n;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(S * kSms));
-    cfg.blockDim = dim3(kMThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -674,7 +704,7 @@ int pick_up_cluster(F kernel, int g1, int64_t items, int* stages, int* clusters,
         if (nkb > UpCfg<BN>::kMaxKb || fixed + 4 * (size_t)UpCfg<BN>::kStage > kSmemMax) continue;
         int n = (int)((kSmemMax - fixed) / UpCfg<BN>::kStage);
         n = n > 12 ? 12 : n;
-        const int64_t nc = resident_clusters(kernel, S, kSmemMax, 1, cache);
+        const int64_t nc = resident_clusters(kernel, S, kUpThreads, kSmemMax, 1, cache);
         const int64_t active = (items < nc ? items : nc) * S;
         const double block = active * 2.52 > 300 ? active * 2.52 : 300.0;
         const double c = (double)((items + nc - 1) / nc) * (2 * nkb * block + 1500 + (S > 1 ? 2000 : 0));
@@ -699,7 +729,7 @@ int launch_up(MoeArgs a, const void* w13, cudaStream_t st) {
     a.S = pick_up_cluster<BN>(k, a.g1, items, &stages, &clusters, resident);
     if (!a.S) return (int)cudaErrorInvalidValue;
     const size_t smem = up_fixed<BN>((a.g1 + a.S - 1) / a.S, a.S) + (size_t)stages * UpCfg<BN>::kStage;
-    return (int)fp4_launch(k, dim3((unsigned)(clusters * a.S)), dim3(kMThreads), smem, st, a.S, g_fb_pdl != 0, tw, tt, a, stages);
+    return (int)fp4_launch(k, dim3((unsigned)(clusters * a.S)), dim3(kUpThreads), smem, st, a.S, false, tw, tt, a, stages);
 }
 
 template <int BN, typename TO>
@@ -717,9 +747,9 @@ int launch_down(MoeArgs a, const void* w2, cudaStream_t st) {
     static int resident[9] = {};
     int S = 1;
     for (int c = 2; c <= 8; ++c)
-        if (units >= 2 * c && tiles <= resident_clusters(k, c, DownCfg<BN>::kSmem, 2, resident)) S = c;
+        if (units >= 2 * c && tiles <= resident_clusters(k, c, kDownThreads, DownCfg<BN>::kSmem, 2, resident)) S = c;
     a.S = S;
-    return (int)fp4_launch(k, dim3((unsigned)(tiles * S)), dim3(kMThreads), DownCfg<BN>::kSmem, st, S, true, tw, a);
+    return (int)fp4_launch(k, dim3((unsigned)(tiles * S)), dim3(kDownThreads), DownCfg<BN>::kSmem, st, S, true, tw, a);
 }
 
 template <int BN>
@@ -736,8 +766,8 @@ int moe_bn(const MoeArgs& a, const void* w13, const void* w2, cudaStream_t st) {
 // x [T, D] (dtype xdt, row stride ldx), logits f32 [T, E] (row stride ldl), bias f32 [E] or null; w13 codes / s13 scales of
 // [E, 2, I, D] mxfp4 (gate, up), w2 / s2 of [E, D, I]; out [T, D] (dtype odt, row stride ldo; accumulate: added to);
 // score 0 sqrt(softplus), 1 sigmoid, 2 softmax; norm: the chosen scores are divided by their sum; limit: SwiGLU clamp
-// (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: min(E, T topk) ceil(I / 128) (128 BN + 512)
-// bytes, BN = 16 up to 16 tokens, else 32.
+// (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: 4096 + min(E, T topk) ceil(I / 128) (128 BN
+// + 512) bytes, BN = 16 up to 16 tokens, else 32.
 FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logits, int64_t ldl, const float* bias, const void* w13,
                       const void* s13, const void* w2, const void* s2, void* out, int64_t odt, int64_t ldo, int64_t accumulate,
                       void* work, int64_t T, int64_t E, int64_t topk, int64_t D, int64_t I, int64_t score, int64_t norm, float scale,
@@ -756,7 +786,8 @@ FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logi
     a.status = fp4_status_ptr();
     if (!a.status) return (int)cudaErrorNotSupported;
     const int64_t bn = T <= 16 ? 16 : 32, pairs = T * topk < E ? T * topk : E;
-    a.hs = (uint8_t*)work;                       // scale chunks, then operand tiles: both 16-byte aligned
+    a.list = (int*)work;                         // list, scale chunks, operand tiles: all 16-byte aligned
+    a.hs = (uint8_t*)work + 4096;
     a.h = a.hs + pairs * a.nit * 512;
     return bn == 16 ? moe_bn<16>(a, w13, w2, st) : moe_bn<32>(a, w13, w2, st);
 }

@@ -285,7 +285,7 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     out, ldo = _product_out(out, T, D, out_dtype or x.dtype, dev)
     if T:
         tile = 128 * (16 if T <= 16 else 32) + 512
-        work = torch.empty(min(E, T * topk) * ((I + 127) // 128) * tile, dtype=torch.uint8, device=dev)
+        work = torch.empty(4096 + min(E, T * topk) * ((I + 127) // 128) * tile, dtype=torch.uint8, device=dev)
         _call(dev, "fb_fp4_moe", x, _DTYPES[x.dtype], ldx, logits, logits.stride(0) if T > 1 else E, bias, w13.codes, w13.scales,
               w2.codes, w2.scales, out, _DTYPES[out.dtype], ldo, int(accumulate), work, T, E, topk, D, I, SCORES[score], int(norm),
               float(scale), float(limit) if limit else math.inf)
