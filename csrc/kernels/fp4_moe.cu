@@ -57,6 +57,7 @@ struct Route {
     float wt[kMaxTok * kMaxTopk];
     uint16_t sel[kMaxTok * kMaxTopk];
     uint16_t act[kMaxE];                      // chosen experts, ascending
+    float mx[kMaxTok], inv[kMaxTok];          // softmax: largest logit, 1 / sum
     int n_act;
 };
 
@@ -73,76 +74,89 @@ __device__ __forceinline__ float score_of(float z, int score, float mx, float in
 }
 
 // All tokens' choices into r, by the first kRouteThreads threads of the block (barrier 2 among them; none at the end).
-// keys: (T + 1) * E words of scratch.  Loops are rolled except for loads: the code runs once per CTA, and straight-line
-// code that runs once costs its instruction fetches (unrolled over the 16 scores of a lane it took 30 us for one token).
-__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, uint32_t* keys) {
+// scratch: (T + 1) * E words.  Every CTA runs this once, before its first weight arrives: what counts is the length of
+// the dependent chain and the size of the code (straight-line code that runs once costs its instruction fetches: with the
+// scores unrolled over a lane's 16 experts it took 30 us for one token), so the score loops are rolled, the selection is a
+// tree over registers, and a token's scores are spread over the warps that have no token of their own.
+__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, float* scratch) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int nw = kRouteThreads / 32;
+    constexpr int nw = kRouteThreads / 32, kPer = kMaxE / 32;
     auto sync = [&]() { asm volatile("bar.sync 2, %0;" ::"n"(kRouteThreads) : "memory"); };
-    const int total = a.T * a.E;
-    float* lg = reinterpret_cast<float*>(keys);     // logits, then in their place the keys
-    float* bias = lg + total;
-#pragma unroll 1
-    for (int i0 = threadIdx.x; i0 < total; i0 += 8 * kRouteThreads) {   // eight loads in flight
-        float z[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int i = i0 + j * kRouteThreads, t = i / a.E;
-            z[j] = i < total ? __ldg(a.logits + t * a.ldl + (i - t * a.E)) : 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (i0 + j * kRouteThreads < total) lg[i0 + j * kRouteThreads] = z[j];
-    }
+    float* lg = scratch;                                                   // logits, then in their place the keys
+    uint32_t* keys = reinterpret_cast<uint32_t*>(scratch);
+    float* bias = scratch + a.T * a.E;
     for (int e = threadIdx.x; e < kMaxE; e += kRouteThreads) {
         r.mask[e] = 0u;
         if (e < a.E && a.bias) bias[e] = __ldg(a.bias + e);
     }
-    sync();
 #pragma unroll 1
     for (int t = warp; t < a.T; t += nw) {
-        float* row = lg + t * a.E;
-        float mx = 0.f, inv = 1.f;
+        float z[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) z[j] = lane + 32 * j < a.E ? __ldg(a.logits + t * a.ldl + lane + 32 * j) : -INFINITY;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j)
+            if (lane + 32 * j < a.E) lg[t * a.E + lane + 32 * j] = z[j];
         if (a.score == kSoftmax) {
-            mx = -INFINITY;
-#pragma unroll 1
-            for (int e = lane; e < a.E; e += 32) mx = fmaxf(mx, row[e]);
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, z[j]);
             mx = warp_max(mx);
             if (mx == -INFINITY) mx = 0.f;
-            float sum = 0.f;
+            __syncwarp();
 #pragma unroll 1
-            for (int e = lane; e < a.E; e += 32) sum += expf(row[e] - mx);
-            inv = 1.f / warp_sum(sum);
+            for (int e = lane; e < a.E; e += 32) sum += expf(lg[t * a.E + e] - mx);
+            sum = warp_sum(sum);
+            if (lane == 0) { r.mx[t] = mx; r.inv[t] = 1.f / sum; }
         }
-        // every score grows with its logit: without a bias the logit itself decides, exactly
-        if (a.bias) {
+    }
+    sync();
+    // every score grows with its logit: without a bias the logit itself decides, exactly
+    if (a.bias) {
+        const int stripes = a.T >= nw ? 1 : nw / a.T;
 #pragma unroll 1
-            for (int e = lane; e < a.E; e += 32) keys[t * a.E + e] = order_key(score_of(row[e], a.score, mx, inv) + bias[e]);
+        for (int u = warp; u < a.T * stripes; u += nw) {
+            const int t = u / stripes, first = (u - t * stripes) * 32 + lane;
+            const float mx = r.mx[t], inv = r.inv[t];
+#pragma unroll 1
+            for (int e = first; e < a.E; e += 32 * stripes) {
+                const float z = lg[t * a.E + e];
+                keys[t * a.E + e] = order_key(score_of(z, a.score, mx, inv) + bias[e]);
+            }
         }
-        __syncwarp();
-        uint32_t key[kMaxE / 32];
+        sync();
+    }
+#pragma unroll 1
+    for (int t = warp; t < a.T; t += nw) {
+        uint32_t key[kPer];
 #pragma unroll
-        for (int j = 0; j < kMaxE / 32; ++j) {
+        for (int j = 0; j < kPer; ++j) {
             const int e = lane + 32 * j;
-            key[j] = e >= a.E ? 0u : a.bias ? keys[t * a.E + e] : order_key(row[e]);
+            key[j] = e >= a.E ? 0u : a.bias ? keys[t * a.E + e] : order_key(lg[t * a.E + e]);
         }
         int mine = 0;
 #pragma unroll 1
         for (int k = 0; k < a.topk; ++k) {
-            uint32_t best = 0;
-            int bj = 0;
+            uint32_t m[kPer];
 #pragma unroll
-            for (int j = 0; j < kMaxE / 32; ++j)
-                if (key[j] > best) { best = key[j]; bj = j; }
-            const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-            const uint32_t cand = best == top ? (uint32_t)(lane + 32 * bj) : 0xffffffffu;
-            const int e = (int)__reduce_min_sync(0xffffffffu, cand);
-            if (lane == k) mine = e;
+            for (int j = 0; j < kPer; ++j) m[j] = key[j];
 #pragma unroll
-            for (int j = 0; j < kMaxE / 32; ++j)
-                if (e == lane + 32 * j) key[j] = 0u;
+            for (int o = kPer / 2; o > 0; o >>= 1)
+#pragma unroll
+                for (int j = 0; j < o; ++j) m[j] = max(m[j], m[j + o]);
+            const uint32_t top = __reduce_max_sync(0xffffffffu, m[0]);
+            uint32_t hit = 0;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) hit |= key[j] == top ? 1u << j : 0u;
+            const uint32_t cand = hit ? (uint32_t)(lane + 32 * (__ffs(hit) - 1)) : 0xffffffffu;
+            const uint32_t e = __reduce_min_sync(0xffffffffu, cand);
+            if (lane == k) mine = (int)e;
+            const uint32_t gone = (e & 31u) == (uint32_t)lane ? 1u << (e >> 5) : 0u;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                if (gone >> j & 1) key[j] = 0u;
         }
-        float p = lane < a.topk ? score_of(__ldg(a.logits + t * a.ldl + mine), a.score, mx, inv) : 0.f;
+        float p = lane < a.topk ? score_of(__ldg(a.logits + t * a.ldl + mine), a.score, r.mx[t], r.inv[t]) : 0.f;
         if (a.norm) p = p / (warp_sum(p) + 1e-20f);
         if (lane < a.topk) {
             r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
@@ -152,13 +166,14 @@ __device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, uint32_t* 
     }
     sync();
     if (warp == 0) {
+        uint32_t on[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) on[j] = __ballot_sync(0xffffffffu, r.mask[lane + 32 * j] != 0u);
         int n = 0;
-#pragma unroll 1
-        for (int e0 = 0; e0 < a.E; e0 += 32) {
-            const bool on = e0 + lane < a.E && r.mask[e0 + lane] != 0u;
-            const uint32_t b = __ballot_sync(0xffffffffu, on);
-            if (on) r.act[n + __popc(b & ((1u << lane) - 1u))] = (uint16_t)(e0 + lane);
-            n += __popc(b);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (on[j] >> lane & 1) r.act[n + __popc(on[j] & ((1u << lane) - 1u))] = (uint16_t)(lane + 32 * j);
+            n += __popc(on[j]);
         }
         if (lane == 0) r.n_act = n;
         __syncwarp();
@@ -272,47 +287,46 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         tc::tmem_alloc(tmem_slot, C::kTmem);
     }
     if (threadIdx.x < kRouteThreads) {
-        route_all(a, R, reinterpret_cast<uint32_t*>(base_g + st_off));
+        route_all(a, R, reinterpret_cast<float*>(base_g + st_off));
     } else {
         // ---- this CTA's K range of x, quantised, in operand form ----
         const TX* x = reinterpret_cast<const TX*>(a.x);
         const bool vec = ((uintptr_t)x & 15) == 0 && a.ldx * (int64_t)sizeof(TX) % 16 == 0;
-        const int per_row = nkb * 16;    // 8-value units
-        const int units = a.T * per_row;
-        const int tid = threadIdx.x - kRouteThreads;
         constexpr int kN = kUpThreads - kRouteThreads, kBatch = 4;
+        // a thread keeps its eight columns over the tokens (four loads in flight); a block of 32 columns is four lanes
 #pragma unroll 1
-        for (int u0 = 0; u0 < units; u0 += kBatch * kN) {   // four loads in flight per thread
-            float v[kBatch][8];
-            int at[kBatch], sat[kBatch];   // where the unit and (from a block's first lane) its scale go; -1: nowhere
+        for (int c0 = 0; c0 < nkb * 16; c0 += kN) {
+            const int c = c0 + threadIdx.x - kRouteThreads;
+            const int col = kb0 * 128 + c * 8, kb = c >> 4, u16 = c & 15;      // u16: 8-byte unit of the 128-byte row
+            const bool in = c < nkb * 16;
+            const int n = in ? max(0, min(8, a.D - col)) : 0;
+            const TX* xc = x + min(col, a.D - 1);
+#pragma unroll 1
+            for (int t0 = 0; t0 < a.T; t0 += kBatch) {
+                float v[kBatch][8];
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                const int u = u0 + b * kN + tid;
-                const int t = u < units ? u / per_row : 0, c = u < units ? u - t * per_row : 0;
-                const int col = kb0 * 128 + c * 8, kb = c >> 4, u16 = c & 15;      // u16: 8-byte unit of the 128-byte row
-                load8(x + t * a.ldx + min(col, a.D - 1), u < units ? max(0, min(8, a.D - col)) : 0, vec && u < units, v[b]);
-                at[b] = u < units ? kb * (BN * 128) + t * 128 + (((u16 >> 1) ^ (t & 7)) << 4) + (u16 & 1) * 8 : -1;
-                sat[b] = (c & 3) == 0 ? (int)xsf_off + kb * 512 + t * 16 + (u16 >> 2) : -1;
-            }
+                for (int b = 0; b < kBatch; ++b) load8(xc + min(t0 + b, a.T - 1) * a.ldx, n, vec, v[b]);
 #pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-                uint32_t m = 0;
+                for (int b = 0; b < kBatch; ++b) {
+                    const int t = t0 + b;
+                    uint32_t m = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[b][i]));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                const uint32_t sb = ue8m0_of(m, 1e-4f, kInv448);
-                const float inv = sb == 255u ? 0.f : ue8m0_inv(sb);
-                uint32_t w[2];
+                    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[b][i]));
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                    const uint32_t sb = ue8m0_of(m, 1e-4f, kInv448);
+                    const float inv = sb == 255u ? 0.f : ue8m0_inv(sb);
+                    uint32_t w[2];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i] * inv, v[b][4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i + 2] * inv, v[b][4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-                    w[i] = sb == 255u ? 0u : lo | hi << 16;
-                }
-                if (at[b] >= 0) {
-                    *reinterpret_cast<uint2*>(base_g + at[b]) = make_uint2(w[0], w[1]);
-                    if (sat[b] >= 0) base_g[sat[b]] = (uint8_t)sb;
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i] * inv, v[b][4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i + 2] * inv, v[b][4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                        w[i] = sb == 255u ? 0u : lo | hi << 16;
+                    }
+                    if (in && t < a.T) {
+                        *reinterpret_cast<uint2*>(base_g + kb * (BN * 128) + t * 128 + (((u16 >> 1) ^ (t & 7)) << 4) + (u16 & 1) * 8) = make_uint2(w[0], w[1]);
+                        if ((c & 3) == 0) base_g[xsf_off + kb * 512 + t * 16 + (u16 >> 2)] = (uint8_t)sb;
+                    }
                 }
             }
         }
@@ -490,14 +504,14 @@ template <int BN>
 struct DownCfg {
     static constexpr int kA = 128 * 128;
     static constexpr int kStage = kA + BN * 128 + 1024;         // weights, h tile, both scale chunks
-    static constexpr int kStages = (111 * 1024 - 1024 - 256) / kStage;   // two CTAs per SM, each with 1 KB of static tables
+    static constexpr int kStages = 10;                          // one CTA per SM: 87 KB of weights in flight
     static constexpr int kTmem = 64;                            // BN accumulator columns + 2 x 8 of scales
     static constexpr size_t kSmem = (size_t)kStages * kStage + 1024 + 256;
     static_assert((size_t)BN * 128 * 4 <= (size_t)kStages * kStage && kStages * 16 + 16 <= 256, "smem");
 };
 
 template <int BN, typename TO>
-__global__ void __launch_bounds__(kDownThreads, 2)
+__global__ void __launch_bounds__(kDownThreads, 1)
 fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a) {
     using C = DownCfg<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -743,11 +757,13 @@ int launch_down(MoeArgs a, const void* w2, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
     const int tiles = (a.D + 127) / 128;
     const int64_t pairs = (int64_t)a.T * a.topk, units = (pairs < a.E ? pairs : a.E) * a.nit;
-    // as many K splits as keep all clusters resident at two CTAs per SM, with two blocks each at least
+    // As many K splits as keep all clusters resident at one CTA per SM, with two blocks each at least.  (Two CTAs per SM
+    // take turns on the tensor core, which costs a change of accumulator per block: 0.41 us per block and CTA against
+    // 0.165 us alone, and the SMs that got only one CTA wait for the others.)
     static int resident[9] = {};
     int S = 1;
     for (int c = 2; c <= 8; ++c)
-        if (units >= 2 * c && tiles <= resident_clusters(k, c, kDownThreads, DownCfg<BN>::kSmem, 2, resident)) S = c;
+        if (units >= 2 * c && tiles <= resident_clusters(k, c, kDownThreads, DownCfg<BN>::kSmem, 1, resident)) S = c;
     a.S = S;
     return (int)fp4_launch(k, dim3((unsigned)(tiles * S)), dim3(kDownThreads), DownCfg<BN>::kSmem, st, S, true, tw, a);
 }
