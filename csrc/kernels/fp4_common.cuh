@@ -49,6 +49,25 @@ inline cudaError_t fp4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     return e;
 }
 
+// cuTensorMapEncodeTiled, 2-D, 128-byte swizzle, no interleave, zero fill.
+inline int fp4_encode_tmap(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                           const cuuint32_t* box, const cuuint32_t* estr) {
+    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeFn fn = nullptr;
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || !p)
+            return (int)cudaErrorNotSupported;
+        fn = (EncodeFn)p;
+    }
+    const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+}
+
 // cudaFuncSetAttribute once per kernel and device.
 template <typename F>
 inline cudaError_t fp4_allow_smem(F kernel, size_t bytes, unsigned long long& done) {
@@ -99,6 +118,14 @@ __device__ __forceinline__ bool elect_one() {
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
     return p != 0;
 }
+
+// Tiled TMA store of a box in shared memory (clipped at the tensor's ends) and its bulk groups (per thread).
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t smem_src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_src) : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+template <int N> __device__ __forceinline__ void bulk_wait() { asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory"); }
 
 // ---- clusters ------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {

@@ -23,23 +23,26 @@ using namespace fp4;
 
 constexpr int kBK = 256;          // values per stage row (128 bytes)
 constexpr int kGThreads = 320;
-constexpr int kEpi = 256;         // epilogue threads
+constexpr int kEpi = 256;         // epilogue threads: two warps per lane quarter
 
-template <int FMT, int BN>
+template <int FMT, int BN, bool SWAP>
 struct GemmCfg {
     static constexpr int kChunks = FMT == kMxFp4 ? 2 : 4;              // scale chunks of a stage per 128 rows
     static constexpr int kQAtoms = (BN + 127) / 128;
     static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
     static constexpr int kSfa = 512 * kChunks, kSfb = kSfa * kQAtoms;
     static constexpr int kStageBytes = (kABytes + kBBytes + kSfa + kSfb + 1023) / 1024 * 1024;
-    static constexpr int kBudget = BN <= 32 ? 113 * 1024 : 225 * 1024;  // up to 32 columns: two CTAs per SM
-    static constexpr int kStages = (kBudget - 1280) / kStageBytes;
+    // P = X: each epilogue warp stages its rows of the output in two buffers of 32 rows x 128 bytes
+    static constexpr int kStaging = SWAP ? 0 : (kEpi / 32) * 2 * 4096;
+    static constexpr int kBudget = BN <= 32 ? 112 * 1024 : 227 * 1024;  // up to 32 columns: two CTAs per SM
+    static constexpr int kBars = 512;
+    static constexpr int kStages = (kBudget - kBars - kStaging) / kStageBytes;
     static constexpr int kSfCols = 4 * kChunks * (1 + kQAtoms);        // tensor memory columns of a stage's scales
     static constexpr int kAcc = BN < 32 ? 32 : BN;
     static constexpr int kNeed = kAcc + 2 * kSfCols;
     static constexpr int kTmem = kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
-    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + 1024 + 256;
-    static_assert(kStages >= 3 && kStages * 16 + 32 <= 256, "stages");
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kStaging + kBars;
+    static_assert(kStages >= 3 && kStages * 16 + 32 <= kBars, "stages");
     static_assert((size_t)BN * 128 * 4 <= (size_t)kStages * kStageBytes, "the partial tile reuses the stages");
 };
 
@@ -71,36 +74,89 @@ struct GemmArgs {
     int* status;
 };
 
-template <typename T, bool SWAP, int BN>
-__device__ __forceinline__ void store_direct(const GemmArgs& a, uint32_t tmem, int warp, int lane, int64_t p0, int64_t q0) {
-    // warp w of 0..7: lane quarter w & 3, column half w >> 2 (all columns in 16s)
+// P = W (few rows of X): lane = output column, a warp's store is 32 neighbouring outputs of one row.
+template <typename T, int BN>
+__device__ __forceinline__ void store_columns(const GemmArgs& a, uint32_t tmem, int warp, int lane, int64_t p0, int64_t q0) {
+    // warp w of 0..7: lane quarter w & 3, column half w >> 2
     const int quarter = warp & 3;
     const int64_t p = p0 + quarter * 32 + lane;
-    T* out = reinterpret_cast<T*>(a.out);
     constexpr int kHalf = BN >= 32 ? BN / 2 : BN;
     if (BN < 32 && warp >= 4) return;
     const int c0 = (warp >> 2) * kHalf;
 #pragma unroll 1
-    for (int c = c0; c < c0 + kHalf; c += 16) {
-        if (q0 + c >= a.Q) break;
+    for (int c = c0; c < c0 + kHalf && q0 + c < a.Q; c += 16) {
         uint32_t r[16];
         tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c, r);
         tmem_ld_wait();
         if (p >= a.P) continue;
         const int n = (int)min((int64_t)16, a.Q - (q0 + c));
-        if (SWAP) {   // lane = output column: a warp's store is 32 neighbouring outputs of row q0 + c + j
+        T* out = reinterpret_cast<T*>(a.out) + (q0 + c) * a.ldo + p;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                if (j < n) out[(q0 + c + j) * a.ldo + p] = from_f32<T>(__uint_as_float(r[j]) * a.alpha);
-        } else {
-            float v[8];
-            T* o = out + p * a.ldo + q0 + c;
+        for (int j = 0; j < 16; ++j)
+            if (j < n) out[j * a.ldo] = from_f32<T>(__uint_as_float(r[j]) * a.alpha);
+    }
+}
+
+// P = X: a lane holds a row's outputs side by side.  They go through two 32-row x 128-byte buffers of this warp (16-byte
+// units swizzled as TMA's 128-byte mode: no bank conflicts) and leave as TMA stores, which the tensor core does not wait
+// for: the accumulator is given back as soon as it is read.  Rows that TMA cannot address (base or row stride not a
+// multiple of 16 bytes) leave as stores of 32 neighbouring outputs.
+template <typename T, int BN>
+__device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap* tmap_o, uint32_t tmem, uint32_t buf0, int warp, int lane,
+                                           int64_t p0, int64_t q0, uint32_t acc_empty, int& turn) {
+    constexpr int kCols = 128 / (int)sizeof(T), kChunks = BN / 2 / kCols;   // columns of a buffer, buffers of this warp's half
+    static_assert(kChunks >= 1, "a warp's half is a buffer at least");
+    const int quarter = warp & 3, c0 = (warp >> 2) * (BN / 2);
+    const int64_t row0 = p0 + quarter * 32;
+#pragma unroll 1
+    for (int ch = 0; ch < kChunks; ++ch, turn ^= 1) {   // the buffers take turns, across tiles too
+        const uint32_t buf = buf0 + (uint32_t)turn * 4096;
+        const int64_t q = q0 + c0 + ch * kCols;
+        if (lane == 0) bulk_wait_read<1>();      // the store before the last has left this buffer
+        __syncwarp();
+        uint32_t r[kCols];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+        for (int c = 0; c < kCols; c += 16) tmem_ld16(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(c0 + ch * kCols + c), *reinterpret_cast<uint32_t(*)[16]>(r + c));
+        tmem_ld_wait();
+        if (ch == kChunks - 1) {
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty);
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(r[8 * h + j]) * a.alpha;
-                if (n > 8 * h) store8(o + 8 * h, n - 8 * h, a.vec != 0, v);
+        for (int u = 0; u < 8; ++u) {            // 16-byte units
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(__uint_as_float(r[u * 4 + i]) * a.alpha);
+                else w[i] = pack2<T>(__uint_as_float(r[u * 8 + 2 * i]) * a.alpha, __uint_as_float(r[u * 8 + 2 * i + 1]) * a.alpha);
             }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + ((u ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+        }
+        if (a.vec) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                if (q < a.Q && row0 < a.P) tma_store_2d(tmap_o, (int)q, (int)row0, buf);
+                bulk_commit();
+            }
+        } else {
+            __syncwarp();
+            const int rows = (int)min((int64_t)32, a.P - row0);
+#pragma unroll 1
+            for (int i = 0; i < rows; ++i) {
+                T* out = reinterpret_cast<T*>(a.out) + (row0 + i) * a.ldo + q;
+#pragma unroll
+                for (int h = 0; h < kCols; h += 32) {
+                    const int c = h + lane, byte = c * (int)sizeof(T);
+                    T v;
+                    const uint32_t at = buf + i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15);
+                    if constexpr (sizeof(T) == 4) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+                    else { uint16_t u; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(at) : "memory"); v = *reinterpret_cast<T*>(&u); }
+                    if (q + c < a.Q) out[c] = v;
+                }
+            }
+            __syncwarp();
         }
     }
 }
@@ -125,15 +181,18 @@ __device__ __forceinline__ void store_reduced(const GemmArgs& a, uint32_t part, 
 
 template <int FMT, int BN, bool SWAP>
 __global__ void __launch_bounds__(kGThreads, BN <= 32 ? 2 : 1)
-fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q, const GemmArgs a) {
-    using C = GemmCfg<FMT, BN>;
-    extern __shared__ uint8_t smem_raw[];
-    const uint32_t base = (tc::smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t bars = base + C::kStages * C::kStageBytes;
+fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
+                const __grid_constant__ CUtensorMap tmap_o, const GemmArgs a) {
+    using C = GemmCfg<FMT, BN, SWAP>;
+    // no static shared memory: the swizzled tiles start on 1024 bytes without padding (three stages and the staging buffers
+    // of the widest tile fill all but 768 bytes)
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t base = tc::smem_u32(smem_raw);
+    const uint32_t staging = base + C::kStages * C::kStageBytes, bars = staging + C::kStaging;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (C::kStages + s); };
     const uint32_t acc_full = bars + 16u * C::kStages, acc_empty = acc_full + 8u, tmem_slot = acc_full + 16u;
-    __shared__ int s_fail;
+    int& s_fail = *reinterpret_cast<int*>(smem_raw + (acc_full + 20u - base));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = a.splits, rank = S > 1 ? (int)cluster_rank() : 0;
@@ -153,7 +212,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     };
 
     if (threadIdx.x == 0) {
-        s_fail = 0;
+        s_fail = (base & 1023u) != 0;   // (never: then nothing is stored and the status says so)
         for (int s = 0; s < C::kStages; ++s) {
             tc::mbar_init(full(s), 1);
             tc::mbar_init(empty(s), 1);
@@ -163,6 +222,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         tc::mbar_fence_init();
         tc::prefetch_tmap(&tmap_p);
         tc::prefetch_tmap(&tmap_q);
+        if (!SWAP) tc::prefetch_tmap(&tmap_o);
     }
     if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
     tc::tc_fence_before();
@@ -257,7 +317,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         const int w = warp - 2;
         // warps 2..9: TMEM lane quarter = warp & 3
         const int quarter_warp = (warp & 3) | (w >= 4 ? 4 : 0);
-        int tile_no = 0;
+        int tile_no = 0, turn = 0;
         for (int t = first; t < n_tiles; t += step, ++tile_no) {
             int64_t p0, q0;
             tile_at(t, p0, q0);
@@ -284,15 +344,24 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                     }
                 }
             } else if (go) {
-                if (a.dtype == kBf16) store_direct<__nv_bfloat16, SWAP, BN>(a, tmem, quarter_warp, lane, p0, q0);
-                else if (a.dtype == kF16) store_direct<__half, SWAP, BN>(a, tmem, quarter_warp, lane, p0, q0);
-                else store_direct<float, SWAP, BN>(a, tmem, quarter_warp, lane, p0, q0);
+                if constexpr (SWAP) {
+                    if (a.dtype == kBf16) store_columns<__nv_bfloat16, BN>(a, tmem, quarter_warp, lane, p0, q0);
+                    else if (a.dtype == kF16) store_columns<__half, BN>(a, tmem, quarter_warp, lane, p0, q0);
+                    else store_columns<float, BN>(a, tmem, quarter_warp, lane, p0, q0);
+                } else {
+                    const uint32_t buf = staging + (uint32_t)w * 8192;
+                    if (a.dtype == kBf16) store_rows<__nv_bfloat16, BN>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
+                    else if (a.dtype == kF16) store_rows<__half, BN>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
+                    else store_rows<float, BN>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
+                    continue;   // (store_rows gave the accumulator back)
+                }
             }
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty);   // also after a failed wait
             if (!go) break;
         }
+        if (!SWAP && S == 1 && lane == 0) bulk_wait<0>();
     }
     __syncwarp();
     tc::tc_fence_before();
@@ -326,20 +395,34 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     }
 }
 
+// Output [rows, cols] in boxes of 32 rows x 128 bytes, 128-byte swizzle.
+int make_tmap_out(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t ld, int dtype) {
+    static_assert(kF32 == 0 && kBf16 == 1 && kF16 == 2, "the order of the table below");
+    const CUtensorMapDataType types[3] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16};
+    const uint64_t esz = dtype == kF32 ? 4 : 2;
+    cuuint64_t dims[2] = {cols, rows};
+    cuuint64_t strides[1] = {ld * esz};
+    cuuint32_t box[2] = {(cuuint32_t)(128 / esz), 32};
+    cuuint32_t estr[2] = {1, 1};
+    return fp4_encode_tmap(map, types[dtype], base, dims, strides, box, estr);
+}
+
 template <int FMT, int BN, bool SWAP>
 int launch_gemm(const GemmArgs& a, const void* pc, const void* qc, int grid, cudaStream_t st) {
-    using C = GemmCfg<FMT, BN>;
-    CUtensorMap tp, tq;
+    using C = GemmCfg<FMT, BN, SWAP>;
+    CUtensorMap tp, tq, to;
     const uint64_t bytes = (uint64_t)(64 * groups(a.K));
     // the row end (a multiple of 64 bytes) lies inside a 128-byte box of the last stage: what is behind it reads zero
     int rc = fb_make_tmap_2d(&tp, pc, (uint64_t)a.P, bytes, 128, 128, 1);
     if (!rc) rc = fb_make_tmap_2d(&tq, qc, (uint64_t)a.Q, bytes, BN, 128, 1);
+    to = tp;   // (not used by P = W or an output that TMA cannot address)
+    if (!rc && !SWAP && a.vec) rc = make_tmap_out(&to, a.out, (uint64_t)a.P, (uint64_t)a.Q, (uint64_t)a.ldo, a.dtype);
     if (rc) return rc;
     auto k = fp4_gemm_kernel<FMT, BN, SWAP>;
     static unsigned long long allowed = 0;
     cudaError_t e = fp4_allow_smem(k, C::kSmem, allowed);
     if (e != cudaSuccess) return (int)e;
-    return (int)fp4_launch(k, dim3((unsigned)grid), dim3(kGThreads), C::kSmem, st, a.splits, a.pdl != 0, tp, tq, a);
+    return (int)fp4_launch(k, dim3((unsigned)grid), dim3(kGThreads), C::kSmem, st, a.splits, a.pdl != 0, tp, tq, to, a);
 }
 
 template <int FMT>
@@ -366,14 +449,25 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
     }
     a.P = M; a.Q = N; a.sfp = xs; a.sfq = ws;
     a.tiles_p = (int)((M + 127) / 128);
-    const int64_t t256 = (int64_t)a.tiles_p * ((N + 255) / 256), t128 = (int64_t)a.tiles_p * ((N + 127) / 128);
-    // tiles of 256 columns unless the narrower ones fill the last wave better
-    const bool wide = (t256 + sms - 1) / sms * 2 <= (t128 + sms - 1) / sms;
-    a.tiles_q = (int)((N + (wide ? 255 : 127)) / (wide ? 256 : 128));
-    const int64_t tiles = wide ? t256 : t128;
-    if (tiles > 0x3fffffff) return (int)cudaErrorInvalidValue;
+    // Tile width and K split by the clocks of the longest-running CTA: a stage (256 columns of K) takes about 600 on 256
+    // output columns and 470 on 128 (four MMAs and the scale copies), a tile about 1500 at its ends that the next one does
+    // not hide, an exchange between split CTAs 3000.  Clusters of a split stay resident (33 of 4, 15 of 8).
+    const int resident[4] = {sms, 74, 33, 15};
+    double cost = 0;
+    bool wide = true;
     int S = 1;
-    while (S < 8 && tiles * S * 2 <= sms && nkb >= 4 * S) S *= 2;
+    for (int w = 0; w < 2; ++w) {
+        const int64_t tiles = (int64_t)a.tiles_p * ((N + (w ? 255 : 127)) / (w ? 256 : 128));
+        for (int l = 0; l < 4; ++l) {
+            const int s = 1 << l;
+            if (l && (tiles > resident[l] || nkb < 2 * s)) break;
+            const double c = (double)((tiles + sms - 1) / sms) * ((double)((nkb + s - 1) / s) * (w ? 600 : 470) + 1500) + (s > 1 ? 3000 : 0);
+            if (cost == 0 || c < cost) { cost = c; wide = w; S = s; }
+        }
+    }
+    a.tiles_q = (int)((N + (wide ? 255 : 127)) / (wide ? 256 : 128));
+    const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;
+    if (tiles > 0x3fffffff) return (int)cudaErrorInvalidValue;
     a.splits = S;
     const int grid = S > 1 ? (int)tiles * S : (int)(tiles < sms ? tiles : sms);
     if (wide) return launch_gemm<FMT, 256, false>(a, xc, wc, grid, st);

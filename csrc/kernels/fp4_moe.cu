@@ -655,26 +655,12 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
 
 // Tensor map of 4-bit codes [rows][cols] (cols a multiple of 128), boxes of 128 codes x box_rows in the padded form.
 int make_tmap_u4(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows) {
-    typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-    static EncodeFn fn = nullptr;
-    if (!fn) {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || !p)
-            return (int)cudaErrorNotSupported;
-        fn = (EncodeFn)p;
-    }
     if (((uintptr_t)base & 31) || cols % 128) return (int)cudaErrorInvalidValue;
     cuuint64_t dims[2] = {cols, rows};
     cuuint64_t strides[1] = {cols / 2};
     cuuint32_t box[2] = {128, box_rows};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, 2, const_cast<void*>(base), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
+    return fp4_encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B, base, dims, strides, box, estr);
 }
 
 constexpr int kSms = 148;
