@@ -13,7 +13,7 @@
 // x / s with s a power of two is a product with the exact reciprocal.  For an e4m3 scale the quotient has to be the
 // correctly rounded one (a bf16 value over a 4-bit scale often lies exactly on the border of two codes, and a product
 // with the rounded reciprocal falls to either side): Markstein's correction, q0 = u r, q = q0 + (u - q0 s) r with
-// r = rn(1 / s), two FMAs per value after one division per block.
+// r = rn(1 / s), two FMAs per value after one reciprocal per block.
 #include "fp4_common.cuh"
 
 namespace {
@@ -24,11 +24,6 @@ __device__ int g_fp4_status[4];
 
 constexpr int kQThreads = 256;
 constexpr int kQCols = 256;   // columns of a warp's pass
-
-__device__ __forceinline__ float div_by(float u, float s, float r) {
-    const float q0 = __fmul_rn(u, r);
-    return __fmaf_rn(__fmaf_rn(-q0, s, u), r, q0);
-}
 
 // Tile of this CTA: rows (tile * 128 + 8 * sub + warp) + 32 g, columns 256 * ct ...; bt = matrix of the batch.
 struct Place { int64_t bt; int64_t row; int64_t tile; int i; int64_t col; };
@@ -67,31 +62,8 @@ fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int ve
     uint32_t word[4];   // this lane's group of four blocks: their scale bytes, row by row
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        if (FMT == kNvFp4 && scaled) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[g][j] = div_by(v[g][j], ts, inv_ts);
-        }
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[g][j]));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        if (FMT == kMxFp4) m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        uint32_t byte, code;
-        if (FMT == kMxFp4) {
-            byte = ue8m0_of(m, 6.f * 1.17549435e-38f, kInv6);
-            const float inv = ue8m0_inv(min(byte, 253u));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[g][j] *= inv;
-        } else {
-            byte = m >= kInfBits ? 0x7fu
-                                 : (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(fmaxf(__uint_as_float(m), 6.f / 512.f), 6.f),
-                                                                   __NV_SATFINITE, __NV_E4M3);
-            const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
-            const float s = __half2float(*reinterpret_cast<const __half*>(&hr)), r = __frcp_rn(s);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[g][j] = div_by(v[g][j], s, r);
-        }
-        code = m >= kInfBits ? 0u : e2m1x8(v[g]);   // a block that is not finite: NaN scale, zero codes
+        uint32_t byte;
+        const uint32_t code = quantize8<FMT>(v[g], scaled, ts, inv_ts, byte);
         const int64_t r = p.row + 32 * g;
         // columns in 8s up to the padded row end (64 bytes per group of 128 columns)
         if (r < rows && p.col < 128 * G)

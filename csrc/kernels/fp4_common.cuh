@@ -186,6 +186,41 @@ __device__ __forceinline__ uint32_t ue8m0_of(uint32_t amax_bits, float floor, fl
 // 1 / 2^(e - 127) for e in 1..253
 __device__ __forceinline__ float ue8m0_inv(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
+// u / s rounded to nearest, from r = rn(1 / s): Markstein's correction of the product u r.
+__device__ __forceinline__ float div_by(float u, float s, float r) {
+    const float q0 = __fmul_rn(u, r);
+    return __fmaf_rn(__fmaf_rn(-q0, s, u), r, q0);
+}
+
+// Eight consecutive values of a row -> their codes (value j in nibble j) and the scale byte of their block, which is this
+// lane and its neighbours (four lanes of mxfp4, two of nvfp4; whole warps call).  scaled: nvfp4 with a tensor scale ts.
+template <int FMT>
+__device__ __forceinline__ uint32_t quantize8(float (&v)[8], bool scaled, float ts, float inv_ts, uint32_t& byte) {
+    if (FMT == kNvFp4 && scaled) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = div_by(v[j], ts, inv_ts);
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    if (FMT == kMxFp4) m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    if (FMT == kMxFp4) {
+        byte = ue8m0_of(m, 6.f * 1.17549435e-38f, kInv6);
+        const float inv = ue8m0_inv(min(byte, 253u));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= inv;
+    } else {
+        byte = m >= kInfBits ? 0x7fu
+                             : (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(fmaxf(__uint_as_float(m), 6.f / 512.f), 6.f), __NV_SATFINITE, __NV_E4M3);
+        const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
+        const float s = __half2float(*reinterpret_cast<const __half*>(&hr)), r = __frcp_rn(s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = div_by(v[j], s, r);
+    }
+    return m >= kInfBits ? 0u : e2m1x8(v);   // a block that is not finite: NaN scale, zero codes
+}
+
 // ---- values of the three element types -----------------------------------------------------------
 template <int DT> struct Elem;
 template <> struct Elem<kF32> { using T = float; };

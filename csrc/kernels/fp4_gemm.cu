@@ -24,24 +24,27 @@ using namespace fp4;
 constexpr int kBK = 256;          // values per stage row (128 bytes)
 constexpr int kGThreads = 320;
 constexpr int kEpi = 256;         // epilogue threads: two warps per lane quarter
+constexpr int kQxBlocks = 8;      // QX: blocks of X that a CTA holds
 
-template <int FMT, int BN, bool SWAP>
+template <int FMT, int BN, bool SWAP, bool QX>
 struct GemmCfg {
     static constexpr int kChunks = FMT == kMxFp4 ? 2 : 4;              // scale chunks of a stage per 128 rows
     static constexpr int kQAtoms = (BN + 127) / 128;
     static constexpr int kABytes = 128 * 128, kBBytes = BN * 128;
     static constexpr int kSfa = 512 * kChunks, kSfb = kSfa * kQAtoms;
-    static constexpr int kStageBytes = (kABytes + kBBytes + kSfa + kSfb + 1023) / 1024 * 1024;
+    static constexpr int kXBlock = kBBytes + kSfb;   // QX: a block of X (256 columns of K) lives outside the stages
+    static constexpr int kStageBytes = (kABytes + kSfa + (QX ? 0 : kXBlock) + 1023) / 1024 * 1024;
     // P = X: each epilogue warp stages its rows of the output in two buffers of 32 rows x 128 bytes
     static constexpr int kStaging = SWAP ? 0 : (kEpi / 32) * 2 * 4096;
     static constexpr int kBudget = BN <= 32 ? 112 * 1024 : 227 * 1024;  // up to 32 columns: two CTAs per SM
     static constexpr int kBars = 512;
-    static constexpr int kStages = (kBudget - kBars - kStaging) / kStageBytes;
+    static constexpr int kXRoom = QX ? kQxBlocks * kXBlock : 0;
+    static constexpr int kStages = (kBudget - kBars - kStaging - kXRoom) / kStageBytes;
     static constexpr int kSfCols = 4 * kChunks * (1 + kQAtoms);        // tensor memory columns of a stage's scales
     static constexpr int kAcc = BN < 32 ? 32 : BN;
     static constexpr int kNeed = kAcc + 2 * kSfCols;
     static constexpr int kTmem = kNeed <= 128 ? 128 : kNeed <= 256 ? 256 : 512;
-    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kStaging + kBars;
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kXRoom + kStaging + kBars;
     static_assert(kStages >= 3 && kStages * 16 + 32 <= kBars, "stages");
     static_assert((size_t)BN * 128 * 4 <= (size_t)kStages * kStageBytes, "the partial tile reuses the stages");
 };
@@ -66,6 +69,10 @@ __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uin
 
 struct GemmArgs {
     const uint8_t *sfp, *sfq;
+    const void* x;            // QX: the rows to quantise (row stride ldx, element type xdt; tensor scale xts if scaled)
+    int64_t ldx;
+    float xts, xinv;
+    int xdt, scaled;
     void* out;
     int64_t ldo;
     int64_t P, Q, K;
@@ -179,19 +186,56 @@ __device__ __forceinline__ void store_reduced(const GemmArgs& a, uint32_t part, 
     }
 }
 
-template <int FMT, int BN, bool SWAP>
+// The K range of X (kb0 .. kb1 in blocks of 256 columns) quantised into operand form: per block [BN][128 bytes] swizzled
+// codes, then the scale chunks.  Columns behind K count as zeros (their scales have to be numbers).
+template <int FMT, typename C>
+__device__ __forceinline__ void quantize_x(const GemmArgs& a, uint8_t* room, int t, int kb0, int kb1, uint32_t x_full, int lane) {
+    const int units = (kb1 - kb0) * 32;                    // of eight columns
+    const int esz = a.xdt == kF32 ? 4 : 2;
+    const bool vec = ((uintptr_t)a.x & 15) == 0 && a.ldx * esz % 16 == 0;
+#pragma unroll 1
+    for (int64_t m = 0; m < a.Q; ++m) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < units; c0 += kEpi) {
+            const int c = c0 + t;
+            const int64_t col = (int64_t)kb0 * kBK + 8 * c;
+            const int n = c < units ? (int)max((int64_t)0, min((int64_t)8, a.K - col)) : 0;
+            const int64_t at = m * a.ldx + (n ? col : 0);
+            float v[8];
+            if (a.xdt == kBf16) load8(reinterpret_cast<const __nv_bfloat16*>(a.x) + at, n, vec, v);
+            else if (a.xdt == kF16) load8(reinterpret_cast<const __half*>(a.x) + at, n, vec, v);
+            else load8(reinterpret_cast<const float*>(a.x) + at, n, vec, v);
+            uint32_t byte;
+            const uint32_t code = quantize8<FMT>(v, a.scaled != 0, a.xts, a.xinv, byte);
+            if (c < units) {
+                uint8_t* blk = room + (c >> 5) * C::kXBlock;
+                const int u = c & 31;                      // 4 bytes of codes each
+                *reinterpret_cast<uint32_t*>(blk + m * 128 + (((u >> 2) ^ (int)(m & 7)) << 4) + (u & 3) * 4) = code;
+                constexpr int kPer = FMT == kMxFp4 ? 4 : 2;
+                const int b = u / kPer;                    // block of the 256 columns
+                if (u % kPer == 0) blk[C::kBBytes + (b >> 2) * 512 + m * 16 + (b & 3)] = (uint8_t)byte;
+            }
+        }
+    }
+    fence_proxy_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(x_full);
+}
+
+template <int FMT, int BN, bool SWAP, bool QX>
 __global__ void __launch_bounds__(kGThreads, BN <= 32 ? 2 : 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                 const __grid_constant__ CUtensorMap tmap_o, const GemmArgs a) {
-    using C = GemmCfg<FMT, BN, SWAP>;
+    using C = GemmCfg<FMT, BN, SWAP, QX>;
     // no static shared memory: the swizzled tiles start on 1024 bytes without padding (three stages and the staging buffers
     // of the widest tile fill all but 768 bytes)
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     const uint32_t base = tc::smem_u32(smem_raw);
-    const uint32_t staging = base + C::kStages * C::kStageBytes, bars = staging + C::kStaging;
+    const uint32_t xroom = base + C::kStages * C::kStageBytes;   // (the SWAP forms have no staging buffers, the others no X room)
+    const uint32_t staging = xroom, bars = xroom + C::kXRoom + C::kStaging;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (C::kStages + s); };
-    const uint32_t acc_full = bars + 16u * C::kStages, acc_empty = acc_full + 8u, tmem_slot = acc_full + 16u;
+    const uint32_t acc_full = bars + 16u * C::kStages, acc_empty = acc_full + 8u, tmem_slot = acc_full + 16u, x_full = acc_full + 24u;
     int& s_fail = *reinterpret_cast<int*>(smem_raw + (acc_full + 20u - base));
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -219,6 +263,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         }
         tc::mbar_init(acc_full, 1);
         tc::mbar_init(acc_empty, kEpi / 32);
+        if (QX) tc::mbar_init(x_full, kEpi / 32);
         tc::mbar_fence_init();
         tc::prefetch_tmap(&tmap_p);
         tc::prefetch_tmap(&tmap_q);
@@ -230,7 +275,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     tc::tc_fence_after();
     uint32_t tmem;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
-    const uint32_t a_off = 0, b_off = C::kABytes, sfa_off = b_off + C::kBBytes, sfb_off = sfa_off + C::kSfa;
+    const uint32_t a_off = 0, b_off = C::kABytes, sfa_off = b_off + (QX ? 0 : C::kBBytes), sfb_off = sfa_off + C::kSfa;
 
     if (warp == 0) {
         if (elect_one()) {
@@ -241,6 +286,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                 bulk_load(base + s * C::kStageBytes + sfa_off, a.sfp + ((p0 / 128) * Cch + (int64_t)kb * C::kChunks) * 512, 512 * nch, full(s));
             };
             auto issue_q = [&](int s, int kb, int64_t q0, int nch) {
+                if (QX) return;
                 tc::tma_load_2d(base + s * C::kStageBytes + b_off, &tmap_q, kb * 128, (int)q0, full(s));
                 for (int at = 0; at < qatoms; ++at)
                     if (q0 / 128 + at < q_rowtiles)
@@ -249,7 +295,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
             };
             auto arm = [&](int s, int64_t q0, int nch) {
                 const int at = (int)min((int64_t)qatoms, q_rowtiles - q0 / 128);
-                tc::mbar_expect_tx(full(s), C::kABytes + C::kBBytes + 512 * nch * (1 + at));
+                tc::mbar_expect_tx(full(s), QX ? C::kABytes + 512 * nch : C::kABytes + C::kBBytes + 512 * nch * (1 + at));
             };
             auto chunks = [&](int kb) { return (int)min((int64_t)C::kChunks, Cch - (int64_t)kb * C::kChunks); };
             int it = 0;
@@ -283,6 +329,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         if (elect_one()) {
             int it = 0, tile_no = 0;
             bool ok = true;
+            if (QX && !tc::mbar_wait(x_full, 0)) { atomicExch(&s_fail, 1); ok = false; }
             for (int t = first; t < n_tiles && ok; t += step, ++tile_no) {
                 if (tile_no && !tc::mbar_wait(acc_empty, (tile_no - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
                 tc::tc_fence_after();
@@ -298,9 +345,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                         tmem_cp_sf(sfa_t + 4 * c, sf_desc(st + sfa_off + 512 * c));
 #pragma unroll
                         for (int at = 0; at < C::kQAtoms; ++at)   // word c of all atoms side by side: 4 columns per 128 rows
-                            tmem_cp_sf(sfb_t + 4 * (c * C::kQAtoms + at), sf_desc(st + sfb_off + at * C::kSfa + 512 * c));
+                            tmem_cp_sf(sfb_t + 4 * (c * C::kQAtoms + at), sf_desc((QX ? xroom + (kb - kb0) * C::kXBlock + C::kBBytes : st + sfb_off) + at * C::kSfa + 512 * c));
                     }
-                    const uint64_t ad = tc::umma_desc_sw128(st + a_off), bd = tc::umma_desc_sw128(st + b_off);
+                    const uint64_t ad = tc::umma_desc_sw128(st + a_off), bd = tc::umma_desc_sw128(QX ? xroom + (kb - kb0) * C::kXBlock : st + b_off);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         if (k >= steps) break;
@@ -317,6 +364,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         const int w = warp - 2;
         // warps 2..9: TMEM lane quarter = warp & 3
         const int quarter_warp = (warp & 3) | (w >= 4 ? 4 : 0);
+        if constexpr (QX) quantize_x<FMT, C>(a, smem_raw + (xroom - base), threadIdx.x - 64, kb0, kb1, x_full, lane);
         int tile_no = 0, turn = 0;
         for (int t = first; t < n_tiles; t += step, ++tile_no) {
             int64_t p0, q0;
@@ -407,23 +455,26 @@ int make_tmap_out(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, ui
     return fp4_encode_tmap(map, types[dtype], base, dims, strides, box, estr);
 }
 
-template <int FMT, int BN, bool SWAP>
+template <int FMT, int BN, bool SWAP, bool QX = false>
 int launch_gemm(const GemmArgs& a, const void* pc, const void* qc, int grid, cudaStream_t st) {
-    using C = GemmCfg<FMT, BN, SWAP>;
+    using C = GemmCfg<FMT, BN, SWAP, QX>;
     CUtensorMap tp, tq, to;
     const uint64_t bytes = (uint64_t)(64 * groups(a.K));
     // the row end (a multiple of 64 bytes) lies inside a 128-byte box of the last stage: what is behind it reads zero
     int rc = fb_make_tmap_2d(&tp, pc, (uint64_t)a.P, bytes, 128, 128, 1);
-    if (!rc) rc = fb_make_tmap_2d(&tq, qc, (uint64_t)a.Q, bytes, BN, 128, 1);
-    to = tp;   // (not used by P = W or an output that TMA cannot address)
+    tq = to = tp;   // (QX has no operand Q in memory; `to` is not used by P = W or an output that TMA cannot address)
+    if (!rc && !QX) rc = fb_make_tmap_2d(&tq, qc, (uint64_t)a.Q, bytes, BN, 128, 1);
     if (!rc && !SWAP && a.vec) rc = make_tmap_out(&to, a.out, (uint64_t)a.P, (uint64_t)a.Q, (uint64_t)a.ldo, a.dtype);
     if (rc) return rc;
-    auto k = fp4_gemm_kernel<FMT, BN, SWAP>;
+    auto k = fp4_gemm_kernel<FMT, BN, SWAP, QX>;
     static unsigned long long allowed = 0;
     cudaError_t e = fp4_allow_smem(k, C::kSmem, allowed);
     if (e != cudaSuccess) return (int)e;
     return (int)fp4_launch(k, dim3((unsigned)grid), dim3(kGThreads), C::kSmem, st, a.splits, a.pdl != 0, tp, tq, to, a);
 }
+
+constexpr int kNotTaken = -1;     // X is not quantised inside the product at these sizes
+constexpr int kQxRows = 16;       // rows times blocks of 256 columns per CTA up to which it is
 
 template <int FMT>
 int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, const uint8_t* ws, int64_t M, int64_t N, cudaStream_t st) {
@@ -436,10 +487,18 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
         a.P = N; a.Q = M; a.sfp = ws; a.sfq = xs;
         a.tiles_p = (int)((N + 127) / 128);
         a.tiles_q = 1;
+        const int resident[4] = {slots, slots / 2, bn <= 32 ? 71 : 33, bn <= 32 ? 33 : 15};   // clusters of 1, 2, 4, 8
         int S = 1;
-        while (S < 8 && a.tiles_p * S * 2 <= slots && nkb >= 4 * S) S *= 2;
+        for (int l = 1; l < 4; ++l)
+            if (a.tiles_p <= resident[l] && nkb >= 2 << l) S = 1 << l;
         a.splits = S;
         const int grid = S > 1 ? a.tiles_p * S : (a.tiles_p < slots ? a.tiles_p : slots);
+        if (a.x) {
+            // Rows that are quantised on the way: with few values per CTA its idle epilogue warps do it while the first weights
+            // arrive, and the quantiser's own launch goes.
+            if (bn > 16 || (nkb + S - 1) / S > kQxBlocks || M * ((nkb + S - 1) / S) > kQxRows) return kNotTaken;
+            return launch_gemm<FMT, 16, true, true>(a, wc, nullptr, grid, st);
+        }
         switch (bn) {
             case 16: return launch_gemm<FMT, 16, true>(a, wc, xc, grid, st);
             case 32: return launch_gemm<FMT, 32, true>(a, wc, xc, grid, st);
@@ -447,6 +506,7 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
             default: return launch_gemm<FMT, 128, true>(a, wc, xc, grid, st);
         }
     }
+    if (a.x) return kNotTaken;
     a.P = M; a.Q = N; a.sfp = xs; a.sfq = ws;
     a.tiles_p = (int)((M + 127) / 128);
     // Tile width and K split by the clocks of the longest-running CTA: a stage (256 columns of K) takes about 600 on 256
@@ -478,15 +538,13 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
 
 FB_API int fb_fp4_quantize(const void*, int64_t, int64_t, int64_t, void*, void*, int64_t, int64_t, int64_t, int64_t, float, cudaStream_t);
 
-static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, void* out, int64_t dtype, int64_t ldo, int64_t M,
-                      int64_t N, int64_t K, int64_t fmt, float alpha, int pdl, cudaStream_t st) {
-    if (M < 1 || N < 1 || K < 1 || M > 0x7fffff00ll || N > 0x7fffff00ll || K > 0x3fffff00ll || ldo < N || dtype < 0 || dtype > 2 ||
+static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, int64_t M, int64_t N, int64_t fmt, GemmArgs a,
+                      cudaStream_t st) {
+    if (M < 1 || N < 1 || a.K < 1 || M > 0x7fffff00ll || N > 0x7fffff00ll || a.K > 0x3fffff00ll || a.ldo < N || a.dtype < 0 || a.dtype > 2 ||
         (fmt != kMxFp4 && fmt != kNvFp4) || (((uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws) & 15))
         return (int)cudaErrorInvalidValue;
-    GemmArgs a = {};
-    a.out = out; a.ldo = ldo; a.K = K; a.alpha = alpha; a.dtype = (int)dtype; a.pdl = pdl;
-    const int esz = dtype == kF32 ? 4 : 2;
-    a.vec = ((uintptr_t)out & 15) == 0 && ldo * esz % 16 == 0;
+    const int esz = a.dtype == kF32 ? 4 : 2;
+    a.vec = ((uintptr_t)a.out & 15) == 0 && a.ldo * esz % 16 == 0;
     a.status = fp4_status_ptr();
     if (!a.status) return (int)cudaErrorNotSupported;
     return fmt == kMxFp4 ? gemm_fmt<kMxFp4>(a, xc, (const uint8_t*)xs, wc, (const uint8_t*)ws, M, N, st)
@@ -496,19 +554,31 @@ static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void
 // out[M, N] (row stride ldo, dtype 0 f32, 1 bf16, 2 f16) = alpha * X W^T of two 4-bit matrices of one format with K columns.
 FB_API int fb_fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, void* out, int64_t dtype, int64_t ldo,
                          int64_t M, int64_t N, int64_t K, int64_t fmt, float alpha, cudaStream_t st) {
-    return fp4_matmul(xc, xs, wc, ws, out, dtype, ldo, M, N, K, fmt, alpha, 0, st);
+    GemmArgs a = {};
+    a.out = out; a.ldo = ldo; a.K = K; a.alpha = alpha; a.dtype = (int)dtype;
+    return fp4_matmul(xc, xs, wc, ws, M, N, fmt, a, st);
 }
 
-// The same with the rows of x [M, K] (dtype xdt, row stride ldx) quantised first, into `work`: codes
-// [M][64 ceil(K / 128)], then (at the next multiple of 512) the scale chunks.  Two launches; the product's prologue and its
-// first weight tiles overlap the quantiser.
+// The same with the rows of x [M, K] (element type xdt, row stride ldx; nvfp4: tensor scale xts or 0) quantised first: inside the
+// product for few values, else by fb_fp4_quantize into `work`: codes [M][64 ceil(K / 128)], then (at the next multiple of
+// 512) the scale chunks; the product's prologue and its first weight tiles overlap that launch.
 FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, const void* wc, const void* ws, void* out,
                          int64_t dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t fmt, float xts, float alpha,
                          cudaStream_t st) {
-    if (M < 1 || K < 1 || ((uintptr_t)work & 15)) return (int)cudaErrorInvalidValue;
+    if (M < 1 || K < 1 || xdt < 0 || xdt > 2 || ldx < K || ((uintptr_t)work & 15)) return (int)cudaErrorInvalidValue;
+    GemmArgs a = {};
+    a.out = out; a.ldo = ldo; a.K = K; a.alpha = alpha; a.dtype = (int)dtype;
+    a.x = x; a.ldx = ldx; a.xdt = (int)xdt;
+    a.scaled = fmt == kNvFp4 && xts != 0.f && xts != 1.f;
+    a.xts = xts;
+    a.xinv = a.scaled ? (float)(1.0 / (double)xts) : 1.f;
+    int rc = fp4_matmul(nullptr, nullptr, wc, ws, M, N, fmt, a, st);
+    if (rc != kNotTaken) return rc;
     uint8_t* codes = (uint8_t*)work;
     uint8_t* scales = codes + (M * 64 * groups(K) + 511) / 512 * 512;
-    const int rc = fb_fp4_quantize(x, xdt, ldx, 0, codes, scales, 1, M, K, fmt, xts, st);
+    rc = fb_fp4_quantize(x, xdt, ldx, 0, codes, scales, 1, M, K, fmt, xts, st);
     if (rc) return rc;
-    return fp4_matmul(codes, scales, wc, ws, out, dtype, ldo, M, N, K, fmt, alpha, 1, st);
+    a.x = nullptr;
+    a.pdl = 1;
+    return fp4_matmul(codes, scales, wc, ws, M, N, fmt, a, st);
 }

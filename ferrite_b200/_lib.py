@@ -37,6 +37,7 @@ class KernelLib:
                 raise KernelError(f"stale kernel library: built from {self.build_id}, sources are {want}; "
                                   "rebuild with `python -m ferrite_b200.build`")
         self._fns = {}
+        self._fast = {}
         self.launches = 0  # kernels launched through this handle (entry points, not replays)
 
     def fn(self, name: str):
@@ -48,6 +49,22 @@ class KernelLib:
         return f
 
     def call(self, name: str, *args, stream: Optional[int] = None):
+        if stream is None:
+            stream = torch.cuda.current_stream().cuda_stream
+        fast = self._fast.get(name)
+        rc = None
+        if fast is not None:   # argument kinds are known from the first call: ctypes converts plain numbers by itself
+            try:
+                rc = fast(*[a.data_ptr() if type(a) is torch.Tensor else a for a in args], stream)
+            except ctypes.ArgumentError:
+                rc = None
+        if rc is None:
+            rc = self._call_by_kind(name, args, stream)
+        self.launches += 1
+        if rc != 0:
+            raise KernelError(f"{name} failed with CUDA error {rc}")
+
+    def _call_by_kind(self, name: str, args, stream: int) -> int:
         cargs = []
         for a in args:
             if isinstance(a, torch.Tensor) or hasattr(a, "data_ptr"):
@@ -64,13 +81,14 @@ class KernelLib:
                 cargs.append(a)
             else:
                 raise TypeError(f"{name}: unsupported argument {type(a)}")
-        if stream is None:
-            stream = torch.cuda.current_stream().cuda_stream
         cargs.append(ctypes.c_void_p(stream))
         rc = self.fn(name)(*cargs)
-        self.launches += 1
-        if rc != 0:
-            raise KernelError(f"{name} failed with CUDA error {rc}")
+        if name not in self._fast and all(type(c) in (ctypes.c_void_p, ctypes.c_int64, ctypes.c_float) for c in cargs):
+            fast = self.lib[name]   # a function object of its own: the other one keeps taking arguments of any kind
+            fast.restype = ctypes.c_int
+            fast.argtypes = [type(c) for c in cargs]
+            self._fast[name] = fast
+        return rc
 
 
 _LIB: Optional[KernelLib] = None

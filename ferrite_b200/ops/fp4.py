@@ -61,6 +61,13 @@ class Fp4Tensor:
             raise ValueError("codes and scales are contiguous, codes on a 32-byte and scales on a 16-byte boundary")
         self.codes, self.scales, self.fmt, self.shape, self.tensor_scale = codes, scales, fmt, shape, tensor_scale
 
+    @classmethod
+    def _of(cls, codes, scales, fmt, shape, tensor_scale):
+        """Without the checks, for parts that were made here."""
+        t = cls.__new__(cls)
+        t.codes, t.scales, t.fmt, t.shape, t.tensor_scale = codes, scales, fmt, shape, tensor_scale
+        return t
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -113,11 +120,13 @@ def _check_scale(ts: float, fmt: str) -> None:
 
 
 def _call(device: torch.device, name: str, *args) -> None:
-    if torch.cuda.current_device() == device.index:
-        _lib.lib().call(name, *args)
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch.cuda.current_device() == index:
+        _lib.lib().call(name, *args, stream=stream)
     else:
-        with torch.cuda.device(device):
-            _lib.lib().call(name, *args)
+        with torch.cuda.device(index):
+            _lib.lib().call(name, *args, stream=stream)
 
 
 def _matrix(x: torch.Tensor, what: str) -> Tuple[int, int, int, int, int]:
@@ -158,12 +167,13 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp4", tensor_scale: Optional[float] 
         _check_scale(tensor_scale, fmt)
     batch, rows, cols, bs, ld = _matrix(x, "x")
     g = (cols + 127) // 128
-    codes = torch.empty(*x.shape[:-1], 64 * g, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(*x.shape[:-2], (rows + 127) // 128, g if fmt == "mxfp4" else 2 * g, 512, dtype=torch.uint8, device=x.device)
+    lead, dev = x.shape[:-2], x.device
+    codes = torch.empty((*lead, rows, 64 * g), dtype=torch.uint8, device=dev)
+    scales = torch.empty((*lead, (rows + 127) // 128, g if fmt == "mxfp4" else 2 * g, 512), dtype=torch.uint8, device=dev)
     if batch * rows:
-        _call(x.device, "fb_fp4_quantize", x, _DTYPES[x.dtype], ld, bs, codes, scales, batch, rows, cols, FORMATS[fmt],
+        _call(dev, "fb_fp4_quantize", x, _DTYPES[x.dtype], ld, bs, codes, scales, batch, rows, cols, FORMATS[fmt],
               float(tensor_scale or 0.0))
-    return Fp4Tensor(codes, scales, fmt, x.shape, tensor_scale)
+    return Fp4Tensor._of(codes, scales, fmt, tuple(x.shape), tensor_scale)
 
 
 def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.device, what: str = "out") -> torch.Tensor:

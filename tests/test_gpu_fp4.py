@@ -180,7 +180,8 @@ def test_nan_scales_reach_their_rows_only(fmt):
 
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
-@pytest.mark.parametrize("M,N,K", [(1, 384, 1000), (40, 200, 640), (200, 300, 384)])
+@pytest.mark.parametrize("M,N,K", [(1, 384, 1000), (1, 5120, 8192), (2, 640, 2000), (5, 130, 700), (16, 257, 96), (1, 64, 1), (9, 256, 4096),
+                                   (40, 200, 640), (200, 300, 384)])
 def test_linear_is_quantize_and_matmul(fmt, M, N, K):
     g = _gen(K)
     ts = float(torch.tensor(0.03)) if fmt == "nvfp4" else None

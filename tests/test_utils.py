@@ -150,3 +150,34 @@ def test_sources_name_no_closed_constructs():
                 if re.search(pat, text):
                     bad.append((os.path.relpath(fn, ROOT), pat))
     assert not bad, bad
+
+
+def test_kernel_call_converts_arguments_the_same_way_every_time():
+    """The first call of an entry point converts argument by argument, later ones let ctypes do it: every kind arrives alike."""
+    import ctypes
+    import torch
+    from ferrite_b200._lib import KernelLib, KernelError
+    seen = []
+    kinds = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p)
+    fn = kinds(lambda p, i, f, q, s: (seen.append((p, i, round(f, 3), q, s)), 0 if i < 100 else 7)[1])
+
+    class Lib:
+        fb_probe = fn
+
+        def __getitem__(self, name):
+            return ctypes.cast(fn, ctypes.CDLL(None)._FuncPtr)
+
+    k = KernelLib.__new__(KernelLib)
+    k.lib, k._fns, k._fast, k.launches = Lib(), {"fb_probe": fn}, {}, 0
+    t = torch.zeros(4)
+    u = torch.zeros(2)
+    for _ in range(3):
+        k.call("fb_probe", t, 5, 1.5, u, stream=11)
+        k.call("fb_probe", t, True, 2, None, stream=0)
+    p, q = t.data_ptr(), u.data_ptr()
+    assert seen == [(p, 5, 1.5, q, 11), (p, 1, 2.0, None, None)] * 3 and k.launches == 6
+    try:
+        k.call("fb_probe", t, 100, 0.0, u, stream=0)
+        raise AssertionError("an error code has to raise")
+    except KernelError as e:
+        assert "7" in str(e)
