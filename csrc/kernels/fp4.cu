@@ -28,19 +28,21 @@ constexpr int kQCols = 256;   // columns of a warp's pass
 // Tile of this CTA: rows (tile * 128 + 8 * sub + warp) + 32 g, columns 256 * ct ...; bt = matrix of the batch.
 struct Place { int64_t bt; int64_t row; int64_t tile; int i; int64_t col; };
 __device__ __forceinline__ Place place(int64_t rows, int64_t cols) {
-    const int64_t nct = (cols + kQCols - 1) / kQCols, nrt = (rows + 127) / 128;
-    int64_t b = blockIdx.x;
+    // 32-bit divisions (the grid has fewer than 2^31 blocks): in 64 bits they were half of the kernel's instructions
+    const uint32_t nct = (uint32_t)((cols + kQCols - 1) / kQCols), nrt = (uint32_t)((rows + 127) / 128);
+    const uint32_t t = blockIdx.x / nct, ct = blockIdx.x - t * nct, sub = t & 3, rt = t >> 2;
     Place p;
-    const int64_t ct = b % nct;
-    b /= nct;
-    const int sub = (int)(b & 3);
-    b >>= 2;
-    p.tile = b % nrt;
-    p.bt = b / nrt;
-    p.i = sub * 8 + (threadIdx.x >> 5);
+    p.bt = rt / nrt;
+    p.tile = rt - (uint32_t)p.bt * nrt;
+    p.i = (int)(sub * 8 + (threadIdx.x >> 5));
     p.row = p.tile * 128 + p.i;
-    p.col = ct * kQCols + (threadIdx.x & 31) * 8;
+    p.col = (int64_t)ct * kQCols + (threadIdx.x & 31) * 8;
     return p;
+}
+
+// Whether all of this warp's rows and columns exist (the same for the warps of a CTA but for the last row tile).
+__device__ __forceinline__ bool whole(const Place& p, int64_t rows, int64_t cols, int vec) {
+    return vec && p.row + 96 < rows && (p.col | 255) < cols;
 }
 
 template <int FMT, typename T>
@@ -54,12 +56,23 @@ fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int ve
     const T* xb = x + p.bt * bstride;
     const int n = (int)max((int64_t)0, min((int64_t)8, cols - p.col));
     float v[4][8];
+    if (whole(p, rows, cols, vec)) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const int64_t r = p.row + 32 * g;
-        load8(xb + (r < rows ? r * ld + p.col : 0), r < rows ? n : 0, vec && r < rows, v[g]);
+        for (int g = 0; g < 4; ++g) load8(xb + (p.row + 32 * g) * ld + p.col, v[g]);
+    } else {
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {   // (rolled: a predicated element-wise path costs the whole tiles their issue slots)
+            const int64_t r = p.row + 32 * g;
+            float t[8];
+            load8(xb + (r < rows ? r * ld + p.col : 0), r < rows ? n : 0, false, t);
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (h == g) v[h][j] = t[j];
+        }
     }
-    uint32_t word[4];   // this lane's group of four blocks: their scale bytes, row by row
+    uint32_t bytes = 0;   // the scales of this lane's block in the four rows
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         uint32_t byte;
@@ -68,19 +81,22 @@ fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int ve
         // columns in 8s up to the padded row end (64 bytes per group of 128 columns)
         if (r < rows && p.col < 128 * G)
             *reinterpret_cast<uint32_t*>(codes + (p.bt * rows + r) * cstride + p.col / 2) = code;
-        // gather the bytes of four neighbouring blocks (16 lanes of mxfp4, 8 of nvfp4) into a word
-        constexpr int kPer = FMT == kMxFp4 ? 4 : 2;
-        uint32_t w = r < rows && n > 0 ? byte << (8 * (lane / kPer & 3)) : 0u;
-        if (lane % kPer) w = 0;
-#pragma unroll
-        for (int o = 1; o < 4 * kPer; o <<= 1) w |= __shfl_xor_sync(0xffffffffu, w, o);
-        word[g] = w;
+        if (r < rows && n > 0) bytes |= byte << (8 * g);
     }
+    // four neighbouring blocks (16 lanes of mxfp4, 8 of nvfp4) x four rows: fetch the blocks' words, transpose the bytes
+    constexpr int kPer = FMT == kMxFp4 ? 4 : 2;
+    const int head = lane & ~(4 * kPer - 1);
+    uint32_t w[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) w[b] = __shfl_sync(0xffffffffu, bytes, head + b * kPer);
     constexpr int kChunkCols = FMT == kMxFp4 ? 128 : 64;
-    if (lane % (kChunkCols / 8) == 0 && p.col < 128 * G) {
+    if (lane == head && p.col < 128 * G) {
+        const uint32_t a01 = __byte_perm(w[0], w[1], 0x5140), a23 = __byte_perm(w[2], w[3], 0x5140);   // rows 0, 1
+        const uint32_t b01 = __byte_perm(w[0], w[1], 0x7362), b23 = __byte_perm(w[2], w[3], 0x7362);   // rows 2, 3
         const int64_t C = FMT == kMxFp4 ? G : 2 * G, nrt = (rows + 127) / 128;
         uint8_t* chunk = scales + ((p.bt * nrt + p.tile) * C + p.col / kChunkCols) * 512;
-        *reinterpret_cast<uint4*>(chunk + p.i * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+        *reinterpret_cast<uint4*>(chunk + p.i * 16) = make_uint4(__byte_perm(a01, a23, 0x5410), __byte_perm(a01, a23, 0x7632),
+                                                                 __byte_perm(b01, b23, 0x5410), __byte_perm(b01, b23, 0x7632));
     }
 }
 
@@ -103,10 +119,10 @@ fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
     }
     const int shift = FMT == kMxFp4 ? 8 * (int)(p.col / 32 & 3) : 8 * (int)(p.col / 16 & 3);
     const int n = (int)min((int64_t)8, cols - p.col);
+    const bool all = whole(p, rows, cols, vec);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const int64_t r = p.row + 32 * g;
-        if (r >= rows) break;
         const uint32_t byte = w[g] >> shift & 0xffu;
         float s;
         if (FMT == kMxFp4) {
@@ -120,16 +136,19 @@ fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
         e2m1x8_to_f32(code[g], v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], s), ts);
-        store8(out + p.bt * bstride + r * ld + p.col, n, vec, v);
+        T* o = out + p.bt * bstride + r * ld + p.col;
+        if (all) {
+            store8(o, v);
+        } else if (r < rows) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) o[j] = from_f32<T>(v[j]);
+        }
     }
 }
 
 int64_t grid_of(int64_t batch, int64_t rows, int64_t cols) {
     return batch * ((rows + 127) / 128) * 4 * ((cols + kQCols - 1) / kQCols);
-}
-
-bool vec_ok(const void* p, int64_t ld, int64_t bstride, int esz) {
-    return ((uintptr_t)p & 15) == 0 && ld * esz % 16 == 0 && bstride * esz % 16 == 0;
 }
 
 }  // namespace
@@ -172,7 +191,7 @@ FB_API int fb_fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bst
     if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
     const int scaled = fmt == kNvFp4 && ts != 0.f && ts != 1.f;
     const float inv = scaled ? (float)(1.0 / (double)ts) : 1.f;
-    const int vec = vec_ok(x, ld, bstride, dtype == kF32 ? 4 : 2);
+    const int vec = rows_of_8(x, ld, bstride, dtype == kF32 ? 4 : 2);
 #define FP4_Q(F, D)                                                                                                         \
     (int)fp4_launch(fp4_quantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, false,      \
                     (const Elem<D>::T*)x, ld, bstride, vec, (uint8_t*)codes, (uint8_t*)scales, rows, cols, scaled, ts, inv)
@@ -189,7 +208,7 @@ FB_API int fb_fp4_dequantize(const void* codes, const void* scales, void* out, i
         return (int)cudaErrorInvalidValue;
     const int64_t grid = grid_of(batch, rows, cols);
     if (grid > 0x7fffffffll) return (int)cudaErrorInvalidValue;
-    const int vec = vec_ok(out, ld, bstride, dtype == kF32 ? 4 : 2);
+    const int vec = rows_of_8(out, ld, bstride, dtype == kF32 ? 4 : 2);
     const float t = ts == 0.f ? 1.f : ts;
 #define FP4_D(F, D)                                                                                                    \
     (int)fp4_launch(fp4_dequantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, false, \

@@ -192,17 +192,11 @@ __device__ __forceinline__ float div_by(float u, float s, float r) {
     return __fmaf_rn(__fmaf_rn(-q0, s, u), r, q0);
 }
 
-// Eight consecutive values of a row -> their codes (value j in nibble j) and the scale byte of their block, which is this
-// lane and its neighbours (four lanes of mxfp4, two of nvfp4; whole warps call).  scaled: nvfp4 with a tensor scale ts.
+// Eight consecutive values of a row (m: the largest of their |.| as integer, the values divided by the tensor scale already)
+// -> their codes (value j in nibble j) and the scale byte of their block, which is this lane and its neighbours (four
+// lanes of mxfp4, two of nvfp4; whole warps call).
 template <int FMT>
-__device__ __forceinline__ uint32_t quantize8(float (&v)[8], bool scaled, float ts, float inv_ts, uint32_t& byte) {
-    if (FMT == kNvFp4 && scaled) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = div_by(v[j], ts, inv_ts);
-    }
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(v[j]));
+__device__ __forceinline__ uint32_t quantize8(float (&v)[8], uint32_t m, uint32_t& byte) {
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
     if (FMT == kMxFp4) m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
     if (FMT == kMxFp4) {
@@ -221,6 +215,35 @@ __device__ __forceinline__ uint32_t quantize8(float (&v)[8], bool scaled, float 
     return m >= kInfBits ? 0u : e2m1x8(v);   // a block that is not finite: NaN scale, zero codes
 }
 
+// max(|a|, |b|) that keeps a NaN (as the largest integer).
+__device__ __forceinline__ float max_abs_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
+// Largest |.| of eight values as an integer that orders NaN > infinity > numbers.
+__device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
+    float m[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m[j] = max_abs_nan(v[2 * j], v[2 * j + 1]);
+    return __float_as_uint(max_abs_nan(max_abs_nan(m[0], m[1]), max_abs_nan(m[2], m[3])));
+}
+
+// The same with the values as they are loaded; scaled: nvfp4 with a tensor scale ts.
+template <int FMT>
+__device__ __forceinline__ uint32_t quantize8(float (&v)[8], bool scaled, float ts, float inv_ts, uint32_t& byte) {
+    if (FMT == kNvFp4 && scaled) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = div_by(v[j], ts, inv_ts);
+    }
+    return quantize8<FMT>(v, max_bits8(v), byte);
+}
+
+// Whether rows of a matrix can be read and written eight values at a time.
+inline bool rows_of_8(const void* p, int64_t ld, int64_t bstride, int esz) {
+    return (uintptr_t)p % (8 * esz) == 0 && ld % 8 == 0 && bstride % 8 == 0;
+}
+
 // ---- values of the three element types -----------------------------------------------------------
 template <int DT> struct Elem;
 template <> struct Elem<kF32> { using T = float; };
@@ -230,29 +253,33 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
-// p[0 .. 7] -> f32; `n` of them exist (the others read 0); vec: p is 16-byte aligned.
+// p[0 .. 7] -> f32, all of them there; p is aligned to the eight values (16 bytes, f32 32).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        asm("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+            : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p));
+    } else {
+        const uint4 a = ldg_nc_v4(p);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                v[2 * i] = bf16lo(w[i]);
+                v[2 * i + 1] = bf16hi(w[i]);
+            } else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+}
+// The first n of them (the others read 0); vec: p is aligned as above.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]) {
     if (vec && n >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            const uint4 a = ldg_nc_v4(p), b = ldg_nc_v4(p + 4);
-            v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
-            v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
-        } else {
-            const uint4 a = ldg_nc_v4(p);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                    v[2 * i] = bf16lo(w[i]);
-                    v[2 * i + 1] = bf16hi(w[i]);
-                } else {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                    v[2 * i] = f.x;
-                    v[2 * i + 1] = f.y;
-                }
-            }
-        }
+        load8(p, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
@@ -271,21 +298,14 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
         return *reinterpret_cast<const uint32_t*>(&h);
     }
 }
-// The first n of eight values to p.
+// Eight values to p (aligned as for load8).
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int n, bool vec, const float (&v)[8]) {
-    if (vec && n >= 8) {
-        if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < n) p[i] = from_f32<T>(v[i]);
-    }
+__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                     "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+    else
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
 
 }  // namespace fp4

@@ -192,7 +192,7 @@ template <int FMT, typename C>
 __device__ __forceinline__ void quantize_x(const GemmArgs& a, uint8_t* room, int t, int kb0, int kb1, uint32_t x_full, int lane) {
     const int units = (kb1 - kb0) * 32;                    // of eight columns
     const int esz = a.xdt == kF32 ? 4 : 2;
-    const bool vec = ((uintptr_t)a.x & 15) == 0 && a.ldx * esz % 16 == 0;
+    const bool vec = (uintptr_t)a.x % (8 * esz) == 0 && a.ldx % 8 == 0;
 #pragma unroll 1
     for (int64_t m = 0; m < a.Q; ++m) {
 #pragma unroll 1

@@ -291,7 +291,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     } else {
         // ---- this CTA's K range of x, quantised, in operand form ----
         const TX* x = reinterpret_cast<const TX*>(a.x);
-        const bool vec = ((uintptr_t)x & 15) == 0 && a.ldx * (int64_t)sizeof(TX) % 16 == 0;
+        const bool vec = (uintptr_t)x % (8 * sizeof(TX)) == 0 && a.ldx % 8 == 0;
         constexpr int kN = kUpThreads - kRouteThreads, kBatch = 4;
         // a thread keeps its eight columns over the tokens (four loads in flight); a block of 32 columns is four lanes
 #pragma unroll 1

@@ -168,40 +168,36 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp4", tensor_scale: Optional[float] 
     batch, rows, cols, bs, ld = _matrix(x, "x")
     g = (cols + 127) // 128
     lead, dev = x.shape[:-2], x.device
-    codes = torch.empty((*lead, rows, 64 * g), dtype=torch.uint8, device=dev)
-    scales = torch.empty((*lead, (rows + 127) // 128, g if fmt == "mxfp4" else 2 * g, 512), dtype=torch.uint8, device=dev)
+    codes = torch.empty(*lead, rows, 64 * g, dtype=torch.uint8, device=dev)
+    scales = torch.empty(*lead, (rows + 127) // 128, g if fmt == "mxfp4" else 2 * g, 512, dtype=torch.uint8, device=dev)
     if batch * rows:
         _call(dev, "fb_fp4_quantize", x, _DTYPES[x.dtype], ld, bs, codes, scales, batch, rows, cols, FORMATS[fmt],
               float(tensor_scale or 0.0))
     return Fp4Tensor._of(codes, scales, fmt, tuple(x.shape), tensor_scale)
 
 
-def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.device, what: str = "out") -> torch.Tensor:
+def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.device):
+    """``out`` or a new tensor of ``shape``, and its :func:`_matrix`."""
     if out is None:
         if dtype not in _DTYPES:
-            raise TypeError(f"{what} is float32, bfloat16 or float16, got {dtype}")
-        return torch.empty(shape, dtype=dtype, device=device)
+            raise TypeError(f"out is float32, bfloat16 or float16, got {dtype}")
+        out = torch.empty(*shape, dtype=dtype, device=device)
+        rows, cols = shape[-2:]
+        return out, (math.prod(shape[:-2]), rows, cols, rows * cols, cols)
     if tuple(out.shape) != tuple(shape) or out.device != device:
-        raise ValueError(f"{what} must be {tuple(shape)} on {device}, got {tuple(out.shape)} on {out.device}")
-    return out
+        raise ValueError(f"out must be {tuple(shape)} on {device}, got {tuple(out.shape)} on {out.device}")
+    return out, _matrix(out, "out") if out.numel() else (0, 0, 0, 0, 0)
 
 
 def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values of ``q``, rounded once to ``dtype`` (or into ``out``, whose rows may be strided)."""
     if not q.codes.is_cuda:
         raise ValueError("q is not on a CUDA device")
-    out = _out(out, q.shape, dtype, q.device)
-    if out.numel():
-        batch, rows, cols, bs, ld = _matrix(out, "out")
+    out, (batch, rows, cols, bs, ld) = _out(out, q.shape, dtype, q.device)
+    if batch * rows:
         _call(q.device, "fb_fp4_dequantize", q.codes, q.scales, out, _DTYPES[out.dtype], ld, bs, batch, rows, cols,
               FORMATS[q.fmt], float(q.tensor_scale or 0.0))
     return out
-
-
-def _product_out(out, M: int, N: int, dtype, device):
-    out = _out(out, (M, N), dtype, device)
-    _, _, _, _, ldo = _matrix(out, "out") if out.numel() else (0, 0, 0, 0, N)
-    return out, ldo
 
 
 def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -214,7 +210,7 @@ def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, 
     if not x.codes.is_cuda or x.device != w.device:
         raise ValueError(f"matmul takes tensors of one CUDA device, got {x.device} and {w.device}")
     M, N, K = x.shape[0], w.shape[0], x.shape[1]
-    out, ldo = _product_out(out, M, N, out_dtype, x.device)
+    out, (_, _, _, _, ldo) = _out(out, (M, N), out_dtype, x.device)
     if M and N:
         alpha = float(x.tensor_scale or 1.0) * float(w.tensor_scale or 1.0)
         _call(x.device, "fb_fp4_matmul", x.codes, x.scales, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
@@ -234,13 +230,14 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
     if x.device != w.device:
         raise ValueError(f"x is on {x.device}, w on {w.device}")
     N = w.shape[0]
-    out, ldo = _product_out(out, M, N, out_dtype or x.dtype, x.device)
+    dev = x.device
+    out, (_, _, _, _, ldo) = _out(out, (M, N), out_dtype or x.dtype, dev)
     if M and N:
         g = (K + 127) // 128
         work = torch.empty((M * 64 * g + 511) // 512 * 512 + (M + 127) // 128 * (g if w.fmt == "mxfp4" else 2 * g) * 512,
-                           dtype=torch.uint8, device=x.device)
+                           dtype=torch.uint8, device=dev)
         alpha = float(x_scale or 1.0) * float(w.tensor_scale or 1.0)
-        _call(x.device, "fb_fp4_linear", x, _DTYPES[x.dtype], ldx, work, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
+        _call(dev, "fb_fp4_linear", x, _DTYPES[x.dtype], ldx, work, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
               FORMATS[w.fmt], float(x_scale or 0.0), alpha)
     return out
 
@@ -292,7 +289,7 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     if any(t is not None and t.device != dev for t in (x, logits, bias, w2.codes)):
         raise ValueError("moe takes tensors of one device")
     _, _, _, _, ldx = _matrix(x, "x")
-    out, ldo = _product_out(out, T, D, out_dtype or x.dtype, dev)
+    out, (_, _, _, _, ldo) = _out(out, (T, D), out_dtype or x.dtype, dev)
     if T:
         tile = 128 * (16 if T <= 16 else 32) + 512
         work = torch.empty(4096 + min(E, T * topk) * ((I + 127) // 128) * tile, dtype=torch.uint8, device=dev)
