@@ -53,35 +53,49 @@ fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int ve
     const Place p = place(rows, cols);
     const int lane = threadIdx.x & 31;
     const int64_t G = groups(cols), cstride = 64 * G;
-    const T* xb = x + p.bt * bstride;
-    const int n = (int)max((int64_t)0, min((int64_t)8, cols - p.col));
-    float v[4][8];
-    if (whole(p, rows, cols, vec)) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) load8(xb + (p.row + 32 * g) * ld + p.col, v[g]);
-    } else {
-#pragma unroll 1
-        for (int g = 0; g < 4; ++g) {   // (rolled: a predicated element-wise path costs the whole tiles their issue slots)
-            const int64_t r = p.row + 32 * g;
-            float t[8];
-            load8(xb + (r < rows ? r * ld + p.col : 0), r < rows ? n : 0, false, t);
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (h == g) v[h][j] = t[j];
-        }
-    }
+    const T* xp = x + p.bt * bstride + p.row * ld + p.col;
+    uint8_t* cp = codes + (p.bt * rows + p.row) * cstride + p.col / 2;
     uint32_t bytes = 0;   // the scales of this lane's block in the four rows
+    if (whole(p, rows, cols, vec)) {
+        const int64_t step = 32 * ld, cstep = 32 * cstride;
+        if constexpr (sizeof(T) == 2) {
+            uint4 raw[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        uint32_t byte;
-        const uint32_t code = quantize8<FMT>(v[g], scaled, ts, inv_ts, byte);
-        const int64_t r = p.row + 32 * g;
-        // columns in 8s up to the padded row end (64 bytes per group of 128 columns)
-        if (r < rows && p.col < 128 * G)
-            *reinterpret_cast<uint32_t*>(codes + (p.bt * rows + r) * cstride + p.col / 2) = code;
-        if (r < rows && n > 0) bytes |= byte << (8 * g);
+            for (int g = 0; g < 4; ++g) raw[g] = ldg_nc_v4(xp + g * step);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                float v[8];
+                uint32_t byte, code;
+                unpack8<T>(raw[g], v);
+                if (FMT == kNvFp4 && scaled) code = quantize8<FMT>(v, true, ts, inv_ts, byte);
+                else code = quantize8<FMT>(v, max_bits8_packed<T>(raw[g]), byte);
+                *reinterpret_cast<uint32_t*>(cp + g * cstep) = code;
+                bytes |= byte << (8 * g);
+            }
+        } else {
+            float v[4][8];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) load8(xp + g * step, v[g]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                uint32_t byte;
+                *reinterpret_cast<uint32_t*>(cp + g * cstep) = quantize8<FMT>(v[g], scaled, ts, inv_ts, byte);
+                bytes |= byte << (8 * g);
+            }
+        }
+    } else {
+        const int n = (int)max((int64_t)0, min((int64_t)8, cols - p.col));
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+            const bool row = p.row + 32 * g < rows;
+            float v[8];
+            uint32_t byte;
+            load8(row && n ? xp + g * 32 * ld : x, row ? n : 0, false, v);
+            const uint32_t code = quantize8<FMT>(v, scaled, ts, inv_ts, byte);
+            // codes up to the padded row end (64 bytes per group of 128 columns)
+            if (row && p.col < 128 * G) *reinterpret_cast<uint32_t*>(cp + g * 32 * cstride) = code;
+            if (row && n > 0) bytes |= byte << (8 * g);
+        }
     }
     // four neighbouring blocks (16 lanes of mxfp4, 8 of nvfp4) x four rows: fetch the blocks' words, transpose the bytes
     constexpr int kPer = FMT == kMxFp4 ? 4 : 2;

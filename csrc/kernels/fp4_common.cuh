@@ -253,6 +253,35 @@ __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
+// Largest |.| of eight 16-bit values as they are in memory (two per word), in the integer form of max_bits8.
+template <typename T>
+__device__ __forceinline__ uint32_t max_bits8_packed(const uint4& a) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        auto h = [](uint32_t w) { return __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w)); };
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h(a.x), h(a.y)), __hmax2_nan(h(a.z), h(a.w)));
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(&m);
+        return max(w << 16, w & 0xffff0000u);
+    } else {
+        auto h = [](uint32_t w) { return __habs2(*reinterpret_cast<const __half2*>(&w)); };
+        const __half2 m = __hmax2_nan(__hmax2_nan(h(a.x), h(a.y)), __hmax2_nan(h(a.z), h(a.w)));
+        return max(abs_bits(__low2float(m)), abs_bits(__high2float(m)));
+    }
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& a, float (&v)[8]) {
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            v[2 * i] = bf16lo(w[i]);
+            v[2 * i + 1] = bf16hi(w[i]);
+        } else {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+}
 // p[0 .. 7] -> f32, all of them there; p is aligned to the eight values (16 bytes, f32 32).
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -260,19 +289,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
         asm("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p));
     } else {
-        const uint4 a = ldg_nc_v4(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                v[2 * i] = bf16lo(w[i]);
-                v[2 * i + 1] = bf16hi(w[i]);
-            } else {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                v[2 * i] = f.x;
-                v[2 * i + 1] = f.y;
-            }
-        }
+        unpack8<T>(ldg_nc_v4(p), v);
     }
 }
 // The first n of them (the others read 0); vec: p is aligned as above.
