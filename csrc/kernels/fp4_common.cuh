@@ -302,6 +302,22 @@ __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]
         for (int i = 0; i < 8; ++i) v[i] = i < n ? to_f32(p[i]) : 0.f;
     }
 }
+// Eight values as they are in memory.
+template <typename T> struct Raw8 {
+    uint4 w;
+    __device__ __forceinline__ void load(const T* p) { w = ldg_nc_v4(p); }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const { unpack8<T>(w, v); }
+    __device__ __forceinline__ uint32_t max_bits() const { return max_bits8_packed<T>(w); }
+};
+template <> struct Raw8<float> {
+    float f[8];
+    __device__ __forceinline__ void load(const float* p) { load8(p, f); }
+    __device__ __forceinline__ void unpack(float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = f[j];
+    }
+    __device__ __forceinline__ uint32_t max_bits() const { return max_bits8(f); }
+};
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }

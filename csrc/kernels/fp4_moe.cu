@@ -118,7 +118,7 @@ __device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, float* scr
         for (int u = warp; u < a.T * stripes; u += nw) {
             const int t = u / stripes, first = (u - t * stripes) * 32 + lane;
             const float mx = r.mx[t], inv = r.inv[t];
-#pragma unroll 1
+#pragma unroll 4
             for (int e = first; e < a.E; e += 32 * stripes) {
                 const float z = lg[t * a.E + e];
                 keys[t * a.E + e] = order_key(score_of(z, a.score, mx, inv) + bias[e]);
@@ -293,40 +293,61 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         const TX* x = reinterpret_cast<const TX*>(a.x);
         const bool vec = (uintptr_t)x % (8 * sizeof(TX)) == 0 && a.ldx % 8 == 0;
         constexpr int kN = kUpThreads - kRouteThreads, kBatch = 4;
-        // a thread keeps its eight columns over the tokens (four loads in flight); a block of 32 columns is four lanes
+        // e4m3 of eight values (m: the largest |.|) to their place in row t; a block of 32 columns is four lanes
+        auto put = [&](int t, int c, bool in, const float (&v)[8], uint32_t m) {
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+            const uint32_t sb = ue8m0_of(m, 1e-4f, kInv448);
+            const float inv = sb == 255u ? 0.f : ue8m0_inv(sb);
+            uint32_t w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] * inv, v[4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+                const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] * inv, v[4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+                w[i] = sb == 255u ? 0u : lo | hi << 16;
+            }
+            if (in) {
+                const int kb = c >> 4, u16 = c & 15;       // u16: 8-byte unit of the 128-byte row
+                *reinterpret_cast<uint2*>(base_g + kb * (BN * 128) + t * 128 + (((u16 >> 1) ^ (t & 7)) << 4) + (u16 & 1) * 8) = make_uint2(w[0], w[1]);
+                if ((c & 3) == 0) base_g[xsf_off + kb * 512 + t * 16 + (u16 >> 2)] = (uint8_t)sb;
+            }
+        };
+        const int tid = threadIdx.x - kRouteThreads, per_row = nkb * 16;      // units of eight columns
+        if (vec && kb1 * 128 <= a.D) {
+            // a thread keeps its eight columns over the tokens, the next four tokens' loads in flight
 #pragma unroll 1
-        for (int c0 = 0; c0 < nkb * 16; c0 += kN) {
-            const int c = c0 + threadIdx.x - kRouteThreads;
-            const int col = kb0 * 128 + c * 8, kb = c >> 4, u16 = c & 15;      // u16: 8-byte unit of the 128-byte row
-            const bool in = c < nkb * 16;
-            const int n = in ? max(0, min(8, a.D - col)) : 0;
-            const TX* xc = x + min(col, a.D - 1);
+            for (int c0 = 0; c0 < per_row; c0 += kN) {
+                const int c = c0 + tid;
+                const bool in = c < per_row;
+                const TX* xc = x + kb0 * 128 + (in ? c : 0) * 8;
+                Raw8<TX> cur[kBatch], nxt[kBatch];
+#pragma unroll
+                for (int b = 0; b < kBatch; ++b) cur[b].load(xc + min(b, a.T - 1) * a.ldx);
 #pragma unroll 1
-            for (int t0 = 0; t0 < a.T; t0 += kBatch) {
-                float v[kBatch][8];
+                for (int t0 = 0; t0 < a.T; t0 += kBatch) {
 #pragma unroll
-                for (int b = 0; b < kBatch; ++b) load8(xc + min(t0 + b, a.T - 1) * a.ldx, n, vec, v[b]);
+                    for (int b = 0; b < kBatch; ++b) nxt[b].load(xc + min(t0 + kBatch + b, a.T - 1) * a.ldx);
 #pragma unroll
-                for (int b = 0; b < kBatch; ++b) {
-                    const int t = t0 + b;
-                    uint32_t m = 0;
+                    for (int b = 0; b < kBatch; ++b)
+                        if (t0 + b < a.T) {
+                            float v[8];
+                            cur[b].unpack(v);
+                            put(t0 + b, c, in, v, cur[b].max_bits());
+                        }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[b][i]));
-                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                    const uint32_t sb = ue8m0_of(m, 1e-4f, kInv448);
-                    const float inv = sb == 255u ? 0.f : ue8m0_inv(sb);
-                    uint32_t w[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i] * inv, v[b][4 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[b][4 * i + 2] * inv, v[b][4 * i + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-                        w[i] = sb == 255u ? 0u : lo | hi << 16;
-                    }
-                    if (in && t < a.T) {
-                        *reinterpret_cast<uint2*>(base_g + kb * (BN * 128) + t * 128 + (((u16 >> 1) ^ (t & 7)) << 4) + (u16 & 1) * 8) = make_uint2(w[0], w[1]);
-                        if ((c & 3) == 0) base_g[xsf_off + kb * 512 + t * 16 + (u16 >> 2)] = (uint8_t)sb;
-                    }
+                    for (int b = 0; b < kBatch; ++b) cur[b] = nxt[b];
+                }
+            }
+        } else {
+#pragma unroll 1
+            for (int c0 = 0; c0 < per_row; c0 += kN) {
+                const int c = c0 + tid, col = kb0 * 128 + c * 8;
+                const bool in = c < per_row;
+#pragma unroll 1
+                for (int t = 0; t < a.T; ++t) {
+                    float v[8];
+                    load8(x + t * a.ldx + min(col, a.D - 1), in ? max(0, min(8, a.D - col)) : 0, false, v);
+                    put(t, c, in, v, max_bits8(v));
                 }
             }
         }
