@@ -49,9 +49,9 @@ inline cudaError_t fp4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     return e;
 }
 
-// cuTensorMapEncodeTiled, 2-D, 128-byte swizzle, no interleave, zero fill.
+// cuTensorMapEncodeTiled, 2-D, no interleave, zero fill.
 inline int fp4_encode_tmap(CUtensorMap* map, CUtensorMapDataType type, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
-                           const cuuint32_t* box, const cuuint32_t* estr) {
+                           const cuuint32_t* box, const cuuint32_t* estr, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
     typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -64,7 +64,7 @@ inline int fp4_encode_tmap(CUtensorMap* map, CUtensorMapDataType type, const voi
         fn = (EncodeFn)p;
     }
     const CUresult r = fn(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                          swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : (int)cudaErrorInvalidValue;
 }
 

@@ -104,20 +104,21 @@ __device__ __forceinline__ void store_columns(const GemmArgs& a, uint32_t tmem, 
     }
 }
 
-// P = X: a lane holds a row's outputs side by side.  They go through two 32-row x 128-byte buffers of this warp (16-byte
-// units swizzled as TMA's 128-byte mode: no bank conflicts) and leave as TMA stores, which the tensor core does not wait
+// P = X: a lane holds a row's outputs side by side.  They go through two buffers of 32 rows x ROW bytes of this warp
+// (16-byte units swizzled as in TMA's 128- or 64-byte mode) and leave as TMA stores, which the tensor core does not wait
 // for: the accumulator is given back as soon as it is read.  Rows that TMA cannot address (base or row stride not a
 // multiple of 16 bytes) leave as stores of 32 neighbouring outputs.
-template <typename T, int BN>
+template <typename T, int BN, int ROW, bool PAIR = false>
 __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap* tmap_o, uint32_t tmem, uint32_t buf0, int warp, int lane,
                                            int64_t p0, int64_t q0, uint32_t acc_empty, int& turn) {
-    constexpr int kCols = 128 / (int)sizeof(T), kChunks = BN / 2 / kCols;   // columns of a buffer, buffers of this warp's half
+    constexpr int kCols = ROW / (int)sizeof(T), kChunks = BN / 2 / kCols;   // columns of a buffer, buffers of this warp's half
+    auto unit = [](int row, int u) { return (uint32_t)(row * ROW + ((u ^ (ROW == 128 ? row & 7 : row >> 1 & 3)) << 4)); };
     static_assert(kChunks >= 1, "a warp's half is a buffer at least");
     const int quarter = warp & 3, c0 = (warp >> 2) * (BN / 2);
     const int64_t row0 = p0 + quarter * 32;
 #pragma unroll 1
     for (int ch = 0; ch < kChunks; ++ch, turn ^= 1) {   // the buffers take turns, across tiles too
-        const uint32_t buf = buf0 + (uint32_t)turn * 4096;
+        const uint32_t buf = buf0 + (uint32_t)turn * (32 * ROW);
         const int64_t q = q0 + c0 + ch * kCols;
         if (lane == 0) bulk_wait_read<1>();      // the store before the last has left this buffer
         __syncwarp();
@@ -128,17 +129,20 @@ __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap*
         if (ch == kChunks - 1) {
             tc::tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty);
+            if (lane == 0) {
+                if constexpr (PAIR) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc_empty) : "memory");
+                else mbar_arrive(acc_empty);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {            // 16-byte units
+        for (int u = 0; u < ROW / 16; ++u) {     // 16-byte units
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(__uint_as_float(r[u * 4 + i]) * a.alpha);
                 else w[i] = pack2<T>(__uint_as_float(r[u * 8 + 2 * i]) * a.alpha, __uint_as_float(r[u * 8 + 2 * i + 1]) * a.alpha);
             }
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + lane * 128 + ((u ^ (lane & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + unit(lane, u)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         }
         if (a.vec) {
             fence_proxy_async();
@@ -155,9 +159,9 @@ __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap*
                 T* out = reinterpret_cast<T*>(a.out) + (row0 + i) * a.ldo + q;
 #pragma unroll
                 for (int h = 0; h < kCols; h += 32) {
-                    const int c = h + lane, byte = c * (int)sizeof(T);
+                    const int c = h + lane % (kCols < 32 ? kCols : 32), byte = c * (int)sizeof(T);
                     T v;
-                    const uint32_t at = buf + i * 128 + (((byte >> 4) ^ (i & 7)) << 4) + (byte & 15);
+                    const uint32_t at = buf + unit(i, byte >> 4) + (byte & 15);
                     if constexpr (sizeof(T) == 4) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
                     else { uint16_t u; asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(at) : "memory"); v = *reinterpret_cast<T*>(&u); }
                     if (q + c < a.Q) out[c] = v;
@@ -398,9 +402,9 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                     else store_columns<float, BN>(a, tmem, quarter_warp, lane, p0, q0);
                 } else {
                     const uint32_t buf = staging + (uint32_t)w * 8192;
-                    if (a.dtype == kBf16) store_rows<__nv_bfloat16, BN>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
-                    else if (a.dtype == kF16) store_rows<__half, BN>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
-                    else store_rows<float, BN>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
+                    if (a.dtype == kBf16) store_rows<__nv_bfloat16, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
+                    else if (a.dtype == kF16) store_rows<__half, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
+                    else store_rows<float, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
                     continue;   // (store_rows gave the accumulator back)
                 }
             }
@@ -443,16 +447,216 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     }
 }
 
-// Output [rows, cols] in boxes of 32 rows x 128 bytes, 128-byte swizzle.
-int make_tmap_out(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t ld, int dtype) {
+// ---- pairs of CTAs -----------------------------------------------------------------------------------------------
+// One tile of 256 rows of X x 256 rows of W per cluster of two CTAs (tcgen05.mma cta_group::2): each CTA holds 128 rows of
+// either operand and the accumulator of its 128 rows of X; the MMA, issued by rank 0, reads both CTAs' halves of W.  A
+// CTA then fetches 32 KB of codes per 256 columns of K where the single-CTA tile of 128 x 256 fetches 48 KB, and the
+// fabric between L2 and the SMs (about 64 bytes per clock and SM) was what that one waited for.
+// All copies of a stage, both CTAs', complete on rank 0's barrier (TMA with cta_group::2 may signal the pair's other CTA):
+// a first form in which rank 1 passed its completions on took 1370 clocks a stage instead of KSTAGE.
+template <int FMT>
+struct PairCfg {
+    static constexpr int kChunks = FMT == kMxFp4 ? 2 : 4;
+    static constexpr int kA = 128 * 128, kB = 128 * 128;
+    static constexpr int kSfa = 512 * kChunks, kSfb = 2 * kSfa;          // scales: this CTA's rows of X, all 256 rows of W
+    static constexpr int kStageBytes = kA + kB + kSfa + kSfb;
+    static constexpr int kStaging = (kEpi / 32) * 2 * 2048, kBars = 512;   // 64-byte rows: room for a fifth stage
+    static constexpr int kStages = 5;
+    static constexpr int kSfCols = 4 * kChunks * 3;
+    static constexpr int kAcc = 256, kTmem = 512;
+    static constexpr size_t kSmem = (size_t)kStages * kStageBytes + kStaging + kBars;
+    static_assert(kStageBytes % 1024 == 0 && kSmem <= 227 * 1024 && kAcc + 2 * kSfCols <= kTmem, "sizes");
+};
+// TMA box into this CTA's shared memory, completion on a barrier of either CTA of the pair (shared::cluster address).
+__device__ __forceinline__ void tma_load_pair(uint32_t smem_dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(smem_dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+template <int FMT>
+__device__ __forceinline__ void umma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+    if constexpr (FMT == kMxFp4)
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                     " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                     " tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%5], [%6], p;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
+}
+__device__ __forceinline__ void cp_sf_pair(uint32_t taddr, uint64_t sdesc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc) : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs when the MMAs issued so far are complete.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(kGThreads, 1)
+fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
+                     const __grid_constant__ CUtensorMap tmap_sp, const __grid_constant__ CUtensorMap tmap_sq,
+                     const __grid_constant__ CUtensorMap tmap_o, const GemmArgs a) {
+    using C = PairCfg<FMT>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t base = tc::smem_u32(smem_raw);
+    const uint32_t staging = base + C::kStages * C::kStageBytes, bars = staging + C::kStaging;
+    auto full = [&](int s) { return bars + 8u * s; };                     // (rank 0's alone is used)
+    auto empty = [&](int s) { return bars + 8u * (C::kStages + s); };
+    const uint32_t acc_full = bars + 16u * C::kStages, acc_empty = acc_full + 8u, tmem_slot = acc_full + 16u;
+    int& s_fail = *reinterpret_cast<int*>(smem_raw + (acc_full + 20u - base));
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const int64_t G = groups(a.K), Cch = FMT == kMxFp4 ? G : 2 * G;
+    const int nkb = (int)((G + 1) / 2);
+    const int n_tiles = a.tiles_p * a.tiles_q, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    constexpr int kBand = 4;   // bands of tiles along P, so that the pairs in flight share operand tiles through L2
+    auto tile_at = [&](int t, int64_t& p0, int64_t& q0) {
+        const int band = t / (kBand * a.tiles_q), in = t - band * kBand * a.tiles_q;
+        const int h = min(kBand, a.tiles_p - band * kBand);
+        p0 = (int64_t)(band * kBand + in % h) * 256;
+        q0 = (int64_t)(in / h) * 256;
+    };
+    if (threadIdx.x == 0) {
+        s_fail = (base & 1023u) != 0;
+        for (int s = 0; s < C::kStages; ++s) {
+            tc::mbar_init(full(s), 1);
+            tc::mbar_init(empty(s), 1);
+        }
+        tc::mbar_init(acc_full, 1);
+        tc::mbar_init(acc_empty, 2 * kEpi / 32);
+        tc::mbar_fence_init();
+        tc::prefetch_tmap(&tmap_p);
+        tc::prefetch_tmap(&tmap_q);
+        tc::prefetch_tmap(&tmap_o);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "n"(C::kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc::tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc::tc_fence_after();
+    uint32_t tmem;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    constexpr uint32_t b_off = C::kA, sfa_off = C::kA + C::kB, sfb_off = sfa_off + C::kSfa;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            if (a.pdl) pdl_wait();   // X is written by the kernel before this one
+            int s = 0, round = 0;
+            bool ok = true;
+            const uint32_t lead = map_rank(full(0), 0);
+            for (int t = first; t < n_tiles && ok; t += step) {
+                int64_t p0, q0;
+                tile_at(t, p0, q0);
+                // rows of 512 bytes in the scale maps: chunks; what lies behind a matrix's or a row's end reads something finite
+                // or zero and meets no stored output
+                const int64_t sp = (p0 / 128 + rank) * Cch, sq = q0 / 128 * Cch;
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                    const uint32_t st = base + s * C::kStageBytes, bar = lead + 8u * s;
+                    if (rank == 0) tc::mbar_expect_tx(full(s), 2 * C::kStageBytes);
+                    tma_load_pair(st, &tmap_p, kb * 128, (int)p0 + 128 * rank, bar);
+                    tma_load_pair(st + b_off, &tmap_q, kb * 128, (int)q0 + 128 * rank, bar);
+                    tma_load_pair(st + sfa_off, &tmap_sp, 0, (int)sp + kb * C::kChunks, bar);
+                    tma_load_pair(st + sfb_off, &tmap_sq, 0, (int)sq + kb * C::kChunks, bar);
+                    tma_load_pair(st + sfb_off + C::kSfa, &tmap_sq, 0, (int)(sq + Cch) + kb * C::kChunks, bar);
+                    if (++s == C::kStages) { s = 0; ++round; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (elect_one()) {
+            int s = 0, par = 0;
+            bool ok = true;
+            if (rank == 0) {
+                int it = 0, tile_no = 0;
+                for (int t = first; t < n_tiles && ok; t += step, ++tile_no) {
+                    if (tile_no && !tc::mbar_wait(acc_empty, (tile_no - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                    tc::tc_fence_after();
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        if (!tc::mbar_wait(full(s), par)) { atomicExch(&s_fail, 1); ok = false; break; }
+                        tc::tc_fence_after();
+                        const uint32_t st = base + s * C::kStageBytes;
+                        const uint32_t sfa_t = tmem + C::kAcc + (uint32_t)(it & 1) * C::kSfCols, sfb_t = sfa_t + 4 * C::kChunks;
+                        const int steps = (int)min((int64_t)4, (a.K - (int64_t)kb * kBK + 63) / 64);
+                        const int nch = FMT == kMxFp4 ? (steps + 1) / 2 : steps;
+                        auto scales = [&](int c) {
+                            if (c >= nch) return;
+                            cp_sf_pair(sfa_t + 4 * c, sf_desc(st + sfa_off + 512 * c));
+                            cp_sf_pair(sfb_t + 8 * c, sf_desc(st + sfb_off + 512 * c));
+                            cp_sf_pair(sfb_t + 8 * c + 4, sf_desc(st + sfb_off + C::kSfa + 512 * c));
+                        };
+                        const uint64_t ad = tc::umma_desc_sw128(st), bd = tc::umma_desc_sw128(st + b_off);
+                        // the copies of a word's scales go one word ahead of its MMAs: they run beside the MMAs before them
+                        scales(0);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if (k >= steps) break;
+                            const int c = FMT == kMxFp4 ? k / 2 : k;
+                            if (FMT == kNvFp4 || k % 2 == 0) scales(c + 1);
+                            // M = 256 of the pair: the field of fp4_idesc holds M = 128
+                            umma_pair<FMT>(tmem, ad + 2u * k, bd + 2u * k, fp4_idesc<FMT>(256, FMT == kMxFp4 ? 2 * (k & 1) : 0) + ((128u >> 4) << 24),
+                                           sfa_t + 4 * c, sfb_t + 8 * c, (kb | k) ? 1u : 0u);
+                        }
+                        commit_pair(empty(s));
+                        if (++s == C::kStages) { s = 0; par ^= 1; }
+                    }
+                    commit_pair(acc_full);
+                }
+            }
+        }
+    } else {
+        const int w = warp - 2, quarter_warp = (warp & 3) | (w >= 4 ? 4 : 0);
+        const uint32_t peer_empty = map_rank(acc_empty, 0);               // (rank 0's, for both)
+        int tile_no = 0, turn = 0;
+        for (int t = first; t < n_tiles; t += step, ++tile_no) {
+            int64_t p0, q0;
+            tile_at(t, p0, q0);
+            const bool done = tc::mbar_wait(acc_full, tile_no & 1, 4000000000ll);
+            tc::tc_fence_after();
+            if (!done) atomicExch(&s_fail, 1);
+            const bool go = __shfl_sync(0xffffffffu, (done && *(volatile int*)&s_fail == 0) ? 1 : 0, 0) != 0;
+            if (!go) break;
+            const uint32_t buf = staging + (uint32_t)w * 4096;
+            const int64_t pr = p0 + 128 * rank;
+            if (a.dtype == kBf16) store_rows<__nv_bfloat16, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, peer_empty, turn);
+            else if (a.dtype == kF16) store_rows<__half, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, peer_empty, turn);
+            else store_rows<float, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, peer_empty, turn);
+        }
+        if (lane == 0) bulk_wait<0>();
+    }
+    __syncwarp();
+    tc::tc_fence_before();
+    cluster_sync_all();   // no CTA leaves while the pair's MMAs, commits or arrivals may still reach it
+    if (threadIdx.x == 0 && s_fail && a.status) { a.status[0] = FB_TIMEOUT; a.status[1] = blockIdx.x; a.status[2] = 3000; a.status[3] = rank; }
+    if (warp == 1) {
+        tc::tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kTmem) : "memory");
+    }
+}
+
+// Output [rows, cols] in boxes of 32 rows x row_bytes (128 or 64), swizzled.
+int make_tmap_out(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, uint64_t ld, int dtype, int row_bytes) {
     static_assert(kF32 == 0 && kBf16 == 1 && kF16 == 2, "the order of the table below");
     const CUtensorMapDataType types[3] = {CU_TENSOR_MAP_DATA_TYPE_FLOAT32, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16};
     const uint64_t esz = dtype == kF32 ? 4 : 2;
     cuuint64_t dims[2] = {cols, rows};
     cuuint64_t strides[1] = {ld * esz};
-    cuuint32_t box[2] = {(cuuint32_t)(128 / esz), 32};
+    cuuint32_t box[2] = {(cuuint32_t)(row_bytes / esz), 32};
     cuuint32_t estr[2] = {1, 1};
-    return fp4_encode_tmap(map, types[dtype], base, dims, strides, box, estr);
+    return fp4_encode_tmap(map, types[dtype], base, dims, strides, box, estr, row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// Scale chunks as rows of 128 words, in boxes of `box_rows`.
+int make_tmap_scales(CUtensorMap* map, const void* base, uint64_t chunks, uint32_t box_rows) {
+    cuuint64_t dims[2] = {128, chunks};
+    cuuint64_t strides[1] = {512};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    return fp4_encode_tmap(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, dims, strides, box, estr, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <int FMT, int BN, bool SWAP, bool QX = false>
@@ -464,7 +668,7 @@ int launch_gemm(const GemmArgs& a, const void* pc, const void* qc, int grid, cud
     int rc = fb_make_tmap_2d(&tp, pc, (uint64_t)a.P, bytes, 128, 128, 1);
     tq = to = tp;   // (QX has no operand Q in memory; `to` is not used by P = W or an output that TMA cannot address)
     if (!rc && !QX) rc = fb_make_tmap_2d(&tq, qc, (uint64_t)a.Q, bytes, BN, 128, 1);
-    if (!rc && !SWAP && a.vec) rc = make_tmap_out(&to, a.out, (uint64_t)a.P, (uint64_t)a.Q, (uint64_t)a.ldo, a.dtype);
+    if (!rc && !SWAP && a.vec) rc = make_tmap_out(&to, a.out, (uint64_t)a.P, (uint64_t)a.Q, (uint64_t)a.ldo, a.dtype, 128);
     if (rc) return rc;
     auto k = fp4_gemm_kernel<FMT, BN, SWAP, QX>;
     static unsigned long long allowed = 0;
@@ -475,6 +679,26 @@ int launch_gemm(const GemmArgs& a, const void* pc, const void* qc, int grid, cud
 
 constexpr int kNotTaken = -1;     // X is not quantised inside the product at these sizes
 constexpr int kQxRows = 16;       // rows times blocks of 256 columns per CTA up to which it is
+
+template <int FMT>
+int launch_pair(GemmArgs a, const void* pc, const void* qc, cudaStream_t st) {
+    using C = PairCfg<FMT>;
+    CUtensorMap tp, tq, tsp, tsq, to;
+    const uint64_t bytes = (uint64_t)(64 * groups(a.K)), cch = (uint64_t)(FMT == kMxFp4 ? 1 : 2) * groups(a.K);
+    int rc = fb_make_tmap_2d(&tp, pc, (uint64_t)a.P, bytes, 128, 128, 1);
+    if (!rc) rc = fb_make_tmap_2d(&tq, qc, (uint64_t)a.Q, bytes, 128, 128, 1);
+    if (!rc) rc = make_tmap_scales(&tsp, a.sfp, (uint64_t)((a.P + 127) / 128) * cch, C::kChunks);
+    if (!rc) rc = make_tmap_scales(&tsq, a.sfq, (uint64_t)((a.Q + 127) / 128) * cch, C::kChunks);
+    to = tp;   // (not used by an output that TMA cannot address)
+    if (!rc && a.vec) rc = make_tmap_out(&to, a.out, (uint64_t)a.P, (uint64_t)a.Q, (uint64_t)a.ldo, a.dtype, 64);
+    if (rc) return rc;
+    auto k = fp4_gemm_pair_kernel<FMT>;
+    static unsigned long long allowed = 0;
+    cudaError_t e = fp4_allow_smem(k, C::kSmem, allowed);
+    if (e != cudaSuccess) return (int)e;
+    const int tiles = a.tiles_p * a.tiles_q, pairs = 74;
+    return (int)fp4_launch(k, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), dim3(kGThreads), C::kSmem, st, 2, a.pdl != 0, tp, tq, tsp, tsq, to, a);
+}
 
 template <int FMT>
 int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, const uint8_t* ws, int64_t M, int64_t N, cudaStream_t st) {
@@ -509,8 +733,8 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
     if (a.x) return kNotTaken;
     a.P = M; a.Q = N; a.sfp = xs; a.sfq = ws;
     a.tiles_p = (int)((M + 127) / 128);
-    // Tile width and K split by the clocks of the longest-running CTA: a stage (256 columns of K) takes about 600 on 256
-    // output columns and 470 on 128 (four MMAs and the scale copies), a tile about 1500 at its ends that the next one does
+    // Tile width and K split by the clocks of the longest-running CTA: a stage (256 columns of K) takes about 850 on 256
+    // output columns and 560 on 128 (the operands' way from L2), 600 in a pair, a tile about 1500 at its ends that the next one does
     // not hide, an exchange between split CTAs 3000.  Clusters of a split stay resident (33 of 4, 15 of 8).
     const int resident[4] = {sms, 74, 33, 15};
     double cost = 0;
@@ -521,9 +745,17 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
         for (int l = 0; l < 4; ++l) {
             const int s = 1 << l;
             if (l && (tiles > resident[l] || nkb < 2 * s)) break;
-            const double c = (double)((tiles + sms - 1) / sms) * ((double)((nkb + s - 1) / s) * (w ? 600 : 470) + 1500) + (s > 1 ? 3000 : 0);
+            const double c = (double)((tiles + sms - 1) / sms) * ((double)((nkb + s - 1) / s) * (w ? 850 : 560) + 1500) + (s > 1 ? 3000 : 0);
             if (cost == 0 || c < cost) { cost = c; wide = w; S = s; }
         }
+    }
+    const int64_t pair_p = (M + 255) / 256, pair_q = (N + 255) / 256, pair_tiles = pair_p * pair_q;
+    if (pair_tiles > 0x3fffffff) return (int)cudaErrorInvalidValue;
+    if ((double)((pair_tiles + 73) / 74) * ((double)nkb * 600 + 1700) < cost) {
+        a.tiles_p = (int)pair_p;
+        a.tiles_q = (int)pair_q;
+        a.splits = 1;
+        return launch_pair<FMT>(a, xc, wc, st);
     }
     a.tiles_q = (int)((N + (wide ? 255 : 127)) / (wide ? 256 : 128));
     const int64_t tiles = (int64_t)a.tiles_p * a.tiles_q;

@@ -136,7 +136,8 @@ def close(got, want, mag, K, dtype):
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 128, 256), (2, 130, 64), (16, 127, 1000), (17, 300, 96), (33, 129, 2048),
                                    (65, 257, 33), (100, 512, 4160), (128, 128, 128), (129, 255, 160), (333, 1111, 1000),
-                                   (300, 640, 4096), (1, 5120, 8192)])
+                                   (300, 640, 4096), (1, 5120, 8192), (1000, 4700, 1000), (1024, 4608, 640), (1200, 4609, 160),
+                                   (2304, 8200, 96)])
 def test_matmul(fmt, M, N, K):
     g = _gen(M + N + K)
     a = fp4.quantize((torch.randn(M, K, generator=g) * torch.rand(M, 1, generator=g) * 3).cuda(), fmt)
