@@ -29,6 +29,7 @@ from .quant import e2m1_unpack
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LINEAR_INSIDE = 16   # 128-column groups of one row that fb_fp4_linear always quantises inside the product
 
 
 class Fp4Tensor:
@@ -122,7 +123,7 @@ def _check_scale(ts: float, fmt: str) -> None:
 def _call(device: torch.device, name: str, *args) -> None:
     index = device.index
     stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         _lib.lib().call(name, *args, stream=stream)
     else:
         with torch.cuda.device(index):
@@ -135,11 +136,14 @@ def _matrix(x: torch.Tensor, what: str) -> Tuple[int, int, int, int, int]:
         raise TypeError(f"{what} is float32, bfloat16 or float16, got {x.dtype}")
     if not x.is_cuda:
         raise ValueError(f"{what} is not on a CUDA device")
-    if x.dim() < 2:
-        raise ValueError(f"{what} has a shape [..., rows, cols], got {tuple(x.shape)}")
-    rows, cols = x.shape[-2:]
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"{what} has a shape [..., rows, cols], got {tuple(shape)}")
+    rows, cols = shape[-2:]
     if cols < 1:
         raise ValueError(f"{what} has no columns")
+    if len(shape) == 2 and x.is_contiguous():
+        return 1, rows, cols, 0, cols
     ld = x.stride(-2) if rows > 1 else cols
     if (cols > 1 and x.stride(-1) != 1) or ld < cols:
         raise ValueError(f"{what} has rows of consecutive values that do not overlap, got strides {x.stride()}")
@@ -227,18 +231,25 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
     if x_scale is not None:
         _check_scale(x_scale, w.fmt)
     _, M, K, _, ldx = _matrix(x, "x")
-    if x.device != w.device:
-        raise ValueError(f"x is on {x.device}, w on {w.device}")
-    N = w.shape[0]
     dev = x.device
-    out, (_, _, _, _, ldo) = _out(out, (M, N), out_dtype or x.dtype, dev)
+    if dev != w.device:
+        raise ValueError(f"x is on {dev}, w on {w.device}")
+    N = w.shape[0]
+    if out is None:
+        out, ldo = torch.empty(M, N, dtype=out_dtype or x.dtype, device=dev), N
+        if out.dtype not in _DTYPES:
+            raise TypeError(f"out is float32, bfloat16 or float16, got {out.dtype}")
+    else:
+        out, (_, _, _, _, ldo) = _out(out, (M, N), out.dtype, dev)
     if M and N:
         g = (K + 127) // 128
-        work = torch.empty((M * 64 * g + 511) // 512 * 512 + (M + 127) // 128 * (g if w.fmt == "mxfp4" else 2 * g) * 512,
-                           dtype=torch.uint8, device=dev)
-        alpha = float(x_scale or 1.0) * float(w.tensor_scale or 1.0)
+        work = None
+        if M > 1 or g > LINEAR_INSIDE:   # (one row of up to so many groups is quantised inside the product)
+            work = torch.empty((M * 64 * g + 511) // 512 * 512 + (M + 127) // 128 * (g if w.fmt == "mxfp4" else 2 * g) * 512,
+                               dtype=torch.uint8, device=dev)
+        alpha = (x_scale or 1.0) * (w.tensor_scale or 1.0)
         _call(dev, "fb_fp4_linear", x, _DTYPES[x.dtype], ldx, work, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
-              FORMATS[w.fmt], float(x_scale or 0.0), alpha)
+              FORMATS[w.fmt], float(x_scale or 0.0), float(alpha))
     return out
 
 
