@@ -25,6 +25,7 @@ from typing import Dict, List, Optional
 import torch
 
 from .. import _lib
+from ..ops import fp4
 from ..ops import quant as Q
 from ..utils.switches import switches
 from .dsv41_config import Dsv41Config
@@ -92,6 +93,7 @@ class Dsv41DeviceModel:
         self.tc_gemv_min_n = 0
         self.fp4_mma = switches().d4_fp4_mma   # tensor-core routed experts (decode rows)
         self.fp4_mma_rows = 1 << 30
+        self.moe2 = switches().d4_moe_two      # routed experts of decode rows as two kernels (ops/fp4.py)
         # row count from which the routed experts run as block-scaled tcgen05 grouped GEMMs (csrc/kernels/mx_gemm.cu):
         # below it the weight-streaming mma.sync kernels stream every (row, slot) pair's expert once per pair
         self.mx_min_rows = switches().d4_mx_min_rows
@@ -186,7 +188,14 @@ class Dsv41DeviceModel:
                 s2[e].copy_(sc)
             L["w13"], L["s13"], L["w2"], L["s2"] = w13, s13, w2, s2
         # tensor-core expert kernels want 128-value k-blocks and quad-interleaved weight bytes (repacked in place)
-        L["fp4_mma"] = self.fp4_mma and d % 128 == 0 and Il % 64 == 0
+        # (the two-kernel expert layer of ops/fp4.py reads the checkpoint's byte order)
+        L["moe2"] = self.moe2 and d % 128 == 0 and Il % 32 == 0 and E <= fp4.MOE_MAX_EXPERTS and topk <= fp4.MOE_MAX_TOPK and d <= fp4.MOE_MAX_DIM
+        if L["moe2"]:
+            pad = (-Il // 2) % 64   # rows of whole 128-value groups
+            w2 = torch.nn.functional.pad(L["w2"], (0, pad)) if pad else L["w2"]
+            L["moe2_w13"] = fp4.Fp4Tensor(L["w13"], fp4.pack_scales(L["s13"]), "mxfp4", (E, 2, Il, d))
+            L["moe2_w2"] = fp4.Fp4Tensor(w2, fp4.pack_scales(L["s2"]), "mxfp4", (E, d, Il))
+        L["fp4_mma"] = self.fp4_mma and d % 128 == 0 and Il % 64 == 0 and not L["moe2"]
         if L["fp4_mma"]:
             for t in (L["w13"], L["w2"]):
                 self.K.call("fb_d4_fp4_repack", t, t.numel() // t.shape[-1], t.shape[-1], 0)
@@ -615,6 +624,27 @@ class Dsv41DeviceModel:
         d, x, xq = cfg.dim, ws["x"], ws["xq"]
         E, topk = L["E"], L["topk"]
         ldl = ws["rlogit"].shape[1]
+        if (L["moe2"] and n <= fp4.MOE_MAX_TOKENS and not (L.get("mx") and n >= self.mx_min_rows) and x.s is not None
+                and xq.s is not None and d % 64 == 0 and not (self.has_images and L["gate_bvl"] is not None) and self.debug is None):
+            # Decode rows: routing, the experts and the sum over them in two kernels; the shared expert's chain beside the
+            # router's as below
+            if not self._xq_ready:
+                self._quant(x.f, xq, n, d, mask=3)
+            self._xq_ready = False
+            hs, gu = ws["hs"], ws["gu"]
+            self.K.call("fb_gemv_mma_bf16_dual", L["gate_w"], x.s, x.ld, x.plane, ws["rlogit"], ldl, E, d,
+                        L["sh_w13"], xq.s, xq.ld, xq.plane, gu, gu.shape[1], 2 * self.Is, d, n)
+            self.K.call("fb_d4_swiglu_clamp_quant", gu, gu.shape[1], hs.f, self.Is, n, self.Is, float(cfg.swiglu_limit), *hs.sp(1))
+            fp4.moe(x.f[:n, :d], ws["rlogit"][:n, :E], L["moe2_w13"], L["moe2_w2"], topk, bias=L["gate_b"], score="sqrtsoftplus",
+                    norm=topk > 1, scale=float(cfg.route_scale), limit=max(0.0, float(cfg.swiglu_limit)), out=ws["y"][:n])
+            if not self.shared_tp:
+                self._reduce(ws["y"], n)
+            if self.shared_tp or self.world == 1:
+                self._out_gemv(L["sh_w2"], hs, n, d, self.Is, accumulate=True)
+            else:
+                self._fold_next = None
+                self.gemv(L["sh_w2"], hs, ws["y"], n, d, self.Is, accumulate=True)
+            return
         if (L["fp4_mma"] and n <= self.fp4_mma_rows and not (L.get("mx") and n >= self.mx_min_rows) and E <= 384
                 and topk <= 32 and d % 64 == 0 and x.s is not None and xq.s is not None and self.moe_paired):
             # Decode rows.  The router chain (logits -> route) and the shared expert's chain (gate | up -> SwiGLU) do

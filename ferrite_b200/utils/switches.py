@@ -49,6 +49,8 @@ class Switches:
     d4_fused_rows: int = 8          # DSV41: forwards of up to this many rows close their sublayers with the fused GEMV + all-reduce
                                     # (16: two 8-row windows per launch site, 80 launches fewer per 16-row tick but 15.9 vs 15.5 ms)
     d4_fp4_mma: bool = True         # DSV41 routed experts of decode rows on the tensor cores
+    d4_moe_two: bool = False        # DSV41 routed experts of decode rows as the two-kernel layer of ops/fp4.py (routing inside,
+                                    # weights unpacked by TMA); the expert weights then keep the checkpoint's byte order
     d4_attn_tc: bool = False        # DSV41 tensor-core sparse attention (slower than the SIMT kernel at decode sizes)
     d4_fuse_quant: bool = False     # DSV41 activation quantiser fused into hc_pre (a one-CTA latency chain; slower)
     dump_dir: str = ""              # directory for unit dumps ("" = off)

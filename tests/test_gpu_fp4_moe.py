@@ -230,3 +230,48 @@ def test_a_decode_step_of_the_operators_together():
     mq, wo = fp4.reference_dequantize(fp4.quantize(m)), fp4.reference_dequantize(w_out)
     want = mq @ wo.t()
     assert ((y.double() - want).abs() <= (D + 2) * E24 * (mq.abs() @ wo.abs().t()) + 2.0 ** -8 * want.abs()).all()
+
+
+@pytest.mark.parametrize("rows", [1, 5])
+def test_dsv41_decode_through_the_two_kernel_layer(rows):
+    """The tiny DSV41 model with its routed experts as this layer against the per-pair expert kernels: both multiply the
+    same e2m1 x e4m3 values, so the logits agree up to summation order; and a captured step replays it."""
+    from ferrite_b200.models.dsv41 import DictWeights, Dsv41DeviceModel
+    from ferrite_b200.models.dsv41_config import Dsv41Config
+    from ferrite_b200.models.dsv41_weights import random_weights
+    from ferrite_b200.utils.switches import Switches, set_switches
+    cfg = Dsv41Config.tiny()
+    w = random_weights(cfg, 4)
+    ids = torch.randint(0, cfg.vocab_size - 20, (20,), generator=torch.Generator().manual_seed(3)).tolist()
+    logits = {}
+    try:
+        for two in (False, True):
+            set_switches(Switches(d4_moe_two=two))
+            dev = Dsv41DeviceModel(cfg, DictWeights(w), max_rows=8, max_ctx=128)
+            assert all(L["moe2"] == two for L in dev.layers)
+            out = []
+            for i in range(0, len(ids), rows):
+                c = ids[i:i + rows]
+                dev.forward(dev.make_rows([0], [len(c)]), torch.tensor(c, dtype=torch.int32, device="cuda"))
+                out.append(dev.ws["logits"][:len(c)].cpu().clone())
+            torch.cuda.synchronize()
+            fp4.check()
+            logits[two] = torch.cat(out)
+            if two:
+                rs = dev.make_rows([0], [1])
+                tok = torch.tensor(ids[:1], dtype=torch.int32, device="cuda")
+                dev.reset_slot(0)
+                dev.forward(rs, tok, advance=False)
+                want = dev.ws["logits"][:1].clone()
+                dev.reset_slot(0)
+                gr = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(gr):
+                    dev.forward(rs, tok, advance=False)
+                dev.ws["logits"].zero_()
+                gr.replay()
+                assert torch.equal(dev.ws["logits"][:1], want)
+    finally:
+        set_switches(None)
+    a, b = logits[True], logits[False]
+    assert (a - b).abs().max().item() < 2e-3 * b.abs().max().item(), (a - b).abs().max().item()
+    assert torch.equal(a.argmax(-1), b.argmax(-1))
