@@ -194,6 +194,20 @@ __device__ __forceinline__ void umma_w4a8(uint32_t d, uint64_t a, uint64_t b, ui
                  " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
 }
+// The four MMAs of a 128-column block.
+template <int BN>
+__device__ __forceinline__ void mma_block(uint32_t d, uint64_t w, uint64_t x, uint32_t sfw, uint32_t sfx, bool accumulate) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) umma_w4a8(d, w + 2u * k, x + 2u * k, moe_idesc(BN, k), sfw, sfx, accumulate || k ? 1u : 0u);
+}
+// Both stages full (the second only if `two`).  The tensor core holds few MMAs in its queue, so it idles while this thread waits
+// (about 75 clocks, against 156 for a block's four MMAs): two blocks per wait.
+__device__ __forceinline__ bool wait_two(uint32_t bar0, uint32_t par0, uint32_t bar1, uint32_t par1, bool two) {
+    const bool r0 = tc::mbar_try_wait(bar0, par0), r1 = !two || tc::mbar_try_wait(bar1, par1);
+    const bool ok = (r0 || tc::mbar_wait(bar0, par0)) && (r1 || tc::mbar_wait(bar1, par1));
+    tc::tc_fence_after();
+    return ok;
+}
 __device__ __forceinline__ void tmem_ld1(uint32_t taddr, float& v) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=f"(v) : "r"(taddr) : "memory");
 }
@@ -363,9 +377,12 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const int items = R.n_act * a.nit;
     const int first = blockIdx.x / S, step = gridDim.x / S;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 6) {
         if (elect_one()) {
-            int s = 0, round = 0;     // stage and how often the ring went round (no divisions on this thread's path)
+            // Two producers take turns: one thread needs about 310 clocks for a block's wait, count and two copies, more than
+            // the block's MMAs.  Stage and how often the ring went round are counted, not divided for.
+            const int mine = warp == 6;
+            int s = mine, round = 0, it = 0;
             bool ok = true;
             for (int item = first; item < items && ok; item += step) {
                 const int e = R.act[item / a.nit], j = item % a.nit;
@@ -375,8 +392,10 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                 // the barrier counts the packed bytes: 64 per row of 128 codes
                 const uint32_t bytes = (boxes ? boxes * 32 * 64 : 128 * 64) + 512;
                 for (int m = 0; m < 2 && ok; ++m, row += a.I, sf += (int64_t)a.nit * a.g1 * 512) {   // gate, up
-                    const uint8_t* f = sf;
-                    for (int kb = kb0; kb < kb1; ++kb, f += 512) {
+                    const int skip = (it & 1) != mine;
+                    it += nkb;
+                    const uint8_t* f = sf + skip * 512;
+                    for (int kb = kb0 + skip; kb < kb1; kb += 2, f += 1024) {
                         if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
                         const uint32_t st = base + st_off + (uint32_t)s * C::kA;
                         tc::mbar_expect_tx(full(s), bytes);
@@ -384,7 +403,8 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                         else
                             for (int b = 0; b < boxes; ++b) tc::tma_load_2d(st + b * 32 * 128, &tmap_tail, kb * 128, row + 32 * b, full(s));
                         bulk_load(base + sf_off + s * 512, f, 512, full(s));
-                        if (++s == stages) { s = 0; ++round; }
+                        s += 2;
+                        if (s >= stages) { s -= stages; ++round; }
                     }
                 }
             }
@@ -393,7 +413,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         if (elect_one()) {
             // x's scales stay in tensor memory
             for (int kb = 0; kb < nkb; ++kb) tmem_cp_sf(tmem + C::kSfX + 4 * kb, sf_desc(base + xsf_off + kb * 512));
-            int s = 0, par = 0, it = 0, no = 0;
+            int s = 0, par = 0, no = 0;
             bool ok = true;
             for (int item = first; item < items && ok; item += step, ++no) {
                 const int buf = no & 1;
@@ -402,17 +422,22 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                 // all of the gate product, then all of up: a change of accumulator costs about 140 clocks, an MMA 57
                 for (int m = 0; m < 2 && ok; ++m) {
                     const uint32_t d = tmem + (uint32_t)(buf * C::kAccSet + m * BN);
-                    for (int kb = 0; kb < nkb; ++kb, ++it) {
-                        if (!tc::mbar_wait(full(s), par)) { atomicExch(&s_fail, 1); ok = false; break; }
-                        tc::tc_fence_after();
-                        const uint32_t sf = tmem + C::kSfW + (uint32_t)(it & 1) * 4;
+                    for (int kb = 0; kb < nkb; kb += 2) {
+                        const bool two = kb + 1 < nkb;
+                        const int s1 = s + 1 == stages ? 0 : s + 1, par1 = s + 1 == stages ? par ^ 1 : par;
+                        if (!wait_two(full(s), par, full(s1), par1, two)) { atomicExch(&s_fail, 1); ok = false; break; }
+                        const uint32_t sf = tmem + C::kSfW;
                         tmem_cp_sf(sf, sf_desc(base + sf_off + s * 512));
-                        const uint64_t wd = tc::umma_desc_sw128(base + st_off + (uint32_t)s * C::kA);
+                        if (two) tmem_cp_sf(sf + 4, sf_desc(base + sf_off + s1 * 512));
                         const uint64_t xd = tc::umma_desc_sw128(base + (uint32_t)kb * BN * 128);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            umma_w4a8(d, wd + 2u * k, xd + 2u * k, moe_idesc(BN, k), sf, tmem + C::kSfX + 4 * kb, (kb | k) ? 1u : 0u);
+                        mma_block<BN>(d, tc::umma_desc_sw128(base + st_off + (uint32_t)s * C::kA), xd, sf, tmem + C::kSfX + 4 * kb, kb > 0);
                         tc::umma_commit(empty(s));
+                        if (two) {
+                            mma_block<BN>(d, tc::umma_desc_sw128(base + st_off + (uint32_t)s1 * C::kA), xd + BN * 128 / 16, sf + 4, tmem + C::kSfX + 4 * kb + 4, true);
+                            tc::umma_commit(empty(s1));
+                            s = s1;
+                            par = par1;
+                        }
                         if (++s == stages) { s = 0; par ^= 1; }
                     }
                 }
@@ -574,47 +599,47 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
     const int64_t units = (int64_t)s_n * a.nit;
     const int u0 = (int)(units * rank / S), u1 = (int)(units * (rank + 1) / S);
 
-    if (warp == 0) {
-        if (elect_one()) {
-            int ai = u0 / a.nit, kb = u0 - ai * a.nit, e = ai < s_n ? s_act[ai] : 0;
-            auto arm_w = [&](int s) {   // the next block in order
+    if (warp == 0 || warp == 6) {
+        if (elect_one()) {   // two producers, every other block each, as in kernel 1
+            const int mine = warp == 6;
+            int u = u0 + mine, ai = u / a.nit, kb = u - ai * a.nit, s = mine, round = 0;
+            for (; u < u1; u += 2) {
+                if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); break; }
                 const uint32_t st = base + (uint32_t)s * C::kStage;
+                const int e = s_act[ai];
                 tc::mbar_expect_tx(full(s), 128 * 64 + 512 + BN * 128 + 512);
                 tc::tma_load_2d(st, &tmap_w, kb * 128, e * a.D + d0, full(s));
                 bulk_load(st + C::kA + BN * 128, a.s2 + (((int64_t)e * ntd + tile) * a.nit + kb) * 512, 512, full(s));
-                if (++kb == a.nit) {
-                    kb = 0;
-                    if (++ai < s_n) e = s_act[ai];
-                }
-            };
-            auto load_h = [&](int s, int u) {
-                const uint32_t st = base + (uint32_t)s * C::kStage;
                 bulk_load(st + C::kA, a.h + (int64_t)u * (BN * 128), BN * 128, full(s));
                 bulk_load(st + C::kA + BN * 128 + 512, a.hs + (int64_t)u * 512, 512, full(s));
-            };
-            int s = 0, round = 0;
-            for (int u = u0; u < u1; ++u) {
-                if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); break; }
-                arm_w(s);
-                load_h(s, u);
-                if (++s == C::kStages) { s = 0; ++round; }
+                kb += 2;
+                while (kb >= a.nit) { kb -= a.nit; ++ai; }
+                s += 2;
+                if (s >= C::kStages) { s -= C::kStages; ++round; }
             }
         }
     } else if (warp == 1) {
         if (elect_one()) {
             int s = 0, par = 0;
-            for (int it = 0; it < u1 - u0; ++it) {
-                if (!tc::mbar_wait(full(s), par)) { atomicExch(&s_fail, 1); break; }
-                tc::tc_fence_after();
-                const uint32_t st = base + (uint32_t)s * C::kStage;
-                const uint32_t sf = tmem + 32 + (uint32_t)(it & 1) * 8;
+            for (int u = u0; u < u1; u += 2) {
+                const bool two = u + 1 < u1;
+                const int s1 = s + 1 == C::kStages ? 0 : s + 1, par1 = s + 1 == C::kStages ? par ^ 1 : par;
+                if (!wait_two(full(s), par, full(s1), par1, two)) { atomicExch(&s_fail, 1); break; }
+                const uint32_t st = base + (uint32_t)s * C::kStage, st1 = base + (uint32_t)s1 * C::kStage, sf = tmem + 32;
                 tmem_cp_sf(sf, sf_desc(st + C::kA + BN * 128));
                 tmem_cp_sf(sf + 4, sf_desc(st + C::kA + BN * 128 + 512));
-                const uint64_t wd = tc::umma_desc_sw128(st), hd = tc::umma_desc_sw128(st + C::kA);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    umma_w4a8(tmem, wd + 2u * k, hd + 2u * k, moe_idesc(BN, k), sf, sf + 4, (it | k) ? 1u : 0u);
+                if (two) {
+                    tmem_cp_sf(sf + 8, sf_desc(st1 + C::kA + BN * 128));
+                    tmem_cp_sf(sf + 12, sf_desc(st1 + C::kA + BN * 128 + 512));
+                }
+                mma_block<BN>(tmem, tc::umma_desc_sw128(st), tc::umma_desc_sw128(st + C::kA), sf, sf + 4, u > u0);
                 tc::umma_commit(empty(s));
+                if (two) {
+                    mma_block<BN>(tmem, tc::umma_desc_sw128(st1), tc::umma_desc_sw128(st1 + C::kA), sf + 8, sf + 12, true);
+                    tc::umma_commit(empty(s1));
+                    s = s1;
+                    par = par1;
+                }
                 if (++s == C::kStages) { s = 0; par ^= 1; }
             }
             tc::umma_commit(acc_full);
