@@ -58,7 +58,7 @@ struct Route {
     uint16_t sel[kMaxTok * kMaxTopk];
     uint16_t act[kMaxE];                      // chosen experts, ascending
     float mx[kMaxTok], inv[kMaxTok];          // softmax: largest logit, 1 / sum
-    int n_act;
+    int n_act, next;
 };
 
 __device__ __forceinline__ uint32_t order_key(float v) {   // larger float -> larger key; NaN below every number; 0 is free
@@ -73,116 +73,149 @@ __device__ __forceinline__ float score_of(float z, int score, float mx, float in
     return sqrtf(fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
 }
 
-// All tokens' choices into r, by the first kRouteThreads threads of the block (barrier 2 among them; none at the end).
-// scratch: (T + 1) * E words.  Every CTA runs this once, before its first weight arrives: what counts is the length of
-// the dependent chain and the size of the code (straight-line code that runs once costs its instruction fetches: with the
-// scores unrolled over a lane's 16 experts it took 30 us for one token), so the score loops are rolled, the selection is a
-// tree over registers, and a token's scores are spread over the warps that have no token of their own.
-__device__ __forceinline__ void route_all(const MoeArgs& a, Route& r, float* scratch) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int nw = kRouteThreads / 32, kPer = kMaxE / 32;
-    auto sync = [&]() { asm volatile("bar.sync 2, %0;" ::"n"(kRouteThreads) : "memory"); };
-    float* lg = scratch;                                                   // logits, then in their place the keys
-    uint32_t* keys = reinterpret_cast<uint32_t*>(scratch);
-    float* bias = scratch + a.T * a.E;
-    for (int e = threadIdx.x; e < kMaxE; e += kRouteThreads) {
-        r.mask[e] = 0u;
-        if (e < a.E && a.bias) bias[e] = __ldg(a.bias + e);
-    }
-#pragma unroll 1
-    for (int t = warp; t < a.T; t += nw) {
-        float z[kPer];
+// The score for the choice: as score_of within a few units in the last place, in a third of its instructions (every expert of
+// every token takes one).  log1p(e) = 2 atanh(e / (2 + e)), the series to the 13th power: 5e-9 at e = 1.
+__device__ __forceinline__ float key_score(float z, int score, float mx, float inv_sum) {
+    if (score == kSigmoid) return __fdividef(1.f, 1.f + __expf(-z));
+    if (score == kSoftmax) return __expf(z - mx) * inv_sum;
+    const float e = __expf(-fabsf(z)), s = __fdividef(e, 2.f + e), q = s * s;
+    float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
+    p = fmaf(q, p, 1.f / 9.f);
+    p = fmaf(q, p, 1.f / 7.f);
+    p = fmaf(q, p, 1.f / 5.f);
+    p = fmaf(q, p, 1.f / 3.f);
+    p = fmaf(q, p, 1.f);
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaf(2.f * s, p, fmaxf(z, 0.f))));
+    return r;
+}
+
+// Routing.  Every CTA does it once, before its first weight arrives: what counts is the length of the dependent chain and
+// the size of the code (straight-line code that runs once costs its instruction fetches: with the scores unrolled over a
+// lane's 16 experts it took 30 us for one token), so the score loops are rolled and the selection is a tree over registers.
+// From eight tokens on a warp takes a token at a time; below, the first kRouteThreads threads share the scores.
+
+// Logits of token t to row (shared memory); for softmax its largest logit and 1 / sum.  One warp.
+__device__ __forceinline__ void route_load(const MoeArgs& a, Route& r, float* row, int t, int lane) {
+    constexpr int kPer = kMaxE / 32;
+    float z[kPer];
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) z[j] = lane + 32 * j < a.E ? __ldg(a.logits + t * a.ldl + lane + 32 * j) : -INFINITY;
+    for (int j = 0; j < kPer; ++j) z[j] = lane + 32 * j < a.E ? __ldg(a.logits + t * a.ldl + lane + 32 * j) : -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+        if (lane + 32 * j < a.E) row[lane + 32 * j] = z[j];
+    if (a.score == kSoftmax) {
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, z[j]);
+        mx = warp_max(mx);
+        if (mx == -INFINITY) mx = 0.f;
+        __syncwarp();
+#pragma unroll 1
+        for (int e = lane; e < a.E; e += 32) sum += expf(row[e] - mx);
+        sum = warp_sum(sum);
+        if (lane == 0) { r.mx[t] = mx; r.inv[t] = 1.f / sum; }
+    }
+}
+// The row's logits become keys, from expert `first` in steps of `step` (with a bias; without, the logit itself decides, exactly:
+// every score grows with its logit).
+__device__ __forceinline__ void route_keys(const MoeArgs& a, const Route& r, float* row, const float* bias, int t, int first, int step) {
+    const float mx = r.mx[t], inv = r.inv[t];
+#pragma unroll 1
+    for (int e = first; e < a.E; e += step)
+        reinterpret_cast<uint32_t*>(row)[e] = order_key(key_score(row[e], a.score, mx, inv) + bias[e]);
+}
+// The token's choice from its row.  One warp.
+__device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const float* row, int t, int lane) {
+    constexpr int kPer = kMaxE / 32;
+    uint32_t key[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        const int e = lane + 32 * j;
+        key[j] = e >= a.E ? 0u : a.bias ? __float_as_uint(row[e]) : order_key(row[e]);
+    }
+    int mine = 0;
+#pragma unroll 1
+    for (int k = 0; k < a.topk; ++k) {
+        uint32_t m[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) m[j] = key[j];
+#pragma unroll
+        for (int o = kPer / 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int j = 0; j < o; ++j) m[j] = max(m[j], m[j + o]);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, m[0]);
+        uint32_t hit = 0;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) hit |= key[j] == top ? 1u << j : 0u;
+        const uint32_t cand = hit ? (uint32_t)(lane + 32 * (__ffs(hit) - 1)) : 0xffffffffu;
+        const uint32_t e = __reduce_min_sync(0xffffffffu, cand);
+        if (lane == k) mine = (int)e;
+        const uint32_t gone = (e & 31u) == (uint32_t)lane ? 1u << (e >> 5) : 0u;
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
-            if (lane + 32 * j < a.E) lg[t * a.E + lane + 32 * j] = z[j];
-        if (a.score == kSoftmax) {
-            float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) mx = fmaxf(mx, z[j]);
-            mx = warp_max(mx);
-            if (mx == -INFINITY) mx = 0.f;
-            __syncwarp();
-#pragma unroll 1
-            for (int e = lane; e < a.E; e += 32) sum += expf(lg[t * a.E + e] - mx);
-            sum = warp_sum(sum);
-            if (lane == 0) { r.mx[t] = mx; r.inv[t] = 1.f / sum; }
-        }
+            if (gone >> j & 1) key[j] = 0u;
     }
-    sync();
-    // every score grows with its logit: without a bias the logit itself decides, exactly
+    float p = lane < a.topk ? score_of(__ldg(a.logits + t * a.ldl + mine), a.score, r.mx[t], r.inv[t]) : 0.f;
+    if (a.norm) p = p / (warp_sum(p) + 1e-20f);
+    if (lane < a.topk) {
+        r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
+        r.wt[t * kMaxTopk + lane] = p * a.scale;
+        atomicOr(&r.mask[mine], 1u << t);
+    }
+}
+// Few tokens: the first kRouteThreads threads.
+__device__ __forceinline__ void route_together(const MoeArgs& a, Route& r, float* rows, const float* bias) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int nw = kRouteThreads / 32;
+    auto sync = [&]() { asm volatile("bar.sync 2, %0;" ::"n"(kRouteThreads) : "memory"); };
+    if (warp < a.T) route_load(a, r, rows + warp * a.E, warp, lane);
     if (a.bias) {
-        const int stripes = a.T >= nw ? 1 : nw / a.T;
-#pragma unroll 1
-        for (int u = warp; u < a.T * stripes; u += nw) {
-            const int t = u / stripes, first = (u - t * stripes) * 32 + lane;
-            const float mx = r.mx[t], inv = r.inv[t];
-#pragma unroll 4
-            for (int e = first; e < a.E; e += 32 * stripes) {
-                const float z = lg[t * a.E + e];
-                keys[t * a.E + e] = order_key(score_of(z, a.score, mx, inv) + bias[e]);
-            }
+        sync();
+        const int stripes = nw / a.T;
+        if (warp < a.T * stripes) {
+            const int t = warp / stripes;
+            route_keys(a, r, rows + t * a.E, bias, t, (warp - t * stripes) * 32 + lane, 32 * stripes);
         }
         sync();
     }
-#pragma unroll 1
-    for (int t = warp; t < a.T; t += nw) {
-        uint32_t key[kPer];
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int e = lane + 32 * j;
-            key[j] = e >= a.E ? 0u : a.bias ? keys[t * a.E + e] : order_key(lg[t * a.E + e]);
-        }
-        int mine = 0;
-#pragma unroll 1
-        for (int k = 0; k < a.topk; ++k) {
-            uint32_t m[kPer];
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) m[j] = key[j];
-#pragma unroll
-            for (int o = kPer / 2; o > 0; o >>= 1)
-#pragma unroll
-                for (int j = 0; j < o; ++j) m[j] = max(m[j], m[j + o]);
-            const uint32_t top = __reduce_max_sync(0xffffffffu, m[0]);
-            uint32_t hit = 0;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) hit |= key[j] == top ? 1u << j : 0u;
-            const uint32_t cand = hit ? (uint32_t)(lane + 32 * (__ffs(hit) - 1)) : 0xffffffffu;
-            const uint32_t e = __reduce_min_sync(0xffffffffu, cand);
-            if (lane == k) mine = (int)e;
-            const uint32_t gone = (e & 31u) == (uint32_t)lane ? 1u << (e >> 5) : 0u;
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                if (gone >> j & 1) key[j] = 0u;
-        }
-        float p = lane < a.topk ? score_of(__ldg(a.logits + t * a.ldl + mine), a.score, r.mx[t], r.inv[t]) : 0.f;
-        if (a.norm) p = p / (warp_sum(p) + 1e-20f);
-        if (lane < a.topk) {
-            r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
-            r.wt[t * kMaxTopk + lane] = p * a.scale;
-            atomicOr(&r.mask[mine], 1u << t);
-        }
-    }
-    sync();
-    if (warp == 0) {
-        uint32_t on[kPer];
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) on[j] = __ballot_sync(0xffffffffu, r.mask[lane + 32 * j] != 0u);
-        int n = 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            if (on[j] >> lane & 1) r.act[n + __popc(on[j] & ((1u << lane) - 1u))] = (uint16_t)(lane + 32 * j);
-            n += __popc(on[j]);
-        }
-        if (lane == 0) r.n_act = n;
+    __syncwarp();
+    if (warp < a.T) route_pick(a, r, rows + warp * a.E, warp, lane);
+}
+// Many tokens: any warp, the next token that nobody has taken.
+__device__ __forceinline__ void route_in_turn(const MoeArgs& a, Route& r, float* rows, const float* bias) {
+    const int lane = threadIdx.x & 31;
+    for (;;) {
+        int t = 0;
+        if (lane == 0) t = atomicAdd(&r.next, 1);
+        t = __shfl_sync(0xffffffffu, t, 0);
+        if (t >= a.T) break;
+        float* row = rows + t * a.E;
+        route_load(a, r, row, t, lane);
         __syncwarp();
-        if (blockIdx.x == 0) {   // for kernel 2
-            for (int i = lane; i < n; i += 32) a.list[1 + i] = r.act[i];
-            if (lane == 0) a.list[0] = n;
-        }
+        if (a.bias) route_keys(a, r, row, bias, t, lane, 32);
+        __syncwarp();
+        route_pick(a, r, row, t, lane);
     }
-    fence_proxy_async();   // the scratch becomes the target of TMA copies
+}
+// The chosen experts, ascending, to r.act and (block 0) to kernel 2.  One warp, after all choices.
+__device__ __forceinline__ void route_list(const MoeArgs& a, Route& r, int lane) {
+    constexpr int kPer = kMaxE / 32;
+    uint32_t on[kPer];
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) on[j] = __ballot_sync(0xffffffffu, r.mask[lane + 32 * j] != 0u);
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+        if (on[j] >> lane & 1) r.act[n + __popc(on[j] & ((1u << lane) - 1u))] = (uint16_t)(lane + 32 * j);
+        n += __popc(on[j]);
+    }
+    if (lane == 0) r.n_act = n;
+    __syncwarp();
+    if (blockIdx.x == 0) {
+        for (int i = lane; i < n; i += 32) a.list[1 + i] = r.act[i];
+        if (lane == 0) a.list[0] = n;
+    }
 }
 
 // kind::mxf8f6f4: A e2m1 (5), B e4m3 (0), ue8m0 scales, M = 128
@@ -300,8 +333,18 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         __syncwarp();
         tc::tmem_alloc(tmem_slot, C::kTmem);
     }
+    // scratch of the routing, where the first weights will land: the bias, then a row per token
+    float* bias = reinterpret_cast<float*>(base_g + st_off);
+    float* rows = bias + a.E;
+    for (int e = threadIdx.x; e < kMaxE; e += kUpThreads) {
+        R.mask[e] = 0u;
+        if (e < a.E && a.bias) bias[e] = __ldg(a.bias + e);
+    }
+    if (threadIdx.x == 0) R.next = 0;
+    __syncthreads();
+    const bool few = a.T < kRouteThreads / 32;
     if (threadIdx.x < kRouteThreads) {
-        route_all(a, R, reinterpret_cast<float*>(base_g + st_off));
+        if (few) route_together(a, R, rows, bias);
     } else {
         // ---- this CTA's K range of x, quantised, in operand form ----
         const TX* x = reinterpret_cast<const TX*>(a.x);
@@ -365,8 +408,11 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                 }
             }
         }
-        fence_proxy_async();
     }
+    if (!few) route_in_turn(a, R, rows, bias);   // (warps that quantised x join when they are through)
+    fence_proxy_async();                         // x blocks, and the scratch that becomes the target of TMA copies
+    __syncthreads();
+    if (warp == 0) route_list(a, R, lane);
     __syncwarp();
     tc::tc_fence_before();
     if (S > 1) cluster_sync_all(); else __syncthreads();
