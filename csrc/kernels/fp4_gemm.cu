@@ -733,7 +733,7 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
     if (a.x) return kNotTaken;
     a.P = M; a.Q = N; a.sfp = xs; a.sfq = ws;
     a.tiles_p = (int)((M + 127) / 128);
-    // Tile width and K split by the clocks of the longest-running CTA: a stage (256 columns of K) takes about 850 on 256
+    // Tile and K split by the clocks of the longest-running CTA: a stage (256 columns of K) takes about 850 on 256
     // output columns and 560 on 128 (the operands' way from L2), 600 in a pair, a tile about 1500 at its ends that the next one does
     // not hide, an exchange between split CTAs 3000.  Clusters of a split stay resident (33 of 4, 15 of 8).
     const int resident[4] = {sms, 74, 33, 15};
@@ -793,7 +793,8 @@ FB_API int fb_fp4_matmul(const void* xc, const void* xs, const void* wc, const v
 
 // The same with the rows of x [M, K] (element type xdt, row stride ldx; nvfp4: tensor scale xts or 0) quantised first: inside the
 // product for few values, else by fb_fp4_quantize into `work`: codes [M][64 ceil(K / 128)], then (at the next multiple of
-// 512) the scale chunks; the product's prologue and its first weight tiles overlap that launch.
+// 512) the scale chunks; the product's prologue and its first weight tiles overlap that launch.  (One row of up to 2048
+// columns never needs `work`.)
 FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, const void* wc, const void* ws, void* out,
                          int64_t dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t fmt, float xts, float alpha,
                          cudaStream_t st) {
@@ -806,6 +807,7 @@ FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, co
     a.xinv = a.scaled ? (float)(1.0 / (double)xts) : 1.f;
     int rc = fp4_matmul(nullptr, nullptr, wc, ws, M, N, fmt, a, st);
     if (rc != kNotTaken) return rc;
+    if (!work) return (int)cudaErrorInvalidValue;
     uint8_t* codes = (uint8_t*)work;
     uint8_t* scales = codes + (M * 64 * groups(K) + 511) / 512 * 512;
     rc = fb_fp4_quantize(x, xdt, ldx, 0, codes, scales, 1, M, K, fmt, xts, st);

@@ -9,7 +9,7 @@
 // registers: tcgen05.mma kind::mxf8f6f4.block_scale multiplies e2m1 weights with e4m3 activations and applies both
 // scale vectors; the padded 4-bit form that it wants in shared memory (16 codes in 8 bytes, 8 bytes of gap) is what a TMA
 // box of the 4-bit element type writes, so weight bytes go from HBM to the tensor core without passing a register.
-// The weights are the operand on the 128 lanes, ALL tokens (padded to 16 or 32) are the columns, for every expert that any
+// The weights are the operand on the 128 lanes, ALL tokens (padded to 8, 16 or 32) are the columns, for every expert that any
 // token chose: columns of tokens that did not choose the expert cost no bytes, and are dropped (gate | up) or zero (down).
 //
 // Kernel 1 (gate_up): persistent clusters of S CTAs.  Every CTA routes all tokens by itself (a warp per token; the logits
@@ -699,13 +699,12 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
         if (go) {
             // the stages are drained: the partial tile [BN][128] goes into them (a rank without blocks has none: zeros)
 #pragma unroll
-            for (int c = 0; c < BN; c += 16) {
-                uint32_t r[16];
-                tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
-                tmem_ld_wait();
+            for (int c = 0; c < BN; c += 8) {
+                float r[8];
+                tc::tmem_ld8(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(base + (uint32_t)((c + i) * 128 + q * 32 + lane) * 4), "r"(u1 > u0 ? r[i] : 0u) : "memory");
+                for (int i = 0; i < 8; ++i)
+                    asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + (uint32_t)((c + i) * 128 + q * 32 + lane) * 4), "f"(u1 > u0 ? r[i] : 0.f) : "memory");
             }
         }
         tc::tc_fence_before();
@@ -861,7 +860,7 @@ int moe_bn(const MoeArgs& a, const void* w13, const void* w2, cudaStream_t st) {
 // [E, 2, I, D] mxfp4 (gate, up), w2 / s2 of [E, D, I]; out [T, D] (dtype odt, row stride ldo; accumulate: added to);
 // score 0 sqrt(softplus), 1 sigmoid, 2 softmax; norm: the chosen scores are divided by their sum; limit: SwiGLU clamp
 // (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: 4096 + min(E, T topk) ceil(I / 128) (128 BN
-// + 512) bytes, BN = 16 up to 16 tokens, else 32.
+// + 512) bytes, BN = 8 up to 8 tokens, 16 up to 16, else 32.
 FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logits, int64_t ldl, const float* bias, const void* w13,
                       const void* s13, const void* w2, const void* s2, void* out, int64_t odt, int64_t ldo, int64_t accumulate,
                       void* work, int64_t T, int64_t E, int64_t topk, int64_t D, int64_t I, int64_t score, int64_t norm, float scale,
@@ -879,9 +878,10 @@ FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logi
     a.g1 = (int)groups(D); a.nit = (int)((I + 127) / 128);
     a.status = fp4_status_ptr();
     if (!a.status) return (int)cudaErrorNotSupported;
-    const int64_t bn = T <= 16 ? 16 : 32, pairs = T * topk < E ? T * topk : E;
+    // columns of the MMAs: the cost of an MMA does not depend on them, the room that x and h take in shared memory does
+    const int64_t pairs = T * topk < E ? T * topk : E;
     a.list = (int*)work;                         // list, scale chunks, operand tiles: all 16-byte aligned
     a.hs = (uint8_t*)work + 4096;
     a.h = a.hs + pairs * a.nit * 512;
-    return bn == 16 ? moe_bn<16>(a, w13, w2, st) : moe_bn<32>(a, w13, w2, st);
+    return T <= 8 ? moe_bn<8>(a, w13, w2, st) : T <= 16 ? moe_bn<16>(a, w13, w2, st) : moe_bn<32>(a, w13, w2, st);
 }

@@ -193,6 +193,15 @@ def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.d
     return out, _matrix(out, "out") if out.numel() else (0, 0, 0, 0, 0)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory between the first and last elements of two tensors meets."""
+    if not a.numel() or not b.numel():
+        return False
+    span = lambda t: (t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size())
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values of ``q``, rounded once to ``dtype`` (or into ``out``, whose rows may be strided)."""
     if not q.codes.is_cuda:
@@ -206,7 +215,7 @@ def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[
 
 def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ w.T`` of two 4-bit matrices [M, K] and [N, K] of one format: products of the values they stand for, summed in
-    f32 and rounded once."""
+    f32 and rounded once (to ``out_dtype``, or to the type of a given ``out``)."""
     if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"matmul takes [M, K] and [N, K], got {x.shape} and {w.shape}")
     if x.fmt != w.fmt:
@@ -224,8 +233,9 @@ def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, 
 
 def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
            x_scale: Optional[float] = None) -> torch.Tensor:
-    """``quantize(x, w.fmt, x_scale) @ w.T`` for ``x`` [M, K] (f32, bf16, f16) and 4-bit weights [N, K], in one call.
-    ``out_dtype`` defaults to x's."""
+    """``quantize(x, w.fmt, x_scale) @ w.T`` for ``x`` [M, K] (f32, bf16, f16) and 4-bit weights [N, K], in one call
+    (a few short rows in one launch, else two).  ``out_dtype`` defaults to x's; a given ``out`` keeps its own type and must
+    not share memory with x."""
     if x.dim() != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"linear takes [M, K] and 4-bit [N, K], got {tuple(x.shape)} and {w.shape}")
     if x_scale is not None:
@@ -241,6 +251,8 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
             raise TypeError(f"out is float32, bfloat16 or float16, got {out.dtype}")
     else:
         out, (_, _, _, _, ldo) = _out(out, (M, N), out.dtype, dev)
+        if _overlap(out, x):
+            raise ValueError("out and x share memory")
     if M and N:
         g = (K + 127) // 128
         work = None
@@ -302,7 +314,7 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     _, _, _, _, ldx = _matrix(x, "x")
     out, (_, _, _, _, ldo) = _out(out, (T, D), out_dtype or x.dtype, dev)
     if T:
-        tile = 128 * (16 if T <= 16 else 32) + 512
+        tile = 128 * (8 if T <= 8 else 16 if T <= 16 else 32) + 512
         work = torch.empty(4096 + min(E, T * topk) * ((I + 127) // 128) * tile, dtype=torch.uint8, device=dev)
         _call(dev, "fb_fp4_moe", x, _DTYPES[x.dtype], ldx, logits, logits.stride(0) if T > 1 else E, bias, w13.codes, w13.scales,
               w2.codes, w2.scales, out, _DTYPES[out.dtype], ldo, int(accumulate), work, T, E, topk, D, I, SCORES[score], int(norm),

@@ -130,3 +130,12 @@ def test_moe_limits():
         fp4.moe(*_moe_args(E=513, I=32, D=32))
     with pytest.raises(ValueError, match="up to 8192"):
         fp4.moe(*_moe_args(E=2, I=32, D=8193))
+
+
+def test_overlap_of_out_and_x(monkeypatch):
+    b = torch.zeros(4, 256)
+    assert fp4._overlap(b, b[2:]) and fp4._overlap(b[:, :200], b[:, 100:]) and not fp4._overlap(b[:2], b[2:])
+    assert not fp4._overlap(b[:0], b) and not fp4._overlap(b, torch.zeros(4))
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    with pytest.raises(ValueError, match="share memory"):
+        fp4.linear(b[:1, :64], _t(64, 64), out=b[:1, :64])

@@ -98,6 +98,12 @@ CASES = [  # T, E, topk, D, I, score, norm, bias, dtype
     (2, 512, 6, 256, 32, "sigmoid", True, True, torch.float32),
     (4, 6, 2, 5120, 288, "sqrtsoftplus", True, True, torch.bfloat16),
     (20, 4, 2, 7168, 128, "sigmoid", True, False, torch.bfloat16),
+    (2, 6, 2, 5120, 64, "sigmoid", False, True, torch.float32),        # few tiles: clusters of eight
+    (24, 16, 2, 2048, 512, "softmax", True, True, torch.bfloat16),     # clusters of two
+    (12, 9, 3, 3200, 96, "sqrtsoftplus", True, True, torch.float16),   # an odd number of 128-column blocks
+    (32, 96, 6, 1024, 256, "sqrtsoftplus", True, False, torch.bfloat16),
+    (8, 24, 6, 8192, 32, "sigmoid", True, True, torch.bfloat16),       # the widest rows
+    (32, 5, 2, 8192, 64, "softmax", True, True, torch.float32),
 ]
 
 
