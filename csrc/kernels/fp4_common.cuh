@@ -18,9 +18,10 @@ enum Fp4Dtype : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 // Device words that the bounded waits of these kernels report to (the current device's copy); null if CUDA refuses.
 int* fp4_status_ptr();
 
-// Launch with an optional cluster of `cluster` CTAs along x and, with `pdl`, programmatic serialisation against the
-// kernel before it in the stream (always one of this file family that was launched plainly: when it runs, everything
-// before it is complete, so its successor may read what IT does not write before the wait).
+// Launch with an optional cluster of `cluster` CTAs along x and, with `pdl`, programmatic serialisation against the kernel
+// before it in the stream.  A kernel launched so reads nothing before its griddepcontrol.wait but what no kernel of the
+// stream writes while it may be in flight: the product after the quantiser, which is launched plainly (when that runs,
+// everything before it is complete), reads the weights.
 template <typename... KArgs, typename... Args>
 inline cudaError_t fp4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, bool pdl,
                               Args&&... args) {
@@ -282,14 +283,25 @@ __device__ __forceinline__ void unpack8(const uint4& a, float (&v)[8]) {
         }
     }
 }
+// (volatile: a kernel that is launched early must not have these moved above its wait)
+__device__ __forceinline__ uint4 ld_nc_v4(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+__device__ __forceinline__ float ld_f32(const float* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+    return v;
+}
 // p[0 .. 7] -> f32, all of them there; p is aligned to the eight values (16 bytes, f32 32).
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
     if constexpr (sizeof(T) == 4) {
-        asm("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+        asm volatile("ld.global.nc.L1::no_allocate.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
             : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p));
     } else {
-        unpack8<T>(ldg_nc_v4(p), v);
+        unpack8<T>(ld_nc_v4(p), v);
     }
 }
 // The first n of them (the others read 0); vec: p is aligned as above.
@@ -305,7 +317,7 @@ __device__ __forceinline__ void load8(const T* p, int n, bool vec, float (&v)[8]
 // Eight values as they are in memory.
 template <typename T> struct Raw8 {
     uint4 w;
-    __device__ __forceinline__ void load(const T* p) { w = ldg_nc_v4(p); }
+    __device__ __forceinline__ void load(const T* p) { w = ld_nc_v4(p); }
     __device__ __forceinline__ void unpack(float (&v)[8]) const { unpack8<T>(w, v); }
     __device__ __forceinline__ uint32_t max_bits() const { return max_bits8_packed<T>(w); }
 };
