@@ -36,10 +36,12 @@ struct GemmCfg {
     static constexpr int kStageBytes = (kABytes + kSfa + (QX ? 0 : kXBlock) + 1023) / 1024 * 1024;
     // P = X: each epilogue warp stages its rows of the output in two buffers of 32 rows x 128 bytes
     static constexpr int kStaging = SWAP ? 0 : (kEpi / 32) * 2 * 4096;
-    static constexpr int kBudget = BN <= 32 ? 112 * 1024 : 227 * 1024;  // up to 32 columns: two CTAs per SM
+    static constexpr int kBudget = 227 * 1024;   // one CTA per SM: two would take turns on the tensor core, at a change of accumulator
+                                                 // (140 clocks) per stage: 5.2 TB/s of weights against KRATE
     static constexpr int kBars = 512;
     static constexpr int kXRoom = QX ? kQxBlocks * kXBlock : 0;
-    static constexpr int kStages = (kBudget - kBars - kStaging - kXRoom) / kStageBytes;
+    static constexpr int kFit = (kBudget - kBars - kStaging - kXRoom) / kStageBytes;
+    static constexpr int kStages = kFit < 12 ? kFit : 12;
     static constexpr int kSfCols = 4 * kChunks * (1 + kQAtoms);        // tensor memory columns of a stage's scales
     static constexpr int kAcc = BN < 32 ? 32 : BN;
     static constexpr int kNeed = kAcc + 2 * kSfCols;
@@ -227,7 +229,7 @@ __device__ __forceinline__ void quantize_x(const GemmArgs& a, uint8_t* room, int
 }
 
 template <int FMT, int BN, bool SWAP, bool QX>
-__global__ void __launch_bounds__(kGThreads, BN <= 32 ? 2 : 1)
+__global__ void __launch_bounds__(kGThreads, 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                 const __grid_constant__ CUtensorMap tmap_o, const GemmArgs a) {
     using C = GemmCfg<FMT, BN, SWAP, QX>;
@@ -248,6 +250,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
     const int64_t Cch = FMT == kMxFp4 ? G : 2 * G;
     const int nkb_all = (int)((G + 1) / 2);
     const int kb0 = (int)((int64_t)nkb_all * rank / S), kb1 = (int)((int64_t)nkb_all * (rank + 1) / S);
+    // the last stage of K: 64-column MMA steps that hold columns, bytes of scale chunks per 128 rows
+    constexpr uint32_t kFull = 512 * C::kChunks;
+    const int tail_steps = (int)((a.K - (int64_t)(nkb_all - 1) * kBK + 63) / 64);
+    const uint32_t tail_sf = 512 * (uint32_t)(Cch - (int64_t)(nkb_all - 1) * C::kChunks);
     const int n_tiles = a.tiles_p * a.tiles_q;
     const int first = S > 1 ? blockIdx.x / S : blockIdx.x, step = S > 1 ? n_tiles : gridDim.x;
     // tiles in bands of kBand along P, so that the CTAs in flight share operand tiles through L2
@@ -283,83 +289,97 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 
     if (warp == 0) {
         if (elect_one()) {
-            const int qatoms = C::kQAtoms;
-            const int64_t q_rowtiles = (a.Q + 127) / 128;
-            auto issue_p = [&](int s, int kb, int64_t p0, int nch) {
-                tc::tma_load_2d(base + s * C::kStageBytes + a_off, &tmap_p, kb * 128, (int)p0, full(s));
-                bulk_load(base + s * C::kStageBytes + sfa_off, a.sfp + ((p0 / 128) * Cch + (int64_t)kb * C::kChunks) * 512, 512 * nch, full(s));
+            // One thread's dependent instructions are what a stage costs here: addresses are advanced, not computed, and only the
+            // last stage of K looks at how much of it there is.
+            const int q_rowtiles = (int)((a.Q + 127) / 128);
+            const uint32_t pbytes = C::kABytes + kFull, qbytes = QX ? 0u : C::kBBytes;
+            auto load_p = [&](int s, int kb, int p0, const uint8_t* f, uint32_t sf) {
+                tc::tma_load_2d(base + s * C::kStageBytes + a_off, &tmap_p, kb * 128, p0, full(s));
+                bulk_load(base + s * C::kStageBytes + sfa_off, f, sf, full(s));
             };
-            auto issue_q = [&](int s, int kb, int64_t q0, int nch) {
+            auto load_q = [&](int s, int kb, int q0, const uint8_t* f, uint32_t sf, int at) {
                 if (QX) return;
-                tc::tma_load_2d(base + s * C::kStageBytes + b_off, &tmap_q, kb * 128, (int)q0, full(s));
-                for (int at = 0; at < qatoms; ++at)
-                    if (q0 / 128 + at < q_rowtiles)
-                        bulk_load(base + s * C::kStageBytes + sfb_off + at * C::kSfa,
-                                  a.sfq + ((q0 / 128 + at) * Cch + (int64_t)kb * C::kChunks) * 512, 512 * nch, full(s));
+                tc::tma_load_2d(base + s * C::kStageBytes + b_off, &tmap_q, kb * 128, q0, full(s));
+                bulk_load(base + s * C::kStageBytes + sfb_off, f, sf, full(s));
+                if (C::kQAtoms > 1 && at > 1) bulk_load(base + s * C::kStageBytes + sfb_off + C::kSfa, f + Cch * 512, sf, full(s));
             };
-            auto arm = [&](int s, int64_t q0, int nch) {
-                const int at = (int)min((int64_t)qatoms, q_rowtiles - q0 / 128);
-                tc::mbar_expect_tx(full(s), QX ? C::kABytes + 512 * nch : C::kABytes + C::kBBytes + 512 * nch * (1 + at));
-            };
-            auto chunks = [&](int kb) { return (int)min((int64_t)C::kChunks, Cch - (int64_t)kb * C::kChunks); };
-            int it = 0;
+            int s = 0, round = 0;
             bool ok = true;
             for (int t = first; t < n_tiles && ok; t += step) {
                 int64_t p0, q0;
                 tile_at(t, p0, q0);
+                const int at = min(C::kQAtoms, q_rowtiles - (int)(q0 / 128));
+                const uint8_t* fp = a.sfp + ((p0 / 128) * Cch + (int64_t)kb0 * C::kChunks) * 512;
+                const uint8_t* fq = QX ? nullptr : a.sfq + ((q0 / 128) * Cch + (int64_t)kb0 * C::kChunks) * 512;
+                const uint32_t qat = QX ? 0u : (uint32_t)at;
                 int kb = kb0;
                 if (t == first && a.pdl) {
                     // X is written by the kernel before this one: only W (P when swapped) may be read before the wait
                     const int ahead = SWAP ? min(C::kStages, kb1 - kb0) : 0;
                     for (int i = 0; i < ahead; ++i) {
-                        arm(i, q0, chunks(kb0 + i));
-                        issue_p(i, kb0 + i, p0, chunks(kb0 + i));
+                        const uint32_t sf = kb0 + i == nkb_all - 1 ? tail_sf : kFull;
+                        tc::mbar_expect_tx(full(i), C::kABytes + qbytes + sf * (1 + qat));
+                        load_p(i, kb0 + i, (int)p0, fp + i * kFull, sf);
                     }
                     pdl_wait();
-                    for (int i = 0; i < ahead; ++i) issue_q(i, kb0 + i, q0, chunks(kb0 + i));
+                    for (int i = 0; i < ahead; ++i) load_q(i, kb0 + i, (int)q0, fq + i * kFull, kb0 + i == nkb_all - 1 ? tail_sf : kFull, at);
                     kb += ahead;
-                    it += ahead;
+                    fp += ahead * kFull;
+                    fq += ahead * kFull;
+                    s = ahead;
+                    if (s == C::kStages) { s = 0; round = 1; }
                 }
-                for (; kb < kb1; ++kb, ++it) {
-                    const int s = it % C::kStages;
-                    if (it >= C::kStages && !tc::mbar_wait(empty(s), ((it / C::kStages) - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
-                    arm(s, q0, chunks(kb));
-                    issue_p(s, kb, p0, chunks(kb));
-                    issue_q(s, kb, q0, chunks(kb));
+                for (; kb < kb1; ++kb, fp += kFull, fq += kFull) {
+                    if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                    const uint32_t sf = kb == nkb_all - 1 ? tail_sf : kFull;
+                    tc::mbar_expect_tx(full(s), kb == nkb_all - 1 ? C::kABytes + qbytes + sf * (1 + qat) : pbytes + qbytes + kFull * qat);
+                    load_p(s, kb, (int)p0, fp, sf);
+                    load_q(s, kb, (int)q0, fq, sf, at);
+                    if (++s == C::kStages) { s = 0; ++round; }
                 }
             }
         }
     } else if (warp == 1) {
         if (elect_one()) {
-            int it = 0, tile_no = 0;
+            int s = 0, par = 0, flip = 0, tile_no = 0;
             bool ok = true;
             if (QX && !tc::mbar_wait(x_full, 0)) { atomicExch(&s_fail, 1); ok = false; }
             for (int t = first; t < n_tiles && ok; t += step, ++tile_no) {
                 if (tile_no && !tc::mbar_wait(acc_empty, (tile_no - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
                 tc::tc_fence_after();
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int s = it % C::kStages;
-                    if (!tc::mbar_wait(full(s), (it / C::kStages) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
+                uint32_t xb = xroom;   // QX: this stage's block of X
+                for (int kb = kb0; kb < kb1; ++kb) {
+                    if (!tc::mbar_wait(full(s), par)) { atomicExch(&s_fail, 1); ok = false; break; }
                     tc::tc_fence_after();
                     const uint32_t st = base + s * C::kStageBytes;
-                    const uint32_t sfa_t = tmem + C::kAcc + (uint32_t)(it & 1) * C::kSfCols, sfb_t = sfa_t + 4 * C::kChunks;
-                    const int steps = (int)min((int64_t)4, (a.K - (int64_t)kb * kBK + 63) / 64);
-                    const int nch = FMT == kMxFp4 ? (steps + 1) / 2 : steps;
-                    for (int c = 0; c < nch; ++c) {
-                        tmem_cp_sf(sfa_t + 4 * c, sf_desc(st + sfa_off + 512 * c));
+                    const uint32_t sfa_t = tmem + C::kAcc + (uint32_t)flip, sfb_t = sfa_t + 4 * C::kChunks;
+                    flip ^= C::kSfCols;
+                    const uint32_t sfa_s = st + sfa_off, sfb_s = QX ? xb + C::kBBytes : st + sfb_off;
+                    const uint64_t ad = tc::umma_desc_sw128(st + a_off), bd = tc::umma_desc_sw128(QX ? xb : st + b_off);
+                    auto scales = [&](int c) {   // word c of all atoms side by side: 4 columns per 128 rows
+                        tmem_cp_sf(sfa_t + 4 * c, sf_desc(sfa_s + 512 * c));
 #pragma unroll
-                        for (int at = 0; at < C::kQAtoms; ++at)   // word c of all atoms side by side: 4 columns per 128 rows
-                            tmem_cp_sf(sfb_t + 4 * (c * C::kQAtoms + at), sf_desc((QX ? xroom + (kb - kb0) * C::kXBlock + C::kBBytes : st + sfb_off) + at * C::kSfa + 512 * c));
-                    }
-                    const uint64_t ad = tc::umma_desc_sw128(st + a_off), bd = tc::umma_desc_sw128(QX ? xroom + (kb - kb0) * C::kXBlock : st + b_off);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if (k >= steps) break;
+                        for (int at = 0; at < C::kQAtoms; ++at) tmem_cp_sf(sfb_t + 4 * (c * C::kQAtoms + at), sf_desc(sfb_s + at * C::kSfa + 512 * c));
+                    };
+                    auto mma = [&](int k) {
                         const int c = FMT == kMxFp4 ? k / 2 : k;
-                        umma_fp4<FMT>(tmem, ad + 2u * k, bd + 2u * k, fp4_idesc<FMT>(BN, FMT == kMxFp4 ? 2 * (k & 1) : 0),
-                                      sfa_t + 4 * c, sfb_t + 4 * c * C::kQAtoms, (kb > kb0 || k) ? 1u : 0u);
+                        umma_fp4<FMT>(tmem, ad + 2u * k, bd + 2u * k, fp4_idesc<FMT>(BN, FMT == kMxFp4 ? 2 * (k & 1) : 0), sfa_t + 4 * c,
+                                      sfb_t + 4 * c * C::kQAtoms, (kb > kb0 || k) ? 1u : 0u);
+                    };
+                    if (kb < nkb_all - 1 || tail_steps == 4) {
+#pragma unroll
+                        for (int c = 0; c < C::kChunks; ++c) scales(c);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma(k);
+                    } else {
+                        for (int c = 0; c < (FMT == kMxFp4 ? (tail_steps + 1) / 2 : tail_steps); ++c) scales(c);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k)
+                            if (k < tail_steps) mma(k);
                     }
                     tc::umma_commit(empty(s));
+                    if (++s == C::kStages) { s = 0; par ^= 1; }
+                    xb += C::kXBlock;
                 }
                 tc::umma_commit(acc_full);
             }
@@ -509,6 +529,7 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
     const int rank = (int)cluster_rank();
     const int64_t G = groups(a.K), Cch = FMT == kMxFp4 ? G : 2 * G;
     const int nkb = (int)((G + 1) / 2);
+    const int tail_steps = (int)((a.K - (int64_t)(nkb - 1) * kBK + 63) / 64), tail_chunks = FMT == kMxFp4 ? (tail_steps + 1) / 2 : tail_steps;
     const int n_tiles = a.tiles_p * a.tiles_q, first = blockIdx.x >> 1, step = gridDim.x >> 1;
     constexpr int kBand = 4;   // bands of tiles along P, so that the pairs in flight share operand tiles through L2
     auto tile_at = [&](int t, int64_t& p0, int64_t& q0) {
@@ -553,16 +574,19 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
                 tile_at(t, p0, q0);
                 // rows of 512 bytes in the scale maps: chunks; what lies behind a matrix's or a row's end reads something finite
                 // or zero and meets no stored output
-                const int64_t sp = (p0 / 128 + rank) * Cch, sq = q0 / 128 * Cch;
+                int sp = (int)((p0 / 128 + rank) * Cch), sq = (int)(q0 / 128 * Cch), sq1 = sq + (int)Cch;
                 for (int kb = 0; kb < nkb; ++kb) {
                     if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
                     const uint32_t st = base + s * C::kStageBytes, bar = lead + 8u * s;
                     if (rank == 0) tc::mbar_expect_tx(full(s), 2 * C::kStageBytes);
                     tma_load_pair(st, &tmap_p, kb * 128, (int)p0 + 128 * rank, bar);
                     tma_load_pair(st + b_off, &tmap_q, kb * 128, (int)q0 + 128 * rank, bar);
-                    tma_load_pair(st + sfa_off, &tmap_sp, 0, (int)sp + kb * C::kChunks, bar);
-                    tma_load_pair(st + sfb_off, &tmap_sq, 0, (int)sq + kb * C::kChunks, bar);
-                    tma_load_pair(st + sfb_off + C::kSfa, &tmap_sq, 0, (int)(sq + Cch) + kb * C::kChunks, bar);
+                    tma_load_pair(st + sfa_off, &tmap_sp, 0, sp, bar);
+                    tma_load_pair(st + sfb_off, &tmap_sq, 0, sq, bar);
+                    tma_load_pair(st + sfb_off + C::kSfa, &tmap_sq, 0, sq1, bar);
+                    sp += C::kChunks;
+                    sq += C::kChunks;
+                    sq1 += C::kChunks;
                     if (++s == C::kStages) { s = 0; ++round; }
                 }
             }
@@ -581,8 +605,7 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
                         tc::tc_fence_after();
                         const uint32_t st = base + s * C::kStageBytes;
                         const uint32_t sfa_t = tmem + C::kAcc + (uint32_t)(it & 1) * C::kSfCols, sfb_t = sfa_t + 4 * C::kChunks;
-                        const int steps = (int)min((int64_t)4, (a.K - (int64_t)kb * kBK + 63) / 64);
-                        const int nch = FMT == kMxFp4 ? (steps + 1) / 2 : steps;
+                        const int steps = kb == nkb - 1 ? tail_steps : 4, nch = kb == nkb - 1 ? tail_chunks : C::kChunks;
                         auto scales = [&](int c) {
                             if (c >= nch) return;
                             cp_sf_pair(sfa_t + 4 * c, sf_desc(st + sfa_off + 512 * c));
@@ -677,6 +700,8 @@ int launch_gemm(const GemmArgs& a, const void* pc, const void* qc, int grid, cud
     return (int)fp4_launch(k, dim3((unsigned)grid), dim3(kGThreads), C::kSmem, st, a.splits, a.pdl != 0, tp, tq, to, a);
 }
 
+// Clusters of 1 .. 8 CTAs that fit the device at one CTA per SM (measured: a cluster stays inside a GPC).
+constexpr int kResident[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
 constexpr int kNotTaken = -1;     // X is not quantised inside the product at these sizes
 constexpr int kQxRows = 16;       // rows times blocks of 256 columns per CTA up to which it is
 
@@ -707,16 +732,23 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
     if (M <= 128) {
         // weights on the lanes; as many K splits as fill the SMs, with at least two stages each
         const int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-        const int slots = bn <= 32 ? 2 * sms : sms;
         a.P = N; a.Q = M; a.sfp = ws; a.sfq = xs;
         a.tiles_p = (int)((N + 127) / 128);
         a.tiles_q = 1;
-        const int resident[4] = {slots, slots / 2, bn <= 32 ? 71 : 33, bn <= 32 ? 33 : 15};   // clusters of 1, 2, 4, 8
+        // K split by the clocks of the longest-running CTA, as below: a stage takes its MMAs and scale copies or, with many
+        // CTAs, its share of HBM (17.4 KB of weights at 3450 bytes per clock)
+        const double mma = bn <= 32 ? 350 : bn == 64 ? 400 : 470;
+        double cost = 0;
         int S = 1;
-        for (int l = 1; l < 4; ++l)
-            if (a.tiles_p <= resident[l] && nkb >= 2 << l) S = 1 << l;
+        for (int c = 1; c <= 8; ++c) {
+            if (c > 1 && (a.tiles_p > kResident[c] || nkb < 2 * c)) continue;
+            const int64_t active = (int64_t)(a.tiles_p < kResident[c] ? a.tiles_p : kResident[c]) * c;
+            const double stage = active * 5.05 > mma ? active * 5.05 : mma;
+            const double t = (double)((a.tiles_p + kResident[c] - 1) / kResident[c]) * (((nkb + c - 1) / c) * stage + 1500) + (c > 1 ? 3000 : 0);
+            if (cost == 0 || t < cost) { cost = t; S = c; }
+        }
         a.splits = S;
-        const int grid = S > 1 ? a.tiles_p * S : (a.tiles_p < slots ? a.tiles_p : slots);
+        const int grid = S > 1 ? a.tiles_p * S : (a.tiles_p < sms ? a.tiles_p : sms);
         if (a.x) {
             // Rows that are quantised on the way: with few values per CTA its idle epilogue warps do it while the first weights
             // arrive, and the quantiser's own launch goes.
@@ -735,8 +767,7 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
     a.tiles_p = (int)((M + 127) / 128);
     // Tile and K split by the clocks of the longest-running CTA: a stage (256 columns of K) takes about 850 on 256
     // output columns and 560 on 128 (the operands' way from L2), 600 in a pair, a tile about 1500 at its ends that the next one does
-    // not hide, an exchange between split CTAs 3000.  Clusters of a split stay resident (33 of 4, 15 of 8).
-    const int resident[4] = {sms, 74, 33, 15};
+    // not hide, an exchange between split CTAs 3000.  Clusters of a split stay resident.
     double cost = 0;
     bool wide = true;
     int S = 1;
@@ -744,7 +775,7 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
         const int64_t tiles = (int64_t)a.tiles_p * ((N + (w ? 255 : 127)) / (w ? 256 : 128));
         for (int l = 0; l < 4; ++l) {
             const int s = 1 << l;
-            if (l && (tiles > resident[l] || nkb < 2 * s)) break;
+            if (l && (tiles > kResident[s] || nkb < 2 * s)) break;
             const double c = (double)((tiles + sms - 1) / sms) * ((double)((nkb + s - 1) / s) * (w ? 850 : 560) + 1500) + (s > 1 ? 3000 : 0);
             if (cost == 0 || c < cost) { cost = c; wide = w; S = s; }
         }
