@@ -24,7 +24,7 @@ using namespace fp4;
 constexpr int kBK = 256;          // values per stage row (128 bytes)
 constexpr int kGThreads = 320;
 constexpr int kEpi = 256;         // epilogue threads: two warps per lane quarter
-constexpr int kQxBlocks = 8;      // QX: blocks of X that a CTA holds
+constexpr int kQxBlocks = 16;     // QX: blocks of X that a CTA holds
 
 template <int FMT, int BN, bool SWAP, bool QX>
 struct GemmCfg {
@@ -36,8 +36,8 @@ struct GemmCfg {
     static constexpr int kStageBytes = (kABytes + kSfa + (QX ? 0 : kXBlock) + 1023) / 1024 * 1024;
     // P = X: each epilogue warp stages its rows of the output in two buffers of 32 rows x 128 bytes
     static constexpr int kStaging = SWAP ? 0 : (kEpi / 32) * 2 * 4096;
-    static constexpr int kBudget = 227 * 1024;   // one CTA per SM: two would take turns on the tensor core, at a change of accumulator
-                                                 // (140 clocks) per stage: 5.2 TB/s of weights against KRATE
+    static constexpr int kBudget = BN <= 32 && !QX ? 112 * 1024 : 227 * 1024;  // up to 32 columns: two CTAs per SM (1x129280x5120
+                                                                        // mxfp4 61.2 us, 62.9 with one of twice the stages)
     static constexpr int kBars = 512;
     static constexpr int kXRoom = QX ? kQxBlocks * kXBlock : 0;
     static constexpr int kFit = (kBudget - kBars - kStaging - kXRoom) / kStageBytes;
@@ -229,7 +229,7 @@ __device__ __forceinline__ void quantize_x(const GemmArgs& a, uint8_t* room, int
 }
 
 template <int FMT, int BN, bool SWAP, bool QX>
-__global__ void __launch_bounds__(kGThreads, 1)
+__global__ void __launch_bounds__(kGThreads, BN <= 32 && !QX ? 2 : 1)
 fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constant__ CUtensorMap tmap_q,
                 const __grid_constant__ CUtensorMap tmap_o, const GemmArgs a) {
     using C = GemmCfg<FMT, BN, SWAP, QX>;
@@ -473,7 +473,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
 // CTA then fetches 32 KB of codes per 256 columns of K where the single-CTA tile of 128 x 256 fetches 48 KB, and the
 // fabric between L2 and the SMs (about 64 bytes per clock and SM) was what that one waited for.
 // All copies of a stage, both CTAs', complete on rank 0's barrier (TMA with cta_group::2 may signal the pair's other CTA):
-// a first form in which rank 1 passed its completions on took 1370 clocks a stage instead of KSTAGE.
+// a first form in which rank 1 passed its completions on took 1370 clocks a stage instead of about 700.
 template <int FMT>
 struct PairCfg {
     static constexpr int kChunks = FMT == kMxFp4 ? 2 : 4;
@@ -748,7 +748,8 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
             if (cost == 0 || t < cost) { cost = t; S = c; }
         }
         a.splits = S;
-        const int grid = S > 1 ? a.tiles_p * S : (a.tiles_p < sms ? a.tiles_p : sms);
+        const int slots = bn <= 32 && !a.x ? 2 * sms : sms;
+        const int grid = S > 1 ? a.tiles_p * S : (a.tiles_p < slots ? a.tiles_p : slots);
         if (a.x) {
             // Rows that are quantised on the way: with few values per CTA its idle epilogue warps do it while the first weights
             // arrive, and the quantiser's own launch goes.
@@ -824,7 +825,7 @@ FB_API int fb_fp4_matmul(const void* xc, const void* xs, const void* wc, const v
 
 // The same with the rows of x [M, K] (element type xdt, row stride ldx; nvfp4: tensor scale xts or 0) quantised first: inside the
 // product for few values, else by fb_fp4_quantize into `work`: codes [M][64 ceil(K / 128)], then (at the next multiple of
-// 512) the scale chunks; the product's prologue and its first weight tiles overlap that launch.  (One row of up to 2048
+// 512) the scale chunks; the product's prologue and its first weight tiles overlap that launch.  (One row of up to 4096
 // columns never needs `work`.)
 FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, const void* wc, const void* ws, void* out,
                          int64_t dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t fmt, float xts, float alpha,

@@ -29,7 +29,7 @@ from .quant import e2m1_unpack
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-LINEAR_INSIDE = 16   # 128-column groups of one row that fb_fp4_linear always quantises inside the product
+LINEAR_INSIDE = 32   # 128-column groups of one row that fb_fp4_linear always quantises inside the product
 
 
 class Fp4Tensor:
