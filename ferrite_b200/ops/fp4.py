@@ -50,15 +50,14 @@ class Fp4Tensor:
             raise ValueError(f"a 4-bit tensor has a shape [..., rows, cols >= 1], got {shape}")
         if tensor_scale is not None:
             _check_scale(tensor_scale, fmt)
-        g = (shape[-1] + 127) // 128
-        c = g if fmt == "mxfp4" else 2 * g
-        if tuple(codes.shape) != (*shape[:-1], 64 * g) or tuple(scales.shape) != (*shape[:-2], (shape[-2] + 127) // 128, c, 512):
+        g = (shape[-1] + 127) >> 7
+        if codes.shape != (*shape[:-1], 64 * g) or scales.shape != (*shape[:-2], (shape[-2] + 127) >> 7, g if fmt == "mxfp4" else 2 * g, 512):
             raise ValueError(f"codes {tuple(codes.shape)} / scales {tuple(scales.shape)} do not belong to a {fmt} tensor of shape {shape}")
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
             raise TypeError("codes and scales are uint8")
         if codes.device != scales.device:
             raise ValueError("codes and scales are on different devices")
-        if not codes.is_contiguous() or not scales.is_contiguous() or codes.data_ptr() % 32 or scales.data_ptr() % 16:
+        if not (codes.is_contiguous() and scales.is_contiguous()) or codes.data_ptr() & 31 or scales.data_ptr() & 15:
             raise ValueError("codes and scales are contiguous, codes on a 32-byte and scales on a 16-byte boundary")
         self.codes, self.scales, self.fmt, self.shape, self.tensor_scale = codes, scales, fmt, shape, tensor_scale
 
