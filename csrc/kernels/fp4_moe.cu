@@ -310,7 +310,6 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const uint32_t acc_full = bars + 16u * stages, acc_empty = acc_full + 16u, recv_full = acc_empty + 16u, recv_free = recv_full + 32u,
                    tmem_slot = recv_free + 32u;
 
-    pdl_launch();
     if (warp == 9) {
         if (lane == 0) {
             s_fail = 0;
@@ -332,6 +331,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         }
         __syncwarp();
         tc::tmem_alloc(tmem_slot, C::kTmem);
+        pdl_launch();   // not before: a dependent on this SM could take the tensor memory first, and waits for this kernel's end
     }
     // scratch of the routing, where the first weights will land: the bias, then a row per token
     float* bias = reinterpret_cast<float*>(base_g + st_off);
@@ -617,7 +617,6 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = a.S, rank = S > 1 ? (int)cluster_rank() : 0;
     const int tile = blockIdx.x / S, d0 = tile * 128, ntd = (a.D + 127) / 128;
-    pdl_launch();
     if (threadIdx.x == 0) {
         s_fail = 0;
         for (int s = 0; s < C::kStages; ++s) {
@@ -628,7 +627,10 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
         tc::mbar_fence_init();
         tc::prefetch_tmap(&tmap_w);
     }
-    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
+    if (warp == 1) {
+        tc::tmem_alloc(tmem_slot, C::kTmem);
+        pdl_launch();   // as in kernel 1
+    }
     pdl_wait();   // everything below reads what kernel 1 wrote
     if (warp >= 2) {
         const volatile int* list = a.list;   // (a read-only load might move above the wait)
