@@ -81,6 +81,10 @@ class Fp4Tensor:
         [..., rows, cols / block], as ``ops/quant.py::quant_fp4_weight`` returns them.  Copies; done once at load time."""
         if fmt not in FORMATS:
             raise ValueError(f"fmt must be one of {sorted(FORMATS)}, got {fmt!r}")
+        if packed.dim() < 2 or not packed.shape[-1]:
+            raise ValueError(f"packed has a shape [..., rows, cols / 2], got {tuple(packed.shape)}")
+        if packed.device != scale.device:
+            raise ValueError(f"packed is on {packed.device}, scale on {scale.device}")
         rows, cols = packed.shape[-2], 2 * packed.shape[-1]
         if tuple(scale.shape) != (*packed.shape[:-1], cols // BLOCK[fmt]) or cols % BLOCK[fmt]:
             raise ValueError(f"packed {tuple(packed.shape)} and scale {tuple(scale.shape)} do not match for {fmt}")
@@ -117,6 +121,15 @@ def _check_scale(ts: float, fmt: str) -> None:
         raise ValueError("tensor_scale belongs to nvfp4")
     if not (isinstance(ts, (int, float)) and 2.0 ** -100 <= ts <= 2.0 ** 100):
         raise ValueError(f"tensor_scale is a number in [2^-100, 2^100], got {ts!r}")
+
+
+def _alpha(xs: Optional[float], ws: Optional[float]) -> float:
+    """The factor of a product's sums.  (The scales of an ordinary pair multiply to something near one; out of this range the
+    factor itself would overflow f32 or lose bits.)"""
+    alpha = (xs or 1.0) * (ws or 1.0)
+    if not 2.0 ** -100 <= alpha <= 2.0 ** 100:
+        raise ValueError(f"the product of the tensor scales must be in [2^-100, 2^100], got {alpha!r}")
+    return float(alpha)
 
 
 def _call(device: torch.device, name: str, *args) -> None:
@@ -179,8 +192,25 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp4", tensor_scale: Optional[float] 
     return Fp4Tensor._of(codes, scales, fmt, tuple(x.shape), tensor_scale)
 
 
-def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.device):
-    """``out`` or a new tensor of ``shape``, and its :func:`_matrix`."""
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of consecutive last dimensions may share memory: the spans between their first and last elements
+    meet, and they are not columns of one buffer that lie beside each other."""
+    if not a.numel() or not b.numel():
+        return False
+    extent = lambda t: (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    if a0 >= b0 + extent(b) or b0 >= a0 + extent(a):
+        return False
+    if a.dim() == b.dim() == 2 and a.shape[0] > 1 and b.shape[0] > 1:
+        pitch = a.stride(0) * a.element_size()
+        if pitch and pitch == b.stride(0) * b.element_size():
+            d = (b0 - a0) % pitch
+            return d < a.shape[1] * a.element_size() or d + b.shape[1] * b.element_size() > pitch
+    return True
+
+
+def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.device, *operands: torch.Tensor):
+    """``out`` (which must not meet itself or an operand) or a new tensor of ``shape``, and its :func:`_matrix`."""
     if out is None:
         if dtype not in _DTYPES:
             raise TypeError(f"out is float32, bfloat16 or float16, got {dtype}")
@@ -189,23 +219,21 @@ def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.d
         return out, (math.prod(shape[:-2]), rows, cols, rows * cols, cols)
     if tuple(out.shape) != tuple(shape) or out.device != device:
         raise ValueError(f"out must be {tuple(shape)} on {device}, got {tuple(out.shape)} on {out.device}")
-    return out, _matrix(out, "out") if out.numel() else (0, 0, 0, 0, 0)
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory between the first and last elements of two tensors meets."""
-    if not a.numel() or not b.numel():
-        return False
-    span = lambda t: (t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size())
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    if not out.numel():
+        return out, (0, 0, 0, 0, 0)
+    batch, rows, cols, bs, ld = m = _matrix(out, "out")
+    if batch > 1 and bs < (rows - 1) * ld + cols and not (bs >= cols and (batch - 1) * bs + cols <= ld):
+        raise ValueError(f"the matrices of out overlap: strides {out.stride()}")
+    if any(_overlap(out, t) for t in operands):
+        raise ValueError("out and an operand share memory")
+    return out, m
 
 
 def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values of ``q``, rounded once to ``dtype`` (or into ``out``, whose rows may be strided)."""
     if not q.codes.is_cuda:
         raise ValueError("q is not on a CUDA device")
-    out, (batch, rows, cols, bs, ld) = _out(out, q.shape, dtype, q.device)
+    out, (batch, rows, cols, bs, ld) = _out(out, q.shape, dtype, q.device, q.codes, q.scales)
     if batch * rows:
         _call(q.device, "fb_fp4_dequantize", q.codes, q.scales, out, _DTYPES[out.dtype], ld, bs, batch, rows, cols,
               FORMATS[q.fmt], float(q.tensor_scale or 0.0))
@@ -222,9 +250,9 @@ def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, 
     if not x.codes.is_cuda or x.device != w.device:
         raise ValueError(f"matmul takes tensors of one CUDA device, got {x.device} and {w.device}")
     M, N, K = x.shape[0], w.shape[0], x.shape[1]
-    out, (_, _, _, _, ldo) = _out(out, (M, N), out_dtype, x.device)
+    alpha = _alpha(x.tensor_scale, w.tensor_scale)
+    out, (_, _, _, _, ldo) = _out(out, (M, N), out_dtype, x.device, x.codes, x.scales, w.codes, w.scales)
     if M and N:
-        alpha = float(x.tensor_scale or 1.0) * float(w.tensor_scale or 1.0)
         _call(x.device, "fb_fp4_matmul", x.codes, x.scales, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
               FORMATS[x.fmt], alpha)
     return out
@@ -234,11 +262,12 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
            x_scale: Optional[float] = None) -> torch.Tensor:
     """``quantize(x, w.fmt, x_scale) @ w.T`` for ``x`` [M, K] (f32, bf16, f16) and 4-bit weights [N, K], in one call
     (a few short rows in one launch, else two).  ``out_dtype`` defaults to x's; a given ``out`` keeps its own type and must
-    not share memory with x."""
+    not share memory with an operand."""
     if x.dim() != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"linear takes [M, K] and 4-bit [N, K], got {tuple(x.shape)} and {w.shape}")
     if x_scale is not None:
         _check_scale(x_scale, w.fmt)
+    alpha = _alpha(x_scale, w.tensor_scale)
     _, M, K, _, ldx = _matrix(x, "x")
     dev = x.device
     if dev != w.device:
@@ -249,18 +278,15 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
         if out.dtype not in _DTYPES:
             raise TypeError(f"out is float32, bfloat16 or float16, got {out.dtype}")
     else:
-        out, (_, _, _, _, ldo) = _out(out, (M, N), out.dtype, dev)
-        if _overlap(out, x):
-            raise ValueError("out and x share memory")
+        out, (_, _, _, _, ldo) = _out(out, (M, N), out.dtype, dev, x, w.codes, w.scales)
     if M and N:
         g = (K + 127) // 128
         work = None
         if M > 1 or g > LINEAR_INSIDE:   # (one row of up to so many groups is quantised inside the product)
             work = torch.empty((M * 64 * g + 511) // 512 * 512 + (M + 127) // 128 * (g if w.fmt == "mxfp4" else 2 * g) * 512,
                                dtype=torch.uint8, device=dev)
-        alpha = (x_scale or 1.0) * (w.tensor_scale or 1.0)
         _call(dev, "fb_fp4_linear", x, _DTYPES[x.dtype], ldx, work, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
-              FORMATS[w.fmt], float(x_scale or 0.0), float(alpha))
+              FORMATS[w.fmt], float(x_scale or 0.0), alpha)
     return out
 
 
@@ -279,7 +305,9 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     ``scale * score``, with ``norm`` divided by the sum of the chosen scores.  Activations meet the weights as e4m3 with a
     power-of-two scale per 32 values (``ops/quant.py::fp8_act_roundtrip``): x before the gate and up products, and
     ``silu(min(g, limit)) * clamp(u, -limit, limit) * weight`` before the down product (``limit`` 0: no clamp).  The
-    result, summed in f32, is rounded once to ``out_dtype`` (default: x's) or, with ``accumulate``, added to ``out``."""
+    result, summed in f32, is rounded once to ``out_dtype`` (default: x's) or, with ``accumulate``, added to ``out``, which
+    may be x.  A NaN in a token stays in that token's row; a NaN scale in ``w2`` reaches every row of a call in which any token
+    takes that expert (all experts share one accumulator), so ``w2`` should hold none."""
     if score not in SCORES:
         raise ValueError(f"score must be one of {sorted(SCORES)}, got {score!r}")
     if w13.fmt != "mxfp4" or w2.fmt != "mxfp4":
@@ -311,7 +339,7 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     if any(t is not None and t.device != dev for t in (x, logits, bias, w2.codes)):
         raise ValueError("moe takes tensors of one device")
     _, _, _, _, ldx = _matrix(x, "x")
-    out, (_, _, _, _, ldo) = _out(out, (T, D), out_dtype or x.dtype, dev)
+    out, (_, _, _, _, ldo) = _out(out, (T, D), out_dtype or x.dtype, dev, w13.codes, w13.scales, w2.codes, w2.scales)
     if T:
         tile = 128 * (8 if T <= 8 else 16 if T <= 16 else 32) + 512
         work = torch.empty(4096 + min(E, T * topk) * ((I + 127) // 128) * tile, dtype=torch.uint8, device=dev)

@@ -139,3 +139,45 @@ def test_overlap_of_out_and_x(monkeypatch):
     monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
     with pytest.raises(ValueError, match="share memory"):
         fp4.linear(b[:1, :64], _t(64, 64), out=b[:1, :64])
+
+
+def test_columns_of_one_buffer_beside_each_other():
+    b = torch.zeros(4, 256)
+    assert not fp4._overlap(b[:, :100], b[:, 100:]) and not fp4._overlap(b[:, 100:], b[:, :100])
+    assert not fp4._overlap(b[2:, :100], b[:3, 100:]) and fp4._overlap(b[:, :101], b[:, 100:])
+    assert not fp4._overlap(b[:, 100:], b[:, :100].view(torch.int32))
+    assert fp4._overlap(b[:, :100], b.view(2, 512)[:, 100:])   # another row stride: the spans decide
+
+
+def test_an_out_that_meets_itself_or_an_operand(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    q = _t(8, 64, lead=(3,))
+    with pytest.raises(ValueError, match="matrices of out overlap"):
+        fp4.dequantize(q, out=torch.zeros(8, 64).expand(3, 8, 64))
+    with pytest.raises(ValueError, match="matrices of out overlap"):
+        fp4.dequantize(q, out=torch.zeros(4096).as_strided((3, 8, 64), (65, 128, 1)))
+    for out in (torch.zeros(8, 3, 64).transpose(0, 1), torch.zeros(3, 8, 100)[:, :, :64]):   # these do not
+        assert fp4._out(out, (3, 8, 64), out.dtype, out.device)[0] is out
+    w = _t(4, 64)
+    with pytest.raises(ValueError, match="share memory"):
+        fp4.matmul(_t(8, 64), w, out=w.codes.view(-1)[:128].view(torch.float32).view(8, 4))
+
+
+def test_tensor_scales_whose_product_leaves_f32(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    for xs, ws in ((2.0 ** 80, 2.0 ** 80), (2.0 ** -80, 2.0 ** -80)):
+        w = _t(4, 64, "nvfp4")
+        w.tensor_scale = ws
+        x = _t(4, 64, "nvfp4")
+        x.tensor_scale = xs
+        with pytest.raises(ValueError, match="product of the tensor scales"):
+            fp4.matmul(x, w)
+        with pytest.raises(ValueError, match="product of the tensor scales"):
+            fp4.linear(torch.zeros(4, 64), w, x_scale=xs)
+
+
+def test_from_rows_refusals():
+    z = lambda *s: torch.zeros(*s, dtype=torch.uint8)
+    for packed, scale in ((z(16), z(1)), (z(4, 0), z(4, 0)), (z(4, 16), z(4, 2)), (z(4, 8), z(4, 1))):
+        with pytest.raises(ValueError):
+            fp4.Fp4Tensor.from_rows(packed, scale)

@@ -234,3 +234,73 @@ def test_empty_rows():
     assert fp4.matmul(e, w).shape == (0, 64) and fp4.dequantize(e).shape == (0, 256)
     assert fp4.matmul(w, e).shape == (64, 0)
     assert fp4.quantize(torch.empty(0, 4, 64, device="cuda")).shape == (0, 4, 64)
+
+
+def test_columns_of_one_buffer_and_interleaved_batches():
+    """x and out beside each other in one buffer; an out whose matrices interleave."""
+    w = fp4.quantize(torch.randn(96, 256).cuda())
+    b = torch.randn(5, 400, device="cuda")
+    want = fp4.linear(b[:, :256].clone(), w)
+    fp4.linear(b[:, :256], w, out=b[:, 300:396])
+    assert torch.equal(b[:, 300:396], want)
+    q = fp4.quantize(torch.randn(3, 40, 72).cuda())
+    o = torch.empty(40, 3, 72, device="cuda").transpose(0, 1)
+    assert torch.equal(fp4.dequantize(q, out=o), fp4.dequantize(q, torch.float32))
+
+
+FIRST_IN_CAPTURE = """
+import torch
+from ferrite_b200.ops import fp4
+x = torch.randn({M}, 512, device="cuda").bfloat16()
+wf = torch.randn(384, 512, device="cuda")
+logits = torch.randn({M}, 4, device="cuda")
+codes = lambda *s: torch.randint(0, 256, s, dtype=torch.uint8, device="cuda")
+w13 = fp4.Fp4Tensor(codes(4, 2, 128, 256), torch.full((4, 2, 1, 4, 512), 120, dtype=torch.uint8, device="cuda"), "mxfp4", (4, 2, 128, 512))
+w2 = fp4.Fp4Tensor(codes(4, 512, 64), torch.full((4, 4, 1, 512), 120, dtype=torch.uint8, device="cuda"), "mxfp4", (4, 512, 128))
+def run():
+    w = fp4.quantize(wf, "nvfp4")
+    y = fp4.linear(x, w)
+    return w.codes, y, fp4.matmul(fp4.quantize(x, "nvfp4"), w), fp4.moe(x, logits, w13, w2, 2)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = run()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+fp4.check()
+"""
+
+
+@pytest.mark.parametrize("M", [1, 20])
+def test_the_first_call_of_a_process_may_be_captured(M):
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = str(Path(__file__).resolve().parent.parent)
+    r = subprocess.run([sys.executable, "-c", FIRST_IN_CAPTURE.format(M=M)], cwd=root, capture_output=True, text=True, timeout=300,
+                       env={**os.environ, "PYTHONPATH": root})
+    assert r.returncode == 0, r.stderr[-3000:]
+
+
+def test_two_threads_on_two_streams():
+    import threading
+    w = fp4.quantize(torch.randn(512, 1024).cuda())
+    xs = [torch.randn(m, 1024, device="cuda") for m in (1, 7)]
+    want = [fp4.linear(x, w) for x in xs]
+    got = [[], []]
+
+    def work(i):
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(st):
+            got[i] += [fp4.linear(xs[i], w) for _ in range(20)]
+        st.synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in (0, 1)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(len(got[i]) == 20 and all(torch.equal(y, want[i]) for y in got[i]) for i in (0, 1))
+    fp4.check()

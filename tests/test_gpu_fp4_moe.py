@@ -281,3 +281,28 @@ def test_dsv41_decode_through_the_two_kernel_layer(rows):
     a, b = logits[True], logits[False]
     assert (a - b).abs().max().item() < 2e-3 * b.abs().max().item(), (a - b).abs().max().item()
     assert torch.equal(a.argmax(-1), b.argmax(-1))
+
+
+def test_in_place_and_nan_stays_in_its_rows():
+    """out may be x; a token with a NaN, and an expert with a NaN scale in w13, reach the rows that have them only."""
+    T, E, topk, D, I = 6, 8, 2, 256, 64
+    w13, w2 = experts(E, D, I, 5)
+    logits = spread_logits(T, E, 5).cuda()
+    x = torch.randn(T, D, generator=torch.Generator().manual_seed(5)).cuda()
+    want = fp4.moe(x, logits, w13, w2, topk)
+    y = x.clone()
+    fp4.moe(y, logits, w13, w2, topk, out=y)
+    assert torch.equal(y, want)
+    bad = x.clone()
+    bad[2, 17] = float("nan")
+    y = fp4.moe(bad, logits, w13, w2, topk)
+    rest = [t for t in range(T) if t != 2]
+    assert y[2].isnan().all() and torch.equal(y[rest], want[rest])
+    chosen = logits.topk(topk).indices == int(logits[0].argmax())
+    rows = chosen.any(1).cpu()
+    assert rows.any() and not rows.all()
+    broken = fp4.Fp4Tensor(w13.codes, w13.scales.clone(), "mxfp4", w13.shape)
+    broken.scales[int(logits[0].argmax()), 0, 0, 0, 0] = 255     # gate, row 0, block 0
+    y = fp4.moe(x, logits, broken, w2, topk)
+    assert y[rows].isnan().all() and torch.equal(y[~rows], want[~rows])
+    fp4.check()
