@@ -117,16 +117,17 @@ __device__ __forceinline__ void route_load(const MoeArgs& a, Route& r, float* ro
         if (lane == 0) { r.mx[t] = mx; r.inv[t] = 1.f / sum; }
     }
 }
-// The row's logits become keys, from expert `first` in steps of `step` (with a bias; without, the logit itself decides, exactly:
-// every score grows with its logit).
-__device__ __forceinline__ void route_keys(const MoeArgs& a, const Route& r, float* row, const float* bias, int t, int first, int step) {
+// Keys of the row's logits, from expert `first` in steps of `step` (with a bias; without, the logit itself decides, exactly:
+// every score grows with its logit).  They may take the logits' place.
+__device__ __forceinline__ void route_keys(const MoeArgs& a, const Route& r, const float* row, float* keys, const float* bias, int t,
+                                           int first, int step) {
     const float mx = r.mx[t], inv = r.inv[t];
 #pragma unroll 1
     for (int e = first; e < a.E; e += step)
-        reinterpret_cast<uint32_t*>(row)[e] = order_key(key_score(row[e], a.score, mx, inv) + bias[e]);
+        reinterpret_cast<uint32_t*>(keys)[e] = order_key(key_score(row[e], a.score, mx, inv) + bias[e]);
 }
-// The token's choice from its row.  One warp.
-__device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const float* row, int t, int lane) {
+// The token's choice from its row of keys (or, without a bias, of logits); z: its logits.  One warp.
+__device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const float* row, const volatile float* z, int t, int lane) {
     constexpr int kPer = kMaxE / 32;
     uint32_t key[kPer];
 #pragma unroll
@@ -135,6 +136,7 @@ __device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const flo
         key[j] = e >= a.E ? 0u : a.bias ? __float_as_uint(row[e]) : order_key(row[e]);
     }
     int mine = 0;
+    float p = 0.f;
 #pragma unroll 1
     for (int k = 0; k < a.topk; ++k) {
         uint32_t m[kPer];
@@ -150,13 +152,16 @@ __device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const flo
         for (int j = 0; j < kPer; ++j) hit |= key[j] == top ? 1u << j : 0u;
         const uint32_t cand = hit ? (uint32_t)(lane + 32 * (__ffs(hit) - 1)) : 0xffffffffu;
         const uint32_t e = __reduce_min_sync(0xffffffffu, cand);
-        if (lane == k) mine = (int)e;
+        if (lane == k) {
+            mine = (int)e;
+            p = z[e];   // in flight over the rounds that follow
+        }
         const uint32_t gone = (e & 31u) == (uint32_t)lane ? 1u << (e >> 5) : 0u;
 #pragma unroll
         for (int j = 0; j < kPer; ++j)
             if (gone >> j & 1) key[j] = 0u;
     }
-    float p = lane < a.topk ? score_of(ld_f32(a.logits + t * a.ldl + mine), a.score, r.mx[t], r.inv[t]) : 0.f;
+    p = lane < a.topk ? score_of(p, a.score, r.mx[t], r.inv[t]) : 0.f;
     if (a.norm) p = p / (warp_sum(p) + 1e-20f);
     if (lane < a.topk) {
         r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
@@ -164,26 +169,32 @@ __device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const flo
         atomicOr(&r.mask[mine], 1u << t);
     }
 }
-// Few tokens: the first kRouteThreads threads.
-__device__ __forceinline__ void route_together(const MoeArgs& a, Route& r, float* rows, const float* bias) {
+// Few tokens: the first kRouteThreads threads.  Scratch: the bias, a row of logits per token, a row of keys per token.
+__device__ __forceinline__ void route_together(const MoeArgs& a, Route& r, float* bias) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int nw = kRouteThreads / 32;
+    float *rows = bias + a.E, *keys = rows + a.T * a.E;
     auto sync = [&]() { asm volatile("bar.sync 2, %0;" ::"n"(kRouteThreads) : "memory"); };
-    if (warp < a.T) route_load(a, r, rows + warp * a.E, warp, lane);
+    if (warp < a.T) {
+        route_load(a, r, rows + warp * a.E, warp, lane);
+    } else if (a.bias) {   // (a.T < nw: the loads of logits and bias fly together)
+#pragma unroll 4
+        for (int e = (warp - a.T) * 32 + lane; e < a.E; e += (nw - a.T) * 32) bias[e] = ld_f32(a.bias + e);
+    }
     if (a.bias) {
         sync();
         const int stripes = nw / a.T;
         if (warp < a.T * stripes) {
             const int t = warp / stripes;
-            route_keys(a, r, rows + t * a.E, bias, t, (warp - t * stripes) * 32 + lane, 32 * stripes);
+            route_keys(a, r, rows + t * a.E, keys + t * a.E, bias, t, (warp - t * stripes) * 32 + lane, 32 * stripes);
         }
         sync();
     }
     __syncwarp();
-    if (warp < a.T) route_pick(a, r, rows + warp * a.E, warp, lane);
+    if (warp < a.T) route_pick(a, r, (a.bias ? keys : rows) + warp * a.E, rows + warp * a.E, warp, lane);
 }
 // Many tokens: any warp, the next token that nobody has taken.
-__device__ __forceinline__ void route_in_turn(const MoeArgs& a, Route& r, float* rows, const float* bias) {
+__device__ __forceinline__ void route_in_turn(const MoeArgs& a, Route& r, const float* bias, float* rows) {
     const int lane = threadIdx.x & 31;
     for (;;) {
         int t = 0;
@@ -193,9 +204,9 @@ __device__ __forceinline__ void route_in_turn(const MoeArgs& a, Route& r, float*
         float* row = rows + t * a.E;
         route_load(a, r, row, t, lane);
         __syncwarp();
-        if (a.bias) route_keys(a, r, row, bias, t, lane, 32);
+        if (a.bias) route_keys(a, r, row, row, bias, t, lane, 32);
         __syncwarp();
-        route_pick(a, r, row, t, lane);
+        route_pick(a, r, row, a.logits + t * a.ldl, t, lane);
     }
 }
 // The chosen experts, ascending, to r.act and (block 0) to kernel 2.  One warp, after all choices.
@@ -277,12 +288,15 @@ struct UpCfg {
     static_assert(kSfX + 4 * kMaxKb <= kTmem, "tensor memory");
 };
 
-// Shared memory of kernel 1: x blocks | their scale chunks | receive slots | stages | stage scales | barriers
+// Shared memory of kernel 1: x blocks | their scale chunks, then receive slots | stages | stage scales | barriers.  The scale
+// chunks are in tensor memory before the first tile is through, so the slots may take their place once the owner says so
+// (32 tokens, 5120 columns, S = 2: seven stages instead of six).
 template <int BN>
 __host__ __device__ constexpr size_t up_recv_bytes(int S) { return S == 1 ? 0 : (size_t)(S - 1) * (S >= 4 ? 1 : 4 / S) * 2 * BN * 128; }
 template <int BN>
 __host__ __device__ constexpr size_t up_front(int nkb, int S) {
-    return ((size_t)nkb * (BN * 128 + 512) + up_recv_bytes<BN>(S) + 1023) / 1024 * 1024;
+    const size_t sf = (size_t)nkb * 512, recv = up_recv_bytes<BN>(S);
+    return ((size_t)nkb * BN * 128 + (sf > recv ? sf : recv) + 1023) / 1024 * 1024;
 }
 template <int BN>
 __host__ __device__ constexpr size_t up_fixed(int nkb, int S) { return up_front<BN>(nkb, S) + 1024 + UpCfg<BN>::kBars; }
@@ -301,7 +315,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
     const int kb0 = a.g1 * rank / S, kb1 = a.g1 * (rank + 1) / S, nkb = kb1 - kb0;
     const int nkb_max = (a.g1 + S - 1) / S;
     const uint32_t xsf_off = (uint32_t)nkb_max * BN * 128;
-    const uint32_t recv_off = xsf_off + (uint32_t)nkb_max * 512;
+    const uint32_t recv_off = xsf_off;
     const uint32_t st_off = (uint32_t)up_front<BN>(nkb_max, S);
     const uint32_t sf_off = st_off + (uint32_t)stages * C::kA;
     const uint32_t bars = base + sf_off + (uint32_t)stages * 512;
@@ -333,17 +347,18 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         tc::tmem_alloc(tmem_slot, C::kTmem);
         pdl_launch();   // not before: a dependent on this SM could take the tensor memory first, and waits for this kernel's end
     }
-    // scratch of the routing, where the first weights will land: the bias, then a row per token
-    float* bias = reinterpret_cast<float*>(base_g + st_off);
-    float* rows = bias + a.E;
+    float* scratch = reinterpret_cast<float*>(base_g + st_off);   // of the routing, where the first weights will land
+    const bool few = a.T < kRouteThreads / 32;
     for (int e = threadIdx.x; e < kMaxE; e += kUpThreads) R.mask[e] = 0u;
     if (threadIdx.x == 0) R.next = 0;
-    pdl_wait();   // everything below reads what may come from the kernel before
-    for (int e = threadIdx.x; e < a.E && a.bias; e += kUpThreads) bias[e] = ld_f32(a.bias + e);
     __syncthreads();
-    const bool few = a.T < kRouteThreads / 32;
+    pdl_wait();   // everything below reads what may come from the kernel before
+    if (!few && a.bias) {
+        for (int e = threadIdx.x; e < a.E; e += kUpThreads) scratch[e] = ld_f32(a.bias + e);
+        __syncthreads();
+    }
     if (threadIdx.x < kRouteThreads) {
-        if (few) route_together(a, R, rows, bias);
+        if (few) route_together(a, R, scratch);
     } else {
         // ---- this CTA's K range of x, quantised, in operand form ----
         const TX* x = reinterpret_cast<const TX*>(a.x);
@@ -408,7 +423,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             }
         }
     }
-    if (!few) route_in_turn(a, R, rows, bias);   // (warps that quantised x join when they are through)
+    if (!few) route_in_turn(a, R, scratch, scratch + a.E);   // (warps that quantised x join when they are through)
     fence_proxy_async();                         // x blocks, and the scratch that becomes the target of TMA copies
     __syncthreads();
     if (warp == 0) route_list(a, R, lane);
@@ -504,7 +519,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             if (!go) break;
             const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * C::kAccSet);
             if (S > 1 && rank != owner) {
-                if (no && !wait_cluster(recv_free + 8u * q, (no - 1) & 1)) { atomicExch(&s_fail, 1); break; }
+                if (!wait_cluster(recv_free + 8u * q, no & 1)) { atomicExch(&s_fail, 1); break; }
                 const int src = rank < owner ? rank : rank - 1;
                 const uint32_t dst = map_rank(slots + (uint32_t)src * 2 * BN * 128 + lane * 4, owner);
 #pragma unroll 1
@@ -527,6 +542,8 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                 }
                 continue;
             }
+            // (the first tile's MMAs are complete, so x's scales have left the slots' place)
+            if (S > 1 && no == 0 && lane < S && lane != rank) arrive_cluster(map_rank(recv_free + 8u * q, lane));
             if (S > 1 && !wait_cluster(recv_full + 8u * q, no & 1)) { atomicExch(&s_fail, 1); break; }
             // sums of the S parts in rank order, SwiGLU and the block quantiser: lane = row of I, 32 rows = one block
             const uint32_t mask = R.mask[e];
