@@ -148,8 +148,8 @@ fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restri
         }
         float v[8];
         e2m1x8_to_f32(code[g], v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], s), ts);
+        mul8(v, s);
+        if (ts != 1.f) mul8(v, ts);
         T* o = out + p.bt * bstride + r * ld + p.col;
         if (all) {
             store8(o, v);

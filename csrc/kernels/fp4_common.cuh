@@ -187,10 +187,41 @@ __device__ __forceinline__ uint32_t ue8m0_of(uint32_t amax_bits, float floor, fl
 // 1 / 2^(e - 127) for e in 1..253
 __device__ __forceinline__ float ue8m0_inv(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
+// Two f32 in a register pair: the products and sums below take both in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ void mul8(float (&v)[8], float f) {
+    const uint64_t ff = pair(f, f);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) unpair(mul2(pair(v[j], v[j + 1]), ff), v[j], v[j + 1]);
+}
+
 // u / s rounded to nearest, from r = rn(1 / s): Markstein's correction of the product u r.
 __device__ __forceinline__ float div_by(float u, float s, float r) {
     const float q0 = __fmul_rn(u, r);
     return __fmaf_rn(__fmaf_rn(-q0, s, u), r, q0);
+}
+__device__ __forceinline__ void div8_by(float (&v)[8], float s, float r) {
+    const uint64_t ns = pair(-s, -s), rr = pair(r, r);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const uint64_t u = pair(v[j], v[j + 1]), q0 = mul2(u, rr);
+        unpair(fma2(fma2(q0, ns, u), rr, q0), v[j], v[j + 1]);
+    }
 }
 
 // Eight consecutive values of a row (m: the largest of their |.| as integer, the values divided by the tensor scale already)
@@ -203,15 +234,13 @@ __device__ __forceinline__ uint32_t quantize8(float (&v)[8], uint32_t m, uint32_
     if (FMT == kMxFp4) {
         byte = ue8m0_of(m, 6.f * 1.17549435e-38f, kInv6);
         const float inv = ue8m0_inv(min(byte, 253u));
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
+        mul8(v, inv);
     } else {
         byte = m >= kInfBits ? 0x7fu
-                             : (uint32_t)__nv_cvt_float_to_fp8(__fdiv_rn(fmaxf(__uint_as_float(m), 6.f / 512.f), 6.f), __NV_SATFINITE, __NV_E4M3);
+                             : (uint32_t)__nv_cvt_float_to_fp8(div_by(fmaxf(__uint_as_float(m), 6.f / 512.f), 6.f, kInv6), __NV_SATFINITE, __NV_E4M3);
         const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
         const float s = __half2float(*reinterpret_cast<const __half*>(&hr)), r = __frcp_rn(s);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = div_by(v[j], s, r);
+        div8_by(v, s, r);
     }
     return m >= kInfBits ? 0u : e2m1x8(v);   // a block that is not finite: NaN scale, zero codes
 }
@@ -234,8 +263,7 @@ __device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
 template <int FMT>
 __device__ __forceinline__ uint32_t quantize8(float (&v)[8], bool scaled, float ts, float inv_ts, uint32_t& byte) {
     if (FMT == kNvFp4 && scaled) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = div_by(v[j], ts, inv_ts);
+        div8_by(v, ts, inv_ts);
     }
     return quantize8<FMT>(v, max_bits8(v), byte);
 }
