@@ -210,7 +210,10 @@ __device__ __forceinline__ void mul8(float (&v)[8], float f) {
     for (int j = 0; j < 8; j += 2) unpair(mul2(pair(v[j], v[j + 1]), ff), v[j], v[j + 1]);
 }
 
-// u / s rounded to nearest, from r = rn(1 / s): Markstein's correction of the product u r.
+// u / s rounded to nearest, from r = rn(1 / s): Markstein's correction of the product u r.  For an s of four significant bits
+// (an e4m3 number) an r that is off by 2^-22 will do: the residual u - q0 s is exact, so q0 + residual r is off by less than
+// 2^-20 of a step before its rounding, and u / s is never nearer than 1/32 of a step to the middle of two f32 (u and the
+// middle times s are both multiples of 2^-28 of u's binade, and they differ: the middle's 25 bits, times an odd s, are no f32).
 __device__ __forceinline__ float div_by(float u, float s, float r) {
     const float q0 = __fmul_rn(u, r);
     return __fmaf_rn(__fmaf_rn(-q0, s, u), r, q0);
@@ -239,8 +242,10 @@ __device__ __forceinline__ uint32_t quantize8(float (&v)[8], uint32_t m, uint32_
         byte = m >= kInfBits ? 0x7fu
                              : (uint32_t)__nv_cvt_float_to_fp8(div_by(fmaxf(__uint_as_float(m), 6.f / 512.f), 6.f, kInv6), __NV_SATFINITE, __NV_E4M3);
         const __half_raw hr = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3);
-        const float s = __half2float(*reinterpret_cast<const __half*>(&hr)), r = __frcp_rn(s);
-        div8_by(v, s, r);
+        const float s = __half2float(*reinterpret_cast<const __half*>(&hr));
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+        div8_by(v, s, r);   // correctly rounded although r is not: see div_by
     }
     return m >= kInfBits ? 0u : e2m1x8(v);   // a block that is not finite: NaN scale, zero codes
 }

@@ -77,6 +77,23 @@ def test_every_border_of_two_codes(dtype):
         assert same(fp4.reference_dequantize(fp4.quantize(rows.cuda(), fmt)).cpu(), ref_values(rows, fmt))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quotients_by_every_e4m3_scale(dtype):
+    """Every scale byte (its block holds 6 s), with values at random and a few steps around every border of two codes."""
+    g = _gen(11)
+    s = torch.arange(1, 127, dtype=torch.uint8).view(torch.float8_e4m3fn).float()[:, None, None]
+    x = torch.empty(126, 64, 16)
+    near = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])[torch.randint(0, 7, (126, 32, 16), generator=g)] * s
+    bits = near.view(torch.int32) + torch.randint(-3, 4, near.shape, generator=g, dtype=torch.int32)
+    x[:, :32] = bits.view(torch.float32) * (1 - 2 * torch.randint(0, 2, near.shape, generator=g))
+    x[:, 32:] = (torch.rand(126, 32, 16, generator=g) * 2 - 1) * 6 * s
+    x[:, :, 3] = 6 * s[:, :, 0]
+    x = x.view(126, 1024).to(dtype)
+    q = fp4.quantize(x.cuda(), "nvfp4")
+    assert same(fp4.reference_dequantize(q).cpu(), ref_values(x, "nvfp4"))
+    assert torch.equal(fp4.unpack_scales(q.scales, 126, 64).cpu(), torch.arange(1, 127, dtype=torch.uint8)[:, None].expand(126, 64))
+
+
 @pytest.mark.parametrize("ts", [1.0, 0.00037, 2.0 ** -20, 3.7e5, 2.0 ** -100, 2.0 ** 100])
 def test_tensor_scale(ts):
     ts = float(torch.tensor(ts))
