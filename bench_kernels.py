@@ -310,6 +310,48 @@ def make_cases(K, only):
             cases.append(Case(f"mx_gemm.{tag}", wbytes + Mr * D + Mr * Nm * 4, mxfn,
                               f"{Em} experts x {Nm} x {D} e2m1 ({wbytes / 1e6:.0f} MB), {rows_per} rows each (bn {bn}) "
                               f"FLOP={2 * Mr * Nm * D}"))
+    # ---- block-scaled 4-bit operators (ops/fp4.py): quantiser, expander, linear, expert layer for a few tokens ----
+    if want("fp4_"):
+        from ferrite_b200.ops import fp4
+        R, C = 24896, 4096
+        xb = torch.randn(R, C, device=dev).bfloat16()
+        for fmt, per in (("mxfp4", 17 / 32), ("nvfp4", 9 / 16)):
+            if want(f"fp4_quantize.{fmt}"):
+                cases.append(Case(f"fp4_quantize.{fmt}", R * C * (2 + per), lambda fmt=fmt: fp4.quantize(xb, fmt), f"{R} x {C} bf16"))
+            if want(f"fp4_dequantize.{fmt}"):
+                qx, ox = fp4.quantize(xb, fmt), torch.empty_like(xb)
+                cases.append(Case(f"fp4_dequantize.{fmt}", R * C * (2 + per), lambda qx=qx, ox=ox: fp4.dequantize(qx, out=ox), f"{R} x {C} to bf16"))
+        for m, Kd, N, fmt in ((1, 8192, 5120, "mxfp4"), (16, 4096, 24896, "nvfp4"), (1024, 4096, 24896, "mxfp4"), (1024, 4096, 24896, "nvfp4")):
+            name, per = f"fp4_linear.{fmt}.m{m}", 17 / 32 if fmt == "mxfp4" else 9 / 16
+            if not want(name):
+                continue
+            reps = max(2, int(300e6 // (N * Kd * per)) + 1)
+            ws = [fp4.quantize(torch.randn(N, Kd, device=dev), fmt) for _ in range(reps)]
+            xl = torch.randn(m, Kd, device=dev).bfloat16()
+            st = {"i": 0}
+
+            def lin(ws=ws, xl=xl, st=st):
+                st["i"] += 1
+                fp4.linear(xl, ws[st["i"] % len(ws)])
+            cases.append(Case(name, N * Kd * per + m * (Kd + N) * 2, lin, f"{m} x {Kd} x {N}, quantised on the way FLOP={2 * m * N * Kd}"))
+        for T, E, topk, I in ((1, 64, 6, 2304), (5, 64, 3, 2304), (32, 64, 6, 2304)):
+            name = f"fp4_moe.t{T}"
+            if not want(name):
+                continue
+            D, per = 5120, 17 / 32
+            codes = lambda *sh: torch.randint(0, 256, sh, dtype=torch.uint8, device=dev)
+            flat = lambda *sh: torch.full(sh, 120, dtype=torch.uint8, device=dev)
+            w13 = fp4.Fp4Tensor(codes(E, 2, I, D // 2), flat(E, 2, I // 128, D // 128, 512), "mxfp4", (E, 2, I, D))
+            w2 = fp4.Fp4Tensor(codes(E, D, I // 2), flat(E, D // 128, I // 128, 512), "mxfp4", (E, D, I))
+            xs = [torch.randn(T, D, device=dev).bfloat16() for _ in range(8)]
+            lgs = [torch.randn(T, E, device=dev) for _ in range(8)]
+            hit = sum(len(lg.topk(topk).indices.unique()) for lg in lgs) / 8
+            st = {"i": 0}
+
+            def moe(w13=w13, w2=w2, xs=xs, lgs=lgs, topk=topk, st=st):
+                st["i"] += 1
+                fp4.moe(xs[st["i"] % 8], lgs[st["i"] % 8], w13, w2, topk, limit=7.0)
+            cases.append(Case(name, hit * 3 * D * I * per, moe, f"{T} tokens, {hit:.1f} of {E} experts of {D} x {I} on average"))
     # ---- GLM: W8A16 grouped tcgen05 GEMM (e4m3 weights + 128x128 f32 scales, f16 rows), prefill sizes ----
     if want("fp8w_gemm"):
         for tag, Em, Nm, Km, rows_per in (("gate_up.128e.r64", 128, 4096, 4096, 64), ("down.128e.r64", 128, 4096, 2048, 64),

@@ -192,14 +192,19 @@ def quantize(x: torch.Tensor, fmt: str = "mxfp4", tensor_scale: Optional[float] 
     return Fp4Tensor._of(codes, scales, fmt, tuple(x.shape), tensor_scale)
 
 
+def _extent(t: torch.Tensor) -> int:
+    """Bytes from the first to behind the last element."""
+    n = t.numel()
+    if n and not t.is_contiguous():
+        n = 1 + sum((k - 1) * s for k, s in zip(t.shape, t.stride()))
+    return n * t.element_size()
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Whether two tensors of consecutive last dimensions may share memory: the spans between their first and last elements
     meet, and they are not columns of one buffer that lie beside each other."""
-    if not a.numel() or not b.numel():
-        return False
-    extent = lambda t: (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
     a0, b0 = a.data_ptr(), b.data_ptr()
-    if a0 >= b0 + extent(b) or b0 >= a0 + extent(a):
+    if b0 >= a0 + _extent(a) or a0 >= b0 + _extent(b):
         return False
     if a.dim() == b.dim() == 2 and a.shape[0] > 1 and b.shape[0] > 1:
         pitch = a.stride(0) * a.element_size()
