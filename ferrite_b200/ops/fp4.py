@@ -72,6 +72,11 @@ class Fp4Tensor:
     def device(self) -> torch.device:
         return self.codes.device
 
+    def to(self, device, non_blocking: bool = False) -> "Fp4Tensor":
+        """The same tensor on another device."""
+        move = lambda t: t.to(device, non_blocking=non_blocking)
+        return Fp4Tensor(move(self.codes), move(self.scales), self.fmt, self.shape, self.tensor_scale)
+
     def __repr__(self) -> str:
         return f"Fp4Tensor({self.fmt}, shape={self.shape}, tensor_scale={self.tensor_scale}, device={self.device})"
 
@@ -92,6 +97,8 @@ class Fp4Tensor:
             raise TypeError("packed codes and scale bytes are uint8")
         g = (cols + 127) // 128
         codes = torch.nn.functional.pad(packed, (0, 64 * g - cols // 2)).contiguous()
+        if codes.data_ptr() == packed.data_ptr():   # nothing was padded: the caller's bytes, on whatever boundary
+            codes = codes.clone()
         return Fp4Tensor(codes, pack_scales(scale, 128 * g // BLOCK[fmt]), fmt, (*packed.shape[:-1], cols), tensor_scale)
 
 

@@ -181,3 +181,14 @@ def test_from_rows_refusals():
     for packed, scale in ((z(16), z(1)), (z(4, 0), z(4, 0)), (z(4, 16), z(4, 2)), (z(4, 8), z(4, 1))):
         with pytest.raises(ValueError):
             fp4.Fp4Tensor.from_rows(packed, scale)
+
+
+def test_from_rows_copies_bytes_on_any_boundary():
+    raw = torch.randint(0, 256, (3 + 4 * 64,), dtype=torch.uint8)
+    packed = raw[3:].view(4, 64)
+    t = fp4.Fp4Tensor.from_rows(packed, torch.zeros(4, 4, dtype=torch.uint8))
+    before = t.codes.clone()
+    raw.zero_()
+    assert torch.equal(t.codes, before) and before.any()
+    u = t.to("cpu")
+    assert u.shape == t.shape and torch.equal(u.codes, t.codes) and torch.equal(u.scales, t.scales)
