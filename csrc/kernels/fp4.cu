@@ -50,9 +50,10 @@ __device__ __forceinline__ bool whole(const Place& p, int64_t rows, int64_t cols
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(kQThreads)
-fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int vec, uint8_t* __restrict__ codes,
-                    uint8_t* __restrict__ scales, int64_t rows, int64_t cols, int scaled, float ts, float inv_ts) {
-    pdl_launch();   // (launched plainly: its own predecessor is complete)
+fp4_quantize_kernel(const T* x, int64_t ld, int64_t bstride, int vec, uint8_t* codes,
+                    uint8_t* scales, int64_t rows, int64_t cols, int scaled, float ts, float inv_ts) {
+    pdl_wait();
+    pdl_launch();
     const Place p = place(rows, cols);
     const int lane = threadIdx.x & 31;
     const int64_t G = groups(cols), cstride = 64 * G;
@@ -64,7 +65,7 @@ fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int ve
         if constexpr (sizeof(T) == 2) {
             uint4 raw[4];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) raw[g] = ldg_nc_v4(xp + g * step);
+            for (int g = 0; g < 4; ++g) raw[g] = ld_v4(xp + g * step);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 float v[8];
@@ -119,20 +120,22 @@ fp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int64_t bstride, int ve
 
 template <int FMT, typename T>
 __global__ void __launch_bounds__(kQThreads)
-fp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out, int64_t ld,
+fp4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int64_t ld,
                       int64_t bstride, int vec, int64_t rows, int64_t cols, float ts) {
+    pdl_wait();
+    pdl_launch();
     const Place p = place(rows, cols);
     if (p.row >= rows || p.col >= cols) return;
     const int64_t G = groups(cols), cstride = 64 * G, nrt = (rows + 127) / 128;
     constexpr int kChunkCols = FMT == kMxFp4 ? 128 : 64;
     const int64_t C = FMT == kMxFp4 ? G : 2 * G;
-    const uint4 sw = ldg_nc_v4(scales + ((p.bt * nrt + p.tile) * C + p.col / kChunkCols) * 512 + p.i * 16);
+    const uint4 sw = ld_v4(scales + ((p.bt * nrt + p.tile) * C + p.col / kChunkCols) * 512 + p.i * 16);
     const uint32_t w[4] = {sw.x, sw.y, sw.z, sw.w};
     uint32_t code[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         const int64_t r = p.row + 32 * g;
-        code[g] = r < rows ? __ldg(reinterpret_cast<const uint32_t*>(codes + (p.bt * rows + r) * cstride + p.col / 2)) : 0u;
+        code[g] = r < rows ? *reinterpret_cast<const uint32_t*>(codes + (p.bt * rows + r) * cstride + p.col / 2) : 0u;
     }
     const int shift = FMT == kMxFp4 ? 8 * (int)(p.col / 32 & 3) : 8 * (int)(p.col / 16 & 3);
     const int n = (int)min((int64_t)8, cols - p.col);
@@ -197,10 +200,8 @@ FB_API int fb_fp4_status(int* host, int64_t clear, cudaStream_t st) {
     return (int)e;
 }
 
-// x [batch][rows][cols] (element strides bstride, ld, 1; dtype 0 f32, 1 bf16, 2 f16) -> codes, scales (fp4_common.cuh);
-// fmt 0 mxfp4, 1 nvfp4; ts: the tensor's scale (nvfp4, 2^-100 .. 2^100; 0: none).
-FB_API int fb_fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bstride, void* codes, void* scales, int64_t batch,
-                           int64_t rows, int64_t cols, int64_t fmt, float ts, cudaStream_t st) {
+int fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bstride, void* codes, void* scales, int64_t batch, int64_t rows,
+                 int64_t cols, int64_t fmt, float ts, bool pdl, cudaStream_t st) {
     if (batch < 1 || rows < 1 || cols < 1 || (fmt != kMxFp4 && fmt != kNvFp4) || dtype < 0 || dtype > 2 ||
         ((uintptr_t)codes & 15) || ((uintptr_t)scales & 15))
         return (int)cudaErrorInvalidValue;
@@ -210,11 +211,18 @@ FB_API int fb_fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bst
     const float inv = scaled ? (float)(1.0 / (double)ts) : 1.f;
     const int vec = rows_of_8(x, ld, bstride, dtype == kF32 ? 4 : 2);
 #define FP4_Q(F, D)                                                                                                         \
-    (int)fp4_launch(fp4_quantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, false,      \
+    (int)fp4_launch(fp4_quantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, pdl,  \
                     (const Elem<D>::T*)x, ld, bstride, vec, (uint8_t*)codes, (uint8_t*)scales, rows, cols, scaled, ts, inv)
     if (fmt == kMxFp4) return dtype == kF32 ? FP4_Q(kMxFp4, kF32) : dtype == kBf16 ? FP4_Q(kMxFp4, kBf16) : FP4_Q(kMxFp4, kF16);
     return dtype == kF32 ? FP4_Q(kNvFp4, kF32) : dtype == kBf16 ? FP4_Q(kNvFp4, kBf16) : FP4_Q(kNvFp4, kF16);
 #undef FP4_Q
+}
+
+// x [batch][rows][cols] (element strides bstride, ld, 1; dtype 0 f32, 1 bf16, 2 f16) -> codes, scales (fp4_common.cuh);
+// fmt 0 mxfp4, 1 nvfp4; ts: the tensor's scale (nvfp4, 2^-100 .. 2^100; 0: none).
+FB_API int fb_fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bstride, void* codes, void* scales, int64_t batch,
+                           int64_t rows, int64_t cols, int64_t fmt, float ts, cudaStream_t st) {
+    return fp4_quantize(x, dtype, ld, bstride, codes, scales, batch, rows, cols, fmt, ts, true, st);
 }
 
 // codes, scales -> out [batch][rows][cols] (element strides bstride, ld, 1).
@@ -228,7 +236,7 @@ FB_API int fb_fp4_dequantize(const void* codes, const void* scales, void* out, i
     const int vec = rows_of_8(out, ld, bstride, dtype == kF32 ? 4 : 2);
     const float t = ts == 0.f ? 1.f : ts;
 #define FP4_D(F, D)                                                                                                    \
-    (int)fp4_launch(fp4_dequantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, false, \
+    (int)fp4_launch(fp4_dequantize_kernel<F, Elem<D>::T>, dim3((unsigned)grid), dim3(kQThreads), 0, st, 1, true, \
                     (const uint8_t*)codes, (const uint8_t*)scales, (Elem<D>::T*)out, ld, bstride, vec, rows, cols, t)
     if (fmt == kMxFp4) return dtype == kF32 ? FP4_D(kMxFp4, kF32) : dtype == kBf16 ? FP4_D(kMxFp4, kBf16) : FP4_D(kMxFp4, kF16);
     return dtype == kF32 ? FP4_D(kNvFp4, kF32) : dtype == kBf16 ? FP4_D(kNvFp4, kBf16) : FP4_D(kNvFp4, kF16);

@@ -84,7 +84,8 @@ struct GemmArgs {
     int64_t ldo;
     int64_t P, Q, K;
     float alpha;
-    int dtype, vec, tiles_p, tiles_q, splits, pdl;
+    int dtype, vec, tiles_p, tiles_q, splits;
+    int behind;               // the kernel before this one is the quantiser of X, and everything before that is complete
     int* status;
 };
 
@@ -201,6 +202,7 @@ __device__ __forceinline__ void store_reduced(const GemmArgs& a, uint32_t part, 
 // codes, then the scale chunks.  Columns behind K count as zeros (their scales have to be numbers).
 template <int FMT, typename C>
 __device__ __forceinline__ void quantize_x(const GemmArgs& a, uint8_t* room, int t, int kb0, int kb1, uint32_t x_full, int lane) {
+    pdl_wait();
     const int units = (kb1 - kb0) * 32;                    // of eight columns
     const int esz = a.xdt == kF32 ? 4 : 2;
     const bool vec = (uintptr_t)a.x % (8 * esz) == 0 && a.ldx % 8 == 0;
@@ -284,7 +286,11 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         tc::prefetch_tmap(&tmap_q);
         if (!SWAP) tc::prefetch_tmap(&tmap_o);
     }
-    if (warp == 1) tc::tmem_alloc(tmem_slot, C::kTmem);
+    if (warp == 1) {
+        if (!a.behind) pdl_wait();   // for the tensor memory's sake; the threads that read do it for theirs
+        tc::tmem_alloc(tmem_slot, C::kTmem);
+        pdl_launch();
+    }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -318,7 +324,8 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                 const uint8_t* fq = QX ? nullptr : a.sfq + ((q0 / 128) * Cch + (int64_t)kb0 * C::kChunks) * 512;
                 const uint32_t qat = QX ? 0u : (uint32_t)at;
                 int kb = kb0;
-                if (t == first && a.pdl) {
+                if (t == first && !a.behind) pdl_wait();
+                if (t == first && a.behind) {
                     // X is written by the kernel before this one: only W (P when swapped) may be read before the wait
                     const int ahead = SWAP ? min(C::kStages, kb1 - kb0) : 0;
                     for (int i = 0; i < ahead; ++i) {
@@ -557,8 +564,10 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
         tc::prefetch_tmap(&tmap_o);
     }
     if (warp == 1) {
+        if (!a.behind) pdl_wait();
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "n"(C::kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        pdl_launch();
     }
     tc::tc_fence_before();
     __syncthreads();
@@ -570,7 +579,7 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
 
     if (warp == 0) {
         if (elect_one()) {
-            if (a.pdl) pdl_wait();   // X is written by the kernel before this one
+            pdl_wait();
             int s = 0, round = 0;
             bool ok = true;
             const uint32_t lead = map_rank(full(0), 0);
@@ -702,7 +711,7 @@ int launch_gemm(const GemmArgs& a, const void* pc, const void* qc, int grid, cud
     static unsigned long long allowed = 0;
     cudaError_t e = fp4_allow_smem(k, C::kSmem, allowed);
     if (e != cudaSuccess) return (int)e;
-    return (int)fp4_launch(k, dim3((unsigned)grid), dim3(kGThreads), C::kSmem, st, a.splits, a.pdl != 0, tp, tq, to, a);
+    return (int)fp4_launch(k, dim3((unsigned)grid), dim3(kGThreads), C::kSmem, st, a.splits, true, tp, tq, to, a);
 }
 
 // Clusters of 1 .. 8 CTAs that fit the device at one CTA per SM (measured: a cluster stays inside a GPC).
@@ -727,7 +736,7 @@ int launch_pair(GemmArgs a, const void* pc, const void* qc, cudaStream_t st) {
     cudaError_t e = fp4_allow_smem(k, C::kSmem, allowed);
     if (e != cudaSuccess) return (int)e;
     const int tiles = a.tiles_p * a.tiles_q, pairs = 74;
-    return (int)fp4_launch(k, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), dim3(kGThreads), C::kSmem, st, 2, a.pdl != 0, tp, tq, tsp, tsq, to, a);
+    return (int)fp4_launch(k, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))), dim3(kGThreads), C::kSmem, st, 2, true, tp, tq, tsp, tsq, to, a);
 }
 
 template <int FMT>
@@ -805,8 +814,6 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
 
 }  // namespace
 
-FB_API int fb_fp4_quantize(const void*, int64_t, int64_t, int64_t, void*, void*, int64_t, int64_t, int64_t, int64_t, float, cudaStream_t);
-
 static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, int64_t M, int64_t N, int64_t fmt, GemmArgs a,
                       cudaStream_t st) {
     if (M < 1 || N < 1 || a.K < 1 || M > 0x7fffff00ll || N > 0x7fffff00ll || a.K > 0x3fffff00ll || a.ldo < N || a.dtype < 0 || a.dtype > 2 ||
@@ -847,9 +854,9 @@ FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, co
     if (!work) return (int)cudaErrorInvalidValue;
     uint8_t* codes = (uint8_t*)work;
     uint8_t* scales = codes + (M * 64 * groups(K) + 511) / 512 * 512;
-    rc = fb_fp4_quantize(x, xdt, ldx, 0, codes, scales, 1, M, K, fmt, xts, st);
+    rc = fp4_quantize(x, xdt, ldx, 0, codes, scales, 1, M, K, fmt, xts, false, st);
     if (rc) return rc;
     a.x = nullptr;
-    a.pdl = 1;
+    a.behind = 1;
     return fp4_matmul(codes, scales, wc, ws, M, N, fmt, a, st);
 }

@@ -347,9 +347,6 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
             tc::prefetch_tmap(&tmap_w);
             tc::prefetch_tmap(&tmap_tail);
         }
-        __syncwarp();
-        tc::tmem_alloc(tmem_slot, C::kTmem);
-        pdl_launch();   // not before: a dependent on this SM could take the tensor memory first, and waits for this kernel's end
     }
     float* scratch = reinterpret_cast<float*>(base_g + st_off);   // of the routing, where the first weights will land
     const bool few = a.T < kRouteThreads / 32;
@@ -428,6 +425,11 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
         }
     }
     if (!few) route_in_turn(a, R, scratch, scratch + a.E);   // (warps that quantised x join when they are through)
+    __syncwarp();
+    if (warp == 9) {
+        tc::tmem_alloc(tmem_slot, C::kTmem);
+        pdl_launch();   // not before: a dependent on this SM could take the tensor memory first, and waits for this kernel's end
+    }
     fence_proxy_async();                         // x blocks, and the scratch that becomes the target of TMA copies
     __syncthreads();
     if (warp == 0) route_list(a, R, lane);

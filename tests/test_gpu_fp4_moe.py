@@ -306,3 +306,49 @@ def test_in_place_and_nan_stays_in_its_rows():
     y = fp4.moe(x, logits, broken, w2, topk)
     assert y[rows].isnan().all() and torch.equal(y[~rows], want[~rows])
     fp4.check()
+
+
+@pytest.mark.parametrize("T", [1, 4, 24])
+def test_a_chain_of_calls_that_each_read_what_the_one_before_wrote(T):
+    """Kernels start beside the end of their predecessors: back to back, replayed from a graph, or with a wait after every
+    call, the bits are the same."""
+    D, E, topk, I = 1024, 8, 2, 256
+    w13, w2 = experts(E, D, I, 7)
+    g = torch.Generator().manual_seed(7)
+    wa, wb = (fp4.quantize((torch.randn(D, D, generator=g) * D ** -0.5).cuda(), f) for f in ("nvfp4", "mxfp4"))
+    x0 = torch.randn(T, D, generator=g).cuda()
+    router = (torch.randn(E, D, generator=g) * D ** -0.5).cuda()
+
+    def chain(after=lambda: None):
+        x, seen = x0, []
+        for _ in range(6):
+            y = fp4.linear(x, wa)
+            after()
+            q = fp4.quantize(y, "mxfp4")
+            after()
+            z = fp4.dequantize(q, torch.float32)
+            after()
+            m = fp4.matmul(fp4.quantize(z, "mxfp4"), wb, torch.float32)
+            after()
+            m2 = fp4.matmul(q, wb, torch.float32, out=z)       # into what the quantiser before has just read
+            after()
+            x = fp4.moe(m, m2 @ router.t(), w13, w2, topk, scale=3.0, out=m2, accumulate=True)
+            after()
+            x = fp4.linear(x, wb)
+            seen += [y, m, x]
+            x = x / x.std()
+            after()
+        return seen
+
+    want = chain(torch.cuda.synchronize)
+    assert all(t.isfinite().all() and t.std() > 1e-3 for t in want)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(chain(), want))
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = chain()
+    for _ in range(5):
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    fp4.check()
