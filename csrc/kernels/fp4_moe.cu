@@ -21,12 +21,12 @@
 // Kernel 2 (down): a cluster of S CTAs per 128 rows of the output; the (expert, 128 columns of I) blocks of all chosen
 // experts are one long K axis, split over the cluster, accumulated in ONE accumulator: the sum over experts costs
 // nothing.  Partials are summed in rank order.  No atomics anywhere: the same bits every run.
-// Both kernels are launched with programmatic serialisation: they set up (barriers, tensor memory) beside the end of the kernel
+// Both kernels are launched with programmatic serialisation: they set up (barriers, tables) beside the end of the kernel
 // before and wait for it before they read anything (one token, call after call: 36.9 us without it for kernel 1, 34.6 with).
 // Kernel 2 then reads the list of chosen experts, which kernel 1 leaves behind (routing again there cost 4 us at its head).
 // Experts of 5120 x 2304, a call among others: one token (6 experts, 113 MB, 17.2 us of HBM) 34 us: 7 until the first weight of kernel 1
 // (routing 5), 12.5 of weights, 5 until the first weight of kernel 2, 5 of weights, 2 for the sum; 5 tokens (15 experts, 43 us of HBM)
-// 58 us; 32 tokens (88 experts, 252 us of HBM) 317 us, 18 of them routing.  8 tokens of 44 experts of 5120 x 576 (32 us of HBM)
+// 58 us; 32 tokens (88 experts, 252 us of HBM) 313 us, 18 of them routing.  8 tokens of 44 experts of 5120 x 576 (32 us of HBM)
 // 60 us.  The first kernel's weights in flight decide at 32 tokens: six stages beside x and the receive slots 338 us, seven 317.
 #include "fp4_common.cuh"
 
