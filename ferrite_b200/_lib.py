@@ -22,6 +22,9 @@ class KernelError(RuntimeError):
     pass
 
 
+_Tensor = torch.Tensor
+
+
 class KernelLib:
     def __init__(self, path: Path = _LIB_PATH, check_build_id: bool = True):
         if not path.exists():
@@ -55,7 +58,7 @@ class KernelLib:
         rc = None
         if fast is not None:   # argument kinds are known from the first call: ctypes converts plain numbers by itself
             try:
-                rc = fast(*[a.data_ptr() if type(a) is torch.Tensor else a for a in args], stream)
+                rc = fast(*[a.data_ptr() if type(a) is _Tensor else a for a in args], stream)
             except ctypes.ArgumentError:
                 rc = None
         if rc is None:

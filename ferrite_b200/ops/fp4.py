@@ -133,6 +133,8 @@ def _check_scale(ts: float, fmt: str) -> None:
 def _alpha(xs: Optional[float], ws: Optional[float]) -> float:
     """The factor of a product's sums.  (The scales of an ordinary pair multiply to something near one; out of this range the
     factor itself would overflow f32 or lose bits.)"""
+    if xs is None and ws is None:
+        return 1.0
     alpha = (xs or 1.0) * (ws or 1.0)
     if not 2.0 ** -100 <= alpha <= 2.0 ** 100:
         raise ValueError(f"the product of the tensor scales must be in [2^-100, 2^100], got {alpha!r}")
