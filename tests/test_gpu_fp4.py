@@ -321,3 +321,25 @@ def test_two_threads_on_two_streams():
     [t.join() for t in threads]
     assert all(len(got[i]) == 20 and all(torch.equal(y, want[i]) for y in got[i]) for i in (0, 1))
     fp4.check()
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 values: the last rows are what they are in a small call."""
+    R, C = 300_000, 8192
+    t0 = R // 128 * 128
+    x = torch.empty(R, C, dtype=torch.bfloat16, device="cuda")
+    x[:t0].fill_(1.0)
+    x[t0:] = torch.randn(R - t0, C, generator=_gen(4)).cuda()
+    for fmt in ("mxfp4", "nvfp4"):
+        q, tail = fp4.quantize(x, fmt), fp4.quantize(x[t0:], fmt)
+        assert torch.equal(q.codes[t0:], tail.codes) and torch.equal(q.scales[t0 // 128:], tail.scales)
+        d = fp4.dequantize(q)
+        assert torch.equal(d[t0:], fp4.dequantize(tail)) and torch.equal(d[:4], fp4.dequantize(fp4.quantize(x[:4], fmt)))
+        del q, d
+    w = fp4.quantize(torch.randn(C, 128, generator=_gen(5)).cuda(), "nvfp4")
+    xs = x[:, :128]
+    y = fp4.linear(xs, w)
+    assert y.numel() > 2 ** 31
+    for rows in (slice(0, 256), slice(t0, R)):
+        assert torch.equal(y[rows], fp4.linear(xs[rows].contiguous(), w))
+    fp4.check()
