@@ -29,7 +29,8 @@ int* fp4_status_ptr();
 //     exception is the product behind its own quantiser, which reads the weights: the quantiser lets it start after its own
 //     wait, when everything before the quantiser is complete;
 //   * a kernel that waits for another holds no tensor memory that the other may still ask for: tensor memory is taken
-//     after the wait, or behind a kernel of this file's family, which lets dependents start once it has its own.
+//     after the wait.  Of the kernel before nothing is presumed, not even behind a launch of the same call: two host threads
+//     may share a stream, and many a kernel lets its dependents start before it has taken its own.
 template <typename... KArgs, typename... Args>
 inline cudaError_t fp4_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, int cluster, bool pdl,
                               Args&&... args) {

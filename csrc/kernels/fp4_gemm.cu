@@ -286,16 +286,24 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         tc::prefetch_tmap(&tmap_q);
         if (!SWAP) tc::prefetch_tmap(&tmap_o);
     }
-    if (warp == 1) {
-        if (!a.behind) pdl_wait();   // for the tensor memory's sake; the threads that read do it for theirs
-        tc::tmem_alloc(tmem_slot, C::kTmem);
-        pdl_launch();
-    }
-    tc::tc_fence_before();
     __syncthreads();
-    tc::tc_fence_after();
-    uint32_t tmem;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    // Tensor memory, for every warp but the producer.  It is taken behind the wait: whatever kernel is before this one in
+    // the stream (another host thread may have put one between the quantiser and this launch) may still ask for its own.
+    uint32_t tmem = 0;
+    if (warp >= 1) {
+        if constexpr (QX) {
+            if (warp >= 2) quantize_x<FMT, C>(a, smem_raw + (xroom - base), threadIdx.x - 64, kb0, kb1, x_full, lane);
+        }
+        if (warp == 1) {
+            pdl_wait();
+            tc::tmem_alloc(tmem_slot, C::kTmem);
+            pdl_launch();
+        }
+        tc::tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(kGThreads - 32) : "memory");
+        tc::tc_fence_after();
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+    }
     const uint32_t a_off = 0, b_off = C::kABytes, sfa_off = b_off + (QX ? 0 : C::kBBytes), sfb_off = sfa_off + C::kSfa;
 
     if (warp == 0) {
@@ -400,7 +408,6 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
         const int w = warp - 2;
         // warps 2..9: TMEM lane quarter = warp & 3
         const int quarter_warp = (warp & 3) | (w >= 4 ? 4 : 0);
-        if constexpr (QX) quantize_x<FMT, C>(a, smem_raw + (xroom - base), threadIdx.x - 64, kb0, kb1, x_full, lane);
         int tile_no = 0, turn = 0;
         for (int t = first; t < n_tiles; t += step, ++tile_no) {
             int64_t p0, q0;
@@ -564,7 +571,7 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
         tc::prefetch_tmap(&tmap_o);
     }
     if (warp == 1) {
-        if (!a.behind) pdl_wait();
+        pdl_wait();   // before the tensor memory, as above
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "n"(C::kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         pdl_launch();

@@ -650,11 +650,11 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
         tc::mbar_fence_init();
         tc::prefetch_tmap(&tmap_w);
     }
+    pdl_wait();   // everything below reads what kernel 1 wrote
     if (warp == 1) {
-        tc::tmem_alloc(tmem_slot, C::kTmem);
+        tc::tmem_alloc(tmem_slot, C::kTmem);   // behind the wait: the kernel before need not be kernel 1 (another thread on the stream)
         pdl_launch();   // as in kernel 1
     }
-    pdl_wait();   // everything below reads what kernel 1 wrote
     if (warp >= 2) {
         const volatile int* list = a.list;   // (a read-only load might move above the wait)
         const int n = list[0];
