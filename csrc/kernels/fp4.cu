@@ -122,8 +122,9 @@ template <int FMT, typename T>
 __global__ void __launch_bounds__(kQThreads)
 fp4_dequantize_kernel(const uint8_t* codes, const uint8_t* scales, T* out, int64_t ld,
                       int64_t bstride, int vec, int64_t rows, int64_t cols, float ts) {
+    // No early start for the kernel behind this one: what is expanded may be its weights, and the decode GEMVs fetch their first
+    // weights before their wait (common.cuh).
     pdl_wait();
-    pdl_launch();
     const Place p = place(rows, cols);
     if (p.row >= rows || p.col >= cols) return;
     const int64_t G = groups(cols), cstride = 64 * G, nrt = (rows + 127) / 128;

@@ -28,6 +28,7 @@ int* fp4_status_ptr();
 //   * a kernel touches no memory before its griddepcontrol.wait, so completion is transitive along the stream; the one
 //     exception is the product behind its own quantiser, which reads the weights: the quantiser lets it start after its own
 //     wait, when everything before the quantiser is complete;
+//   * the expander lets nothing start early, because its output may be the weights of a kernel that reads them before its wait;
 //   * a kernel that waits for another holds no tensor memory that the other may still ask for: tensor memory is taken
 //     after the wait.  Of the kernel before nothing is presumed, not even behind a launch of the same call: two host threads
 //     may share a stream, and many a kernel lets its dependents start before it has taken its own.

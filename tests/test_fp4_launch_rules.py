@@ -32,3 +32,10 @@ def test_tensor_memory_is_taken_behind_an_unconditional_wait(name, kernels):
             assert waits, f"{kernel} takes tensor memory before an unconditional pdl_wait()"
             assert "pdl_launch();" not in body[:alloc.start()], f"{kernel} lets its dependents start before it has its tensor memory"
     assert seen == kernels
+
+
+def test_the_expander_lets_nothing_start_early():
+    """Its output may be the weights of the next kernel, and the decode GEMVs fetch weights before they wait."""
+    bodies = dict(kernel_bodies("fp4.cu"))
+    assert "pdl_launch" in bodies["fp4_quantize_kernel"] and "pdl_wait();" in bodies["fp4_dequantize_kernel"]
+    assert "pdl_launch" not in bodies["fp4_dequantize_kernel"]
