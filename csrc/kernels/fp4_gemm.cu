@@ -822,24 +822,25 @@ int gemm_fmt(GemmArgs a, const void* xc, const uint8_t* xs, const void* wc, cons
 }  // namespace
 
 static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, int64_t M, int64_t N, int64_t fmt, GemmArgs a,
-                      cudaStream_t st) {
+                      int* status, cudaStream_t st) {
     if (M < 1 || N < 1 || a.K < 1 || M > 0x7fffff00ll || N > 0x7fffff00ll || a.K > 0x3fffff00ll || a.ldo < N || a.dtype < 0 || a.dtype > 2 ||
         (fmt != kMxFp4 && fmt != kNvFp4) || (((uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws) & 15))
         return (int)cudaErrorInvalidValue;
     const int esz = a.dtype == kF32 ? 4 : 2;
     a.vec = ((uintptr_t)a.out & 15) == 0 && a.ldo * esz % 16 == 0;
-    a.status = fp4_status_ptr();
+    a.status = status ? status : fp4_status_ptr();
     if (!a.status) return (int)cudaErrorNotSupported;
     return fmt == kMxFp4 ? gemm_fmt<kMxFp4>(a, xc, (const uint8_t*)xs, wc, (const uint8_t*)ws, M, N, st)
                          : gemm_fmt<kNvFp4>(a, xc, (const uint8_t*)xs, wc, (const uint8_t*)ws, M, N, st);
 }
 
 // out[M, N] (row stride ldo, dtype 0 f32, 1 bf16, 2 f16) = alpha * X W^T of two 4-bit matrices of one format with K columns.
+// status: four words that a wait that ran out reports to, or null for the device's own (fb_fp4_status).
 FB_API int fb_fp4_matmul(const void* xc, const void* xs, const void* wc, const void* ws, void* out, int64_t dtype, int64_t ldo,
-                         int64_t M, int64_t N, int64_t K, int64_t fmt, float alpha, cudaStream_t st) {
+                         int64_t M, int64_t N, int64_t K, int64_t fmt, float alpha, int* status, cudaStream_t st) {
     GemmArgs a = {};
     a.out = out; a.ldo = ldo; a.K = K; a.alpha = alpha; a.dtype = (int)dtype;
-    return fp4_matmul(xc, xs, wc, ws, M, N, fmt, a, st);
+    return fp4_matmul(xc, xs, wc, ws, M, N, fmt, a, status, st);
 }
 
 // The same with the rows of x [M, K] (element type xdt, row stride ldx; nvfp4: tensor scale xts or 0) quantised first: inside the
@@ -848,7 +849,7 @@ FB_API int fb_fp4_matmul(const void* xc, const void* xs, const void* wc, const v
 // columns never needs `work`.)
 FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, const void* wc, const void* ws, void* out,
                          int64_t dtype, int64_t ldo, int64_t M, int64_t N, int64_t K, int64_t fmt, float xts, float alpha,
-                         cudaStream_t st) {
+                         int* status, cudaStream_t st) {
     if (M < 1 || K < 1 || xdt < 0 || xdt > 2 || ldx < K || ((uintptr_t)work & 15)) return (int)cudaErrorInvalidValue;
     GemmArgs a = {};
     a.out = out; a.ldo = ldo; a.K = K; a.alpha = alpha; a.dtype = (int)dtype;
@@ -856,7 +857,7 @@ FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, co
     a.scaled = fmt == kNvFp4 && xts != 0.f && xts != 1.f;
     a.xts = xts;
     a.xinv = a.scaled ? (float)(1.0 / (double)xts) : 1.f;
-    int rc = fp4_matmul(nullptr, nullptr, wc, ws, M, N, fmt, a, st);
+    int rc = fp4_matmul(nullptr, nullptr, wc, ws, M, N, fmt, a, status, st);
     if (rc != kNotTaken) return rc;
     if (!work) return (int)cudaErrorInvalidValue;
     uint8_t* codes = (uint8_t*)work;
@@ -865,5 +866,5 @@ FB_API int fb_fp4_linear(const void* x, int64_t xdt, int64_t ldx, void* work, co
     if (rc) return rc;
     a.x = nullptr;
     a.behind = 1;
-    return fp4_matmul(codes, scales, wc, ws, M, N, fmt, a, st);
+    return fp4_matmul(codes, scales, wc, ws, M, N, fmt, a, status, st);
 }

@@ -884,11 +884,12 @@ int moe_bn(const MoeArgs& a, const void* w13, const void* w2, cudaStream_t st) {
 // [E, 2, I, D] mxfp4 (gate, up), w2 / s2 of [E, D, I]; out [T, D] (dtype odt, row stride ldo; accumulate: added to);
 // score 0 sqrt(softplus), 1 sigmoid, 2 softmax; norm: the chosen scores are divided by their sum; limit: SwiGLU clamp
 // (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: 4096 + min(E, T topk) ceil(I / 128) (128 BN
-// + 512) bytes, BN = 8 up to 8 tokens, 16 up to 16, else 32.
+// + 512) bytes, BN = 8 up to 8 tokens, 16 up to 16, else 32.  status: four words that a wait that ran out reports to, or null
+// for the device's own (fb_fp4_status).
 FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logits, int64_t ldl, const float* bias, const void* w13,
                       const void* s13, const void* w2, const void* s2, void* out, int64_t odt, int64_t ldo, int64_t accumulate,
                       void* work, int64_t T, int64_t E, int64_t topk, int64_t D, int64_t I, int64_t score, int64_t norm, float scale,
-                      float limit, cudaStream_t st) {
+                      float limit, int* status, cudaStream_t st) {
     if (T < 1 || T > kMaxTok || E < 1 || E > kMaxE || topk < 1 || topk > kMaxTopk || topk > E || D < 1 || I < 32 || I % 32 || ldx < D ||
         ldo < D || ldl < E || score < 0 || score > 2 || xdt < 0 || xdt > 2 || odt < 0 || odt > 2 || E * 2 * I > 0x7fffff00ll ||
         E * D > 0x7fffff00ll || D > 0x3fffff || (((uintptr_t)w13 | (uintptr_t)w2) & 31) ||
@@ -900,7 +901,7 @@ FB_API int fb_fp4_moe(const void* x, int64_t xdt, int64_t ldx, const float* logi
     a.scale = scale; a.limit = limit; a.xdt = (int)xdt; a.odt = (int)odt; a.accumulate = accumulate != 0;
     a.T = (int)T; a.E = (int)E; a.topk = (int)topk; a.D = (int)D; a.I = (int)I; a.score = (int)score; a.norm = norm != 0;
     a.g1 = (int)groups(D); a.nit = (int)((I + 127) / 128);
-    a.status = fp4_status_ptr();
+    a.status = status ? status : fp4_status_ptr();
     if (!a.status) return (int)cudaErrorNotSupported;
     // columns of the MMAs: the cost of an MMA does not depend on them, the room that x and h take in shared memory does
     const int64_t pairs = T * topk < E ? T * topk : E;

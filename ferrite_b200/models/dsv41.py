@@ -636,7 +636,7 @@ class Dsv41DeviceModel:
                         L["sh_w13"], xq.s, xq.ld, xq.plane, gu, gu.shape[1], 2 * self.Is, d, n)
             self.K.call("fb_d4_swiglu_clamp_quant", gu, gu.shape[1], hs.f, self.Is, n, self.Is, float(cfg.swiglu_limit), *hs.sp(1))
             fp4.moe(x.f[:n, :d], ws["rlogit"][:n, :E], L["moe2_w13"], L["moe2_w2"], topk, bias=L["gate_b"], score="sqrtsoftplus",
-                    norm=topk > 1, scale=float(cfg.route_scale), limit=max(0.0, float(cfg.swiglu_limit)), out=ws["y"][:n])
+                    norm=topk > 1, scale=float(cfg.route_scale), limit=max(0.0, float(cfg.swiglu_limit)), out=ws["y"][:n], status=self.tc_status)
             if not self.shared_tp:
                 self._reduce(ws["y"], n)
             if self.shared_tp or self.world == 1:

@@ -12,8 +12,12 @@ A block that holds an infinity or a NaN gets the NaN scale: all of its values, a
 
 All functions launch on the current stream of their operands' device, allocate with torch's allocator (nothing is kept
 between calls, so calls may overlap on several streams and be captured) and raise ``ValueError`` / ``TypeError`` for
-arguments they do not take and ``KernelError`` when CUDA refuses a launch.  A wait inside a kernel that ran out is
-reported by :func:`check`.
+arguments they do not take and ``KernelError`` when CUDA refuses a launch.
+
+A wait inside a product or an expert layer that ran out leaves the output unwritten and is reported in four int32 words
+``[code, block, kernel, split]``: in the ``status`` tensor that the call was given (a slice of a
+:class:`~ferrite_b200.parallel.status.StatusArena`, say, which an engine checks after every step), else in words that all
+such calls on a device share and :func:`check` reads.
 """
 from __future__ import annotations
 
@@ -243,6 +247,13 @@ def _out(out: Optional[torch.Tensor], shape, dtype: torch.dtype, device: torch.d
     return out, m
 
 
+def _status(status: Optional[torch.Tensor], device: torch.device) -> Optional[torch.Tensor]:
+    if status is not None and (status.dtype is not torch.int32 or status.dim() != 1 or status.numel() < 4 or status.stride(0) != 1
+                               or status.device != device):
+        raise ValueError(f"status must be four consecutive int32 words on {device}, got {status.dtype} {tuple(status.shape)} on {status.device}")
+    return status
+
+
 def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values of ``q``, rounded once to ``dtype`` (or into ``out``, whose rows may be strided)."""
     if not q.codes.is_cuda:
@@ -254,9 +265,10 @@ def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[
     return out
 
 
-def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
+           status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ w.T`` of two 4-bit matrices [M, K] and [N, K] of one format: products of the values they stand for, summed in
-    f32 and rounded once (to ``out_dtype``, or to the type of a given ``out``)."""
+    f32 and rounded once (to ``out_dtype``, or to the type of a given ``out``).  ``status``: see the module."""
     if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"matmul takes [M, K] and [N, K], got {x.shape} and {w.shape}")
     if x.fmt != w.fmt:
@@ -265,18 +277,19 @@ def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, 
         raise ValueError(f"matmul takes tensors of one CUDA device, got {x.device} and {w.device}")
     M, N, K = x.shape[0], w.shape[0], x.shape[1]
     alpha = _alpha(x.tensor_scale, w.tensor_scale)
+    status = _status(status, x.device)
     out, (_, _, _, _, ldo) = _out(out, (M, N), out_dtype, x.device, x.codes, x.scales, w.codes, w.scales)
     if M and N:
         _call(x.device, "fb_fp4_matmul", x.codes, x.scales, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
-              FORMATS[x.fmt], alpha)
+              FORMATS[x.fmt], alpha, status)
     return out
 
 
 def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None,
-           x_scale: Optional[float] = None) -> torch.Tensor:
+           x_scale: Optional[float] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``quantize(x, w.fmt, x_scale) @ w.T`` for ``x`` [M, K] (f32, bf16, f16) and 4-bit weights [N, K], in one call
     (a few short rows in one launch, else two).  ``out_dtype`` defaults to x's; a given ``out`` keeps its own type and must
-    not share memory with an operand."""
+    not share memory with an operand.  ``status``: see the module."""
     if x.dim() != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"linear takes [M, K] and 4-bit [N, K], got {tuple(x.shape)} and {w.shape}")
     if x_scale is not None:
@@ -286,6 +299,7 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
     dev = x.device
     if dev != w.device:
         raise ValueError(f"x is on {dev}, w on {w.device}")
+    status = _status(status, dev)
     N = w.shape[0]
     if out is None:
         out, ldo = torch.empty(M, N, dtype=out_dtype or x.dtype, device=dev), N
@@ -300,7 +314,7 @@ def linear(x: torch.Tensor, w: Fp4Tensor, out_dtype: Optional[torch.dtype] = Non
             work = torch.empty((M * 64 * g + 511) // 512 * 512 + (M + 127) // 128 * (g if w.fmt == "mxfp4" else 2 * g) * 512,
                                dtype=torch.uint8, device=dev)
         _call(dev, "fb_fp4_linear", x, _DTYPES[x.dtype], ldx, work, w.codes, w.scales, out, _DTYPES[out.dtype], ldo, M, N, K,
-              FORMATS[w.fmt], float(x_scale or 0.0), alpha)
+              FORMATS[w.fmt], float(x_scale or 0.0), alpha, status)
     return out
 
 
@@ -310,7 +324,8 @@ MOE_MAX_TOKENS, MOE_MAX_EXPERTS, MOE_MAX_TOPK, MOE_MAX_DIM = 32, 512, 32, 8192
 
 def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, topk: int, *, bias: Optional[torch.Tensor] = None,
         score: str = "sqrtsoftplus", norm: bool = True, scale: float = 1.0, limit: float = 0.0,
-        out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
+        out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, accumulate: bool = False,
+        status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The routed experts of a layer for up to 32 tokens, in two kernels.
 
     ``x`` [T, D] (f32, bf16, f16), ``logits`` [T, E] f32 of the router, ``w13`` mxfp4 [E, 2, I, D] (gate, up), ``w2`` mxfp4
@@ -321,7 +336,7 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     ``silu(min(g, limit)) * clamp(u, -limit, limit) * weight`` before the down product (``limit`` 0: no clamp).  The
     result, summed in f32, is rounded once to ``out_dtype`` (default: x's) or, with ``accumulate``, added to ``out``, which
     may be x.  A NaN in a token stays in that token's row; a NaN scale in ``w2`` reaches every row of a call in which any token
-    takes that expert (all experts share one accumulator), so ``w2`` should hold none."""
+    takes that expert (all experts share one accumulator), so ``w2`` should hold none.  ``status``: see the module."""
     if score not in SCORES:
         raise ValueError(f"score must be one of {sorted(SCORES)}, got {score!r}")
     if w13.fmt != "mxfp4" or w2.fmt != "mxfp4":
@@ -352,6 +367,7 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     dev = w13.device
     if any(t is not None and t.device != dev for t in (x, logits, bias, w2.codes)):
         raise ValueError("moe takes tensors of one device")
+    status = _status(status, dev)
     _, _, _, _, ldx = _matrix(x, "x")
     out, (_, _, _, _, ldo) = _out(out, (T, D), out_dtype or x.dtype, dev, w13.codes, w13.scales, w2.codes, w2.scales)
     if T:
@@ -359,13 +375,14 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
         work = torch.empty(4096 + min(E, T * topk) * ((I + 127) // 128) * tile, dtype=torch.uint8, device=dev)
         _call(dev, "fb_fp4_moe", x, _DTYPES[x.dtype], ldx, logits, logits.stride(0) if T > 1 else E, bias, w13.codes, w13.scales,
               w2.codes, w2.scales, out, _DTYPES[out.dtype], ldo, int(accumulate), work, T, E, topk, D, I, SCORES[score], int(norm),
-              float(scale), float(limit) if limit else math.inf)
+              float(scale), float(limit) if limit else math.inf, status)
     return out
 
 
 def check(device=None) -> None:
-    """Raise ``KernelError`` if a wait inside one of this module's kernels on ``device`` (default: the current one) ran
-    out since the last check.  Waits for the current stream."""
+    """Raise ``KernelError`` if a wait inside one of this module's kernels on ``device`` (default: the current one) that was
+    given no ``status`` ran out since the last check.  Waits for the current stream alone, and clears the words for every
+    caller on the device: calls that have to be told apart get a ``status`` of their own."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     host = (ctypes.c_int * 4)()
     with torch.cuda.device(dev):

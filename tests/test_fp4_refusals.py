@@ -192,3 +192,27 @@ def test_from_rows_copies_bytes_on_any_boundary():
     assert torch.equal(t.codes, before) and before.any()
     u = t.to("cpu")
     assert u.shape == t.shape and torch.equal(u.codes, t.codes) and torch.equal(u.scales, t.scales)
+
+
+@pytest.mark.parametrize("status", [torch.zeros(4), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 4, dtype=torch.int32),
+                                    torch.zeros(8, dtype=torch.int32)[::2], torch.zeros(4, dtype=torch.int32, device="meta")])
+def test_status_words_that_are_refused(status, monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    for call in (lambda: fp4.matmul(_t(4, 64), _t(8, 64), status=status), lambda: fp4.linear(torch.zeros(4, 64), _t(8, 64), status=status),
+                 lambda: fp4.moe(*_moe_args(), status=status)):
+        with pytest.raises(ValueError, match="status must be"):
+            call()
+
+
+def test_status_words_reach_the_kernels(monkeypatch):
+    """A given tensor, or nothing, is what the entry point is handed behind its last number."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    seen = []
+    monkeypatch.setattr(fp4, "_call", lambda device, name, *args: seen.append((name, args[-1])))
+    own = torch.zeros(12, dtype=torch.int32)[4:8]
+    for status in (own, None):
+        fp4.matmul(_t(4, 64), _t(8, 64), status=status)
+        fp4.linear(torch.zeros(4, 64), _t(8, 64), status=status)
+        fp4.moe(*_moe_args(), status=status)
+    assert [n for n, _ in seen] == ["fb_fp4_matmul", "fb_fp4_linear", "fb_fp4_moe"] * 2
+    assert all(s is own for _, s in seen[:3]) and all(s is None for _, s in seen[3:])

@@ -33,3 +33,45 @@ def test_expanded_weights_of_a_gemv_with_early_starts():
             assert torch.equal(out, want)
     finally:
         K.lib.fb_set_pdl(0)
+
+
+def test_a_wait_that_ran_out_in_the_expert_layer_fails_the_engine_s_step(monkeypatch):
+    """The report of an expired wait, put into the words that the expert layer was given (by the host: nothing hangs), raises on
+    the step that caused it, and the next step is clean."""
+    from ferrite_b200.engine.dsv41_engine import Dsv41Engine
+    from ferrite_b200.models.dsv41 import DictWeights
+    from ferrite_b200.models.dsv41_config import Dsv41Config
+    from ferrite_b200.models.dsv41_weights import random_weights
+    from ferrite_b200.parallel.status import CollectiveTimeout, FB_TIMEOUT
+    from ferrite_b200.utils.switches import Switches, set_switches
+    cfg = Dsv41Config.tiny()
+    try:
+        set_switches(Switches(d4_moe_two=True))
+        eng = Dsv41Engine(cfg, DictWeights(random_weights(cfg, 4)), max_ctx=128, use_graphs=False)
+        eng.prefill([5, 9, 2, 7])
+        eng.step_plain()
+        real, expired = fp4.moe, []
+
+        def moe(*args, **kw):
+            y = real(*args, **kw)
+            if not expired:
+                kw["status"][:4].copy_(torch.tensor([FB_TIMEOUT, 3, 1008, 2], dtype=torch.int32))
+                expired.append(1)
+            return y
+
+        monkeypatch.setattr(fp4, "moe", moe)
+        with pytest.raises(CollectiveTimeout):
+            eng.step_plain()
+        assert expired
+        eng.step_plain()
+    finally:
+        set_switches(None)
+
+
+def test_a_call_writes_no_status_when_nothing_ran_out():
+    w = fp4.quantize(torch.randn(64, 256).cuda())
+    status = torch.zeros(4, dtype=torch.int32, device="cuda")
+    x = torch.randn(3, 256).cuda()
+    assert torch.equal(fp4.linear(x, w, status=status), fp4.linear(x, w))
+    assert torch.equal(fp4.matmul(fp4.quantize(x), w, status=status), fp4.linear(x, w, out_dtype=torch.bfloat16))
+    assert status.tolist() == [0, 0, 0, 0]
