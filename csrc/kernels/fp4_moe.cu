@@ -77,23 +77,6 @@ __device__ __forceinline__ float score_of(float z, int score, float mx, float in
     return sqrtf(fmaxf(z, 0.f) + log1pf(expf(-fabsf(z))));
 }
 
-// The score for the choice: as score_of within a few units in the last place, in a third of its instructions (every expert of
-// every token takes one).  log1p(e) = 2 atanh(e / (2 + e)), the series to the 13th power: 5e-9 at e = 1.
-__device__ __forceinline__ float key_score(float z, int score, float mx, float inv_sum) {
-    if (score == kSigmoid) return __fdividef(1.f, 1.f + __expf(-z));
-    if (score == kSoftmax) return __expf(z - mx) * inv_sum;
-    const float e = __expf(-fabsf(z)), s = __fdividef(e, 2.f + e), q = s * s;
-    float p = fmaf(q, 1.f / 13.f, 1.f / 11.f);
-    p = fmaf(q, p, 1.f / 9.f);
-    p = fmaf(q, p, 1.f / 7.f);
-    p = fmaf(q, p, 1.f / 5.f);
-    p = fmaf(q, p, 1.f / 3.f);
-    p = fmaf(q, p, 1.f);
-    float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(fmaf(2.f * s, p, fmaxf(z, 0.f))));
-    return r;
-}
-
 // Routing.  Every CTA does it once, before its first weight arrives: what counts is the length of the dependent chain and
 // the size of the code (straight-line code that runs once costs its instruction fetches: with the scores unrolled over a
 // lane's 16 experts it took 30 us for one token), so the score loops are rolled and the selection is a tree over registers.
@@ -128,7 +111,7 @@ __device__ __forceinline__ void route_keys(const MoeArgs& a, const Route& r, con
     const float mx = r.mx[t], inv = r.inv[t];
 #pragma unroll 1
     for (int e = first; e < a.E; e += step)
-        reinterpret_cast<uint32_t*>(keys)[e] = order_key(key_score(row[e], a.score, mx, inv) + bias[e]);
+        reinterpret_cast<uint32_t*>(keys)[e] = order_key(score_of(row[e], a.score, mx, inv) + bias[e]);
 }
 // The token's choice from its row of keys (or, without a bias, of logits); z: its logits.  One warp.
 __device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const float* row, const volatile float* z, int t, int lane) {
