@@ -149,7 +149,10 @@ __device__ __forceinline__ void route_pick(const MoeArgs& a, Route& r, const flo
             if (gone >> j & 1) key[j] = 0u;
     }
     p = lane < a.topk ? score_of(p, a.score, r.mx[t], r.inv[t]) : 0.f;
-    if (a.norm) p = p / (warp_sum(p) + 1e-20f);
+    if (a.norm) {   // scores are not negative: a sum of zero is all of them zero
+        const float sum = warp_sum(p);
+        p = sum == 0.f ? 0.f : p / sum;
+    }
     if (lane < a.topk) {
         r.sel[t * kMaxTopk + lane] = (uint16_t)mine;
         r.wt[t * kMaxTopk + lane] = p * a.scale;
@@ -865,7 +868,7 @@ int moe_bn(const MoeArgs& a, const void* w13, const void* w2, cudaStream_t st) {
 
 // x [T, D] (dtype xdt, row stride ldx), logits f32 [T, E] (row stride ldl), bias f32 [E] or null; w13 codes / s13 scales of
 // [E, 2, I, D] mxfp4 (gate, up), w2 / s2 of [E, D, I]; out [T, D] (dtype odt, row stride ldo; accumulate: added to);
-// score 0 sqrt(softplus), 1 sigmoid, 2 softmax; norm: the chosen scores are divided by their sum; limit: SwiGLU clamp
+// score 0 sqrt(softplus), 1 sigmoid, 2 softmax; norm: the chosen scores are divided by their sum (all zero stay zero); limit: SwiGLU clamp
 // (infinity: none).  T <= 32, E <= 512, topk <= min(E, 32), I % 32 == 0.  work: 4096 + min(E, T topk) ceil(I / 128) (128 BN
 // + 512) bytes, BN = 8 up to 8 tokens, 16 up to 16, else 32.  status: four words that a wait that ran out reports to, or null
 // for the device's own (fb_fp4_status).

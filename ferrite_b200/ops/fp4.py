@@ -331,7 +331,7 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
     ``x`` [T, D] (f32, bf16, f16), ``logits`` [T, E] f32 of the router, ``w13`` mxfp4 [E, 2, I, D] (gate, up), ``w2`` mxfp4
     [E, D, I] (I a multiple of 32).  Every token takes the ``topk`` experts of largest ``score(logits) + bias``, computed and
     added in f32 (ties and equal logits to the lower index; NaN below every number; without a bias the logits decide), weighted by
-    ``scale * score``, with ``norm`` divided by the sum of the chosen scores.  Activations meet the weights as e4m3 with a
+    ``scale * score``, with ``norm`` divided by the sum of the chosen scores (scores that are all zero in f32 stay zero).  Activations meet the weights as e4m3 with a
     power-of-two scale per 32 values (``ops/quant.py::fp8_act_roundtrip``): x before the gate and up products, and
     ``silu(min(g, limit)) * clamp(u, -limit, limit) * weight`` before the down product (``limit`` 0: no clamp).  The
     result, summed in f32, is rounded once to ``out_dtype`` (default: x's) or, with ``accumulate``, added to ``out``, which
