@@ -23,6 +23,16 @@ class KernelError(RuntimeError):
 
 
 _Tensor = torch.Tensor
+_NUMBERS = frozenset((int, float, bool, type(None)))
+
+
+def _argument(a, name: str):
+    """What a call hands to ctypes for an argument that is neither a plain tensor nor a plain number."""
+    if hasattr(a, "data_ptr"):      # a View, a Parameter
+        return a.data_ptr()
+    if isinstance(a, (int, float, ctypes._SimpleCData, ctypes.Array, ctypes._Pointer)):
+        return a
+    raise TypeError(f"{name}: unsupported argument {type(a)}")
 
 
 class KernelLib:
@@ -58,7 +68,7 @@ class KernelLib:
         rc = None
         if fast is not None:   # argument kinds are known from the first call: ctypes converts plain numbers by itself
             try:
-                rc = fast(*[a.data_ptr() if type(a) is _Tensor else a for a in args], stream)
+                rc = fast(*[a.data_ptr() if type(a) is _Tensor else a if type(a) in _NUMBERS else _argument(a, name) for a in args], stream)
             except ctypes.ArgumentError:
                 rc = None
         if rc is None:
