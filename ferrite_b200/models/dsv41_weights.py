@@ -155,17 +155,32 @@ def tensor_specs_cached(cfg: Dsv41Config) -> Dict[str, Spec]:
     return tensor_specs(cfg)
 
 
-def estimate_device_bytes(cfg: Dsv41Config, world: int = 1) -> int:
+def moe_two_bytes(cfg: Dsv41Config, world: int = 1) -> int:
+    """Bytes that the two-kernel expert layer (switch ``d4_moe_two``) keeps on a rank beside the experts themselves: their
+    scales once more, in chunks of 128 rows x 4 blocks, and the down codes once more where their rows are no whole 128-column
+    groups (576 columns at TP = 4: 320 bytes a row beside the 288)."""
+    Il, d = padded_inter(cfg, world) if world > 1 else cfg.moe_inter_dim, cfg.dim
+    ti, td = (Il + 127) // 128, (d + 127) // 128
+    per_expert = 3 * ti * td * 512 + (d * 64 * ti if Il % 128 else 0)
+    layers = range(cfg.n_layers + cfg.n_mtp_layers)
+    return sum(cfg.moe_shape(l)[0] for l in layers) * per_expert
+
+
+def estimate_device_bytes(cfg: Dsv41Config, world: int = 1, moe_two: Optional[bool] = None) -> int:
     """Weight bytes one rank of a `world`-way tensor-parallel device model holds: e2m1 experts with their ue8m0 scales
     (17 / 32 byte per value), engram tables as e4m3 bytes, dense and bf16 tensors as bf16 (dense e4m3 weights are
-    expanded at load), f32 vectors; sharded tensors count 1 / world.  Caches and workspaces come on top (a few GB)."""
+    expanded at load), f32 vectors; sharded tensors count 1 / world; what the two-kernel expert layer keeps beside them, if
+    `moe_two` (default: the switch).  Caches and workspaces come on top (a few GB)."""
     import math
+    from ..utils.switches import switches
     per = {"expert": (17 / 32) if cfg.expert_dtype == "fp4" else 2.0, "table": 1.0, "dense": 2.0, "bf16": 2.0, "f32": 4.0,
            "fp4": 17 / 32, "fp8": 2.0}
     total = 0.0
     for spec in tensor_specs_cached(cfg).values():
         n = math.prod(spec.shape) * per.get(spec.kind, 4.0)
         total += n / world if spec.shard is not None else n
+    if switches().d4_moe_two if moe_two is None else moe_two:
+        total += moe_two_bytes(cfg, world)
     return int(total)
 
 

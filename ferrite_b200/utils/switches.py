@@ -50,7 +50,11 @@ class Switches:
                                     # (16: two 8-row windows per launch site, 80 launches fewer per 16-row tick but 15.9 vs 15.5 ms)
     d4_fp4_mma: bool = True         # DSV41 routed experts of decode rows on the tensor cores
     d4_moe_two: bool = False        # DSV41 routed experts of decode rows as the two-kernel layer of ops/fp4.py (routing inside,
-                                    # weights unpacked by TMA); the expert weights then keep the checkpoint's byte order
+                                    # weights unpacked by TMA).  The expert weights then keep the checkpoint's byte order, so
+                                    # rows that the layer does not take (a forward with images, more than 32 rows without the
+                                    # grouped product) run the per-pair expert kernels without the tensor core; and their
+                                    # scales, at widths that are no multiple of 128 the down codes too, are kept twice
+                                    # (dsv41_weights.py::moe_two_bytes: 31 GB a rank at TP = 4, 18 GB at TP = 8)
     d4_attn_tc: bool = False        # DSV41 tensor-core sparse attention (slower than the SIMT kernel at decode sizes)
     d4_fuse_quant: bool = False     # DSV41 activation quantiser fused into hc_pre (a one-CTA latency chain; slower)
     dump_dir: str = ""              # directory for unit dumps ("" = off)

@@ -75,3 +75,22 @@ def test_a_call_writes_no_status_when_nothing_ran_out():
     assert torch.equal(fp4.linear(x, w, status=status), fp4.linear(x, w))
     assert torch.equal(fp4.matmul(fp4.quantize(x), w, status=status), fp4.linear(x, w, out_dtype=torch.bfloat16))
     assert status.tolist() == [0, 0, 0, 0]
+
+
+def test_what_the_expert_layer_keeps_twice_is_what_the_estimate_counts():
+    from ferrite_b200.models.dsv41 import DictWeights, Dsv41DeviceModel
+    from ferrite_b200.models.dsv41_config import Dsv41Config
+    from ferrite_b200.models.dsv41_weights import moe_two_bytes, random_weights
+    from ferrite_b200.utils.switches import Switches, set_switches
+    cfg = Dsv41Config.tiny()
+    try:
+        set_switches(Switches(d4_moe_two=True))
+        dev = Dsv41DeviceModel(cfg, DictWeights(random_weights(cfg, 4)), max_rows=8, max_ctx=128)
+    finally:
+        set_switches(None)
+    kept = 0
+    for L in dev.layers + [m for m in dev.mtp]:
+        assert L["moe2"] and L["moe2_w13"].codes.data_ptr() == L["w13"].data_ptr()
+        kept += L["moe2_w13"].scales.numel() + L["moe2_w2"].scales.numel()
+        kept += L["moe2_w2"].codes.numel() if L["moe2_w2"].codes.data_ptr() != L["w2"].data_ptr() else 0
+    assert kept == moe_two_bytes(cfg)
