@@ -255,7 +255,8 @@ def _status(status: Optional[torch.Tensor], device: torch.device) -> Optional[to
 
 
 def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The values of ``q``, rounded once to ``dtype`` (or into ``out``, whose rows may be strided)."""
+    """The values of ``q``, rounded to ``dtype`` (or into ``out``, whose rows may be strided): once without a tensor scale
+    (code times block scale is exact in f32); with one, their f32 product with the scale, rounded to f32, is."""
     if not q.codes.is_cuda:
         raise ValueError("q is not on a CUDA device")
     out, (batch, rows, cols, bs, ld) = _out(out, q.shape, dtype, q.device, q.codes, q.scales)
@@ -268,7 +269,8 @@ def dequantize(q: Fp4Tensor, dtype: torch.dtype = torch.bfloat16, out: Optional[
 def matmul(x: Fp4Tensor, w: Fp4Tensor, out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None,
            status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ w.T`` of two 4-bit matrices [M, K] and [N, K] of one format: products of the values they stand for, summed in
-    f32 and rounded once (to ``out_dtype``, or to the type of a given ``out``).  ``status``: see the module."""
+    f32, multiplied in f32 by the product of their tensor scales (itself rounded to f32) and rounded to ``out_dtype``, or to the
+    type of a given ``out``.  ``status``: see the module."""
     if len(x.shape) != 2 or len(w.shape) != 2 or x.shape[1] != w.shape[1]:
         raise ValueError(f"matmul takes [M, K] and [N, K], got {x.shape} and {w.shape}")
     if x.fmt != w.fmt:

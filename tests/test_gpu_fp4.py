@@ -343,3 +343,19 @@ def test_offsets_past_32_bits():
     for rows in (slice(0, 256), slice(t0, R)):
         assert torch.equal(y[rows], fp4.linear(xs[rows].contiguous(), w))
     fp4.check()
+
+
+def test_a_tensor_scale_is_multiplied_in_f32_before_the_rounding_to_16_bits():
+    """A value whose product with the scale lies 2e-6 of a step below the middle of two bf16: its f32 rounding is the middle,
+    which goes to the even neighbour above.  (Rounded once it would be the one below.)"""
+    ts, v = 0.04430042579770088, 0.0859375
+    assert float(torch.tensor(ts)) == ts
+    scale = torch.zeros(1, 1, 1, 512, dtype=torch.uint8)
+    scale[..., 0] = torch.tensor(v * 2).to(torch.float8_e4m3fn).view(torch.uint8)
+    codes = torch.zeros(1, 64, dtype=torch.uint8)
+    codes[0, 0] = 1                                                                     # 0.5
+    q = fp4.Fp4Tensor(codes.cuda(), torch.cat([scale, torch.zeros_like(scale)], 2)[0].cuda(), "nvfp4", (1, 16), ts)
+    assert float(fp4.reference_dequantize(q)[0, 0]) == v * ts
+    assert float(fp4.dequantize(q, torch.float32)[0, 0]) == float(torch.tensor(v) * torch.tensor(ts))
+    below, above = 0.0037994384765625, 0.003814697265625
+    assert v * ts < (below + above) / 2 and float(fp4.dequantize(q)[0, 0]) == above
