@@ -33,6 +33,7 @@ from .quant import e2m1_unpack
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_F32_MAX = torch.finfo(torch.float32).max
 LINEAR_INSIDE = 32   # 128-column groups of one row that fb_fp4_linear always quantises inside the product
 
 
@@ -358,8 +359,8 @@ def moe(x: torch.Tensor, logits: torch.Tensor, w13: Fp4Tensor, w2: Fp4Tensor, to
                          f"got {T}, {E}, {topk}")
     if D > MOE_MAX_DIM:
         raise ValueError(f"moe takes rows of up to {MOE_MAX_DIM} values, got {D}")
-    if not (limit >= 0.0) or not math.isfinite(scale):
-        raise ValueError(f"limit must not be negative and scale must be finite, got {limit}, {scale}")
+    if not (limit >= 0.0) or not abs(scale) <= _F32_MAX:
+        raise ValueError(f"limit must not be negative and scale must be finite in f32, got {limit}, {scale}")
     if logits.dtype != torch.float32 or tuple(logits.shape) != (T, E) or (E > 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < E):
         raise ValueError(f"logits must be f32 {(T, E)} with rows of consecutive values, got {logits.dtype} {tuple(logits.shape)} {logits.stride()}")
     if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,) or not bias.is_contiguous()):

@@ -216,3 +216,9 @@ def test_status_words_reach_the_kernels(monkeypatch):
         fp4.moe(*_moe_args(), status=status)
     assert [n for n, _ in seen] == ["fb_fp4_matmul", "fb_fp4_linear", "fb_fp4_moe"] * 2
     assert all(s is own for _, s in seen[:3]) and all(s is None for _, s in seen[3:])
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, float("nan"), float("-inf")])
+def test_a_scale_that_f32_does_not_hold(scale):
+    with pytest.raises(ValueError, match="finite"):
+        fp4.moe(*_moe_args(), scale=scale)
