@@ -191,13 +191,17 @@ int* fp4_status_ptr() {
     return p;
 }
 
-// The status words of the current device's 4-bit kernels into host[4], and zeroed if `clear`; waits for the stream.
+// The status words of the current device's 4-bit kernels into host[4]; waits for the stream.  With `clear` they are zeroed if they
+// report something: a report that another stream's kernel makes after the copy stays for the next call.
 FB_API int fb_fp4_status(int* host, int64_t clear, cudaStream_t st) {
     int* p = fp4_status_ptr();
     if (!p) return (int)cudaErrorNotSupported;
     cudaError_t e = cudaMemcpyAsync(host, p, 16, cudaMemcpyDeviceToHost, st);
-    if (e == cudaSuccess && clear) e = cudaMemsetAsync(p, 0, 16, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess && clear && host[0]) {
+        e = cudaMemsetAsync(p, 0, 16, st);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    }
     return (int)e;
 }
 

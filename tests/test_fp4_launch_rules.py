@@ -39,3 +39,11 @@ def test_the_expander_lets_nothing_start_early():
     bodies = dict(kernel_bodies("fp4.cu"))
     assert "pdl_launch" in bodies["fp4_quantize_kernel"] and "pdl_wait();" in bodies["fp4_dequantize_kernel"]
     assert "pdl_launch" not in bodies["fp4_dequantize_kernel"]
+
+
+def test_reading_the_status_words_erases_no_report_that_it_has_not_seen():
+    text = re.sub(r"//[^\n]*", "", (KERNELS / "fp4.cu").read_text())
+    body = text[text.index("FB_API int fb_fp4_status"):]
+    body = body[:body.index("\n}")]
+    clear = body.index("cudaMemsetAsync")
+    assert body.index("cudaStreamSynchronize") < clear and "host[0]" in body[:clear]

@@ -94,3 +94,15 @@ def test_what_the_expert_layer_keeps_twice_is_what_the_estimate_counts():
         kept += L["moe2_w13"].scales.numel() + L["moe2_w2"].scales.numel()
         kept += L["moe2_w2"].codes.numel() if L["moe2_w2"].codes.data_ptr() != L["w2"].data_ptr() else 0
     assert kept == moe_two_bytes(cfg)
+
+
+def test_the_words_of_check_are_clean_after_ordinary_calls():
+    """Read without and with clearing them."""
+    import ctypes
+    w = fp4.quantize(torch.randn(64, 256).cuda())
+    fp4.linear(torch.randn(3, 256).cuda(), w)
+    host = (ctypes.c_int * 4)(7, 7, 7, 7)
+    for clear in (0, 1):
+        _lib.lib().call("fb_fp4_status", ctypes.cast(host, ctypes.POINTER(ctypes.c_int)), clear)
+        assert list(host) == [0, 0, 0, 0]
+    fp4.check()
