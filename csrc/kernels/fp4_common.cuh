@@ -130,6 +130,22 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+// End of a producer of a ring of stages: its copies have landed, whatever the other warps came to (after a wait that ran out the CTA
+// would end with copies on their way into its shared memory; without one they have landed long before).  full0: the first stage's
+// barrier; s, round: where the next block would go.  step 1: one producer.  step 2: two that take every other block; this one
+// has issued (round stages + s) / 2 blocks, and of these only the last stages / 2 are looked at: a stage further back may be the
+// other one's by now, whose phases would be taken for its own.  That one alone is looked at after a failure, when nothing more is
+// issued and a wait in vain costs its budget.
+__device__ __forceinline__ bool drain_ring(uint32_t full0, int stages, int s, int round, int step, bool ok) {
+    const int issued = (round * stages + s) / step;
+    for (int i = 0; i < issued && i < (stages + (ok ? 0 : step - 1)) / step; ++i) {
+        s -= step;
+        if (s < 0) { s += stages; --round; }
+        if (!tc::mbar_wait(full0 + 8u * s, round & 1)) return false;
+    }
+    return true;
+}
+
 // Tiled TMA store of a box in shared memory (clipped at the tensor's ends) and its bulk groups (per thread).
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, int x, int y, uint32_t smem_src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(smem_src) : "memory");

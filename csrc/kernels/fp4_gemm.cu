@@ -358,6 +358,7 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                     if (++s == C::kStages) { s = 0; ++round; }
                 }
             }
+            if (!drain_ring(full(0), C::kStages, s, round, 1, ok)) atomicExch(&s_fail, 1);
         }
     } else if (warp == 1) {
         if (elect_one()) {
@@ -611,6 +612,8 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
                     if (++s == C::kStages) { s = 0; ++round; }
                 }
             }
+            // (rank 0's barriers count both CTAs' copies, and rank 1 stays until rank 0 is through)
+            if (rank == 0 && !drain_ring(full(0), C::kStages, s, round, 1, ok)) atomicExch(&s_fail, 1);
         }
     } else if (warp == 1) {
         if (elect_one()) {

@@ -460,6 +460,7 @@ fp4_moe_up_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_const
                     }
                 }
             }
+            if (!drain_ring(full(0), stages, s, round, 2, ok)) atomicExch(&s_fail, 1);
         }
     } else if (warp == 1) {
         if (elect_one()) {
@@ -659,8 +660,9 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
         if (elect_one()) {   // two producers, every other block each, as in kernel 1
             const int mine = warp == 6;
             int u = u0 + mine, ai = u / a.nit, kb = u - ai * a.nit, s = mine, round = 0;
+            bool ok = true;
             for (; u < u1; u += 2) {
-                if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); break; }
+                if (round && !tc::mbar_wait(empty(s), (round - 1) & 1)) { atomicExch(&s_fail, 1); ok = false; break; }
                 const uint32_t st = base + (uint32_t)s * C::kStage;
                 const int e = s_act[ai];
                 tc::mbar_expect_tx(full(s), 128 * 64 + 512 + BN * 128 + 512);
@@ -673,6 +675,7 @@ fp4_moe_down_kernel(const __grid_constant__ CUtensorMap tmap_w, const MoeArgs a)
                 s += 2;
                 if (s >= C::kStages) { s -= C::kStages; ++round; }
             }
+            if (!drain_ring(full(0), C::kStages, s, round, 2, ok)) atomicExch(&s_fail, 1);
         }
     } else if (warp == 1) {
         if (elect_one()) {
