@@ -74,6 +74,8 @@ __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uin
                      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
 }
 
+enum Stores : int { kByElement = 0, kTma = 1, kTmaButTheEnd = 2 };   // of P = X
+
 struct GemmArgs {
     const uint8_t *sfp, *sfq;
     const void* x;            // QX: the rows to quantise (row stride ldx, element type xdt; tensor scale xts if scaled)
@@ -84,7 +86,7 @@ struct GemmArgs {
     int64_t ldo;
     int64_t P, Q, K;
     float alpha;
-    int dtype, vec, tiles_p, tiles_q, splits;
+    int dtype, vec /* Stores */, tiles_p, tiles_q, splits;
     int behind;               // the kernel before this one is the quantiser of X, and everything before that is complete
     int* status;
 };
@@ -115,7 +117,8 @@ __device__ __forceinline__ void store_columns(const GemmArgs& a, uint32_t tmem, 
 // P = X: a lane holds a row's outputs side by side.  They go through two buffers of 32 rows x ROW bytes of this warp
 // (16-byte units swizzled as in TMA's 128- or 64-byte mode) and leave as TMA stores, which the tensor core does not wait
 // for: the accumulator is given back as soon as it is read.  Rows that TMA cannot address (base or row stride not a
-// multiple of 16 bytes) leave as stores of 32 neighbouring outputs.
+// multiple of 16 bytes) leave as stores of 32 neighbouring outputs, and so does the buffer in which a row ends inside a 16-byte
+// unit: TMA clips a box at whole units, and what is behind the row's end is not the output's.
 template <typename T, int BN, int ROW, bool PAIR = false>
 __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap* tmap_o, uint32_t tmem, uint32_t buf0, int warp, int lane,
                                            int64_t p0, int64_t q0, uint32_t acc_empty, int& turn) {
@@ -152,7 +155,7 @@ __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap*
             }
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + unit(lane, u)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         }
-        if (a.vec) {
+        if (a.vec == kTma || (a.vec == kTmaButTheEnd && (q + kCols <= a.Q || q >= a.Q))) {
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -176,6 +179,7 @@ __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap*
                 }
             }
             __syncwarp();
+            if (lane == 0) bulk_commit();   // an empty group: the wait above counts buffers
         }
     }
 }
@@ -830,7 +834,7 @@ static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void
         (fmt != kMxFp4 && fmt != kNvFp4) || (((uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws) & 15))
         return (int)cudaErrorInvalidValue;
     const int esz = a.dtype == kF32 ? 4 : 2;
-    a.vec = ((uintptr_t)a.out & 15) == 0 && a.ldo * esz % 16 == 0;
+    a.vec = ((uintptr_t)a.out & 15) || a.ldo * esz % 16 ? kByElement : N * esz % 16 ? kTmaButTheEnd : kTma;
     a.status = status ? status : fp4_status_ptr();
     if (!a.status) return (int)cudaErrorNotSupported;
     return fmt == kMxFp4 ? gemm_fmt<kMxFp4>(a, xc, (const uint8_t*)xs, wc, (const uint8_t*)ws, M, N, st)

@@ -106,3 +106,20 @@ def test_the_words_of_check_are_clean_after_ordinary_calls():
         _lib.lib().call("fb_fp4_status", ctypes.cast(host, ctypes.POINTER(ctypes.c_int)), clear)
         assert list(host) == [0, 0, 0, 0]
     fp4.check()
+
+
+@pytest.mark.parametrize("M,N,K", [(150, 1111, 96), (333, 1111, 1000), (700, 4097, 160), (1200, 4609, 160), (20, 1111, 96)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_outputs_that_end_inside_a_unit_of_an_aligned_buffer(M, N, K, dtype):
+    """Rows that TMA can address (a 16-byte base and row stride) whose last column lies inside a 16-byte unit: what is behind it, and
+    the rows around, stay as they were."""
+    g = torch.Generator().manual_seed(N)
+    a, b = fp4.quantize(torch.randn(M, K, generator=g).cuda(), "nvfp4"), fp4.quantize(torch.randn(N, K, generator=g).cuda(), "nvfp4")
+    want = fp4.matmul(a, b, dtype)
+    wide = torch.full((M + 2, -(-N // 8) * 8 + 24), 5.0, dtype=dtype, device="cuda")
+    out = wide[1:M + 1, 8:N + 8]
+    assert out.data_ptr() % 16 == 0 and out.stride(0) * out.element_size() % 16 == 0
+    fp4.matmul(a, b, out=out)
+    fp4.check()
+    assert torch.equal(out, want)
+    assert (wide[0] == 5).all() and (wide[-1] == 5).all() and (wide[:, :8] == 5).all() and (wide[:, N + 8:] == 5).all()
