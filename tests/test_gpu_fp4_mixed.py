@@ -123,3 +123,46 @@ def test_outputs_that_end_inside_a_unit_of_an_aligned_buffer(M, N, K, dtype):
     fp4.check()
     assert torch.equal(out, want)
     assert (wide[0] == 5).all() and (wide[-1] == 5).all() and (wide[:, :8] == 5).all() and (wide[:, N + 8:] == 5).all()
+
+
+def test_a_matrix_times_itself():
+    for n in (50, 300):
+        q = fp4.quantize(torch.randn(n, 448, generator=torch.Generator().manual_seed(n)).cuda(), "mxfp4")
+        y = fp4.matmul(q, q, torch.float32)
+        v = fp4.reference_dequantize(q)
+        assert ((y.double() - v @ v.t()).abs() <= 450 * 2.0 ** -24 * (v.abs() @ v.abs().t())).all()
+
+
+def test_the_widest_routing_and_two_graphs_of_one_pool():
+    """512 experts, 32 tokens with 32 experts each and a bias: the routing's scratch fills the stages; captured twice into one
+    pool, replayed in turn."""
+    from test_gpu_fp4_moe import check_close, experts, ref_moe, spread_logits
+    T, E, D, I, topk = 32, 512, 256, 32, 32
+    w13, w2 = experts(E, D, I, 31)
+    g = torch.Generator().manual_seed(32)
+    x, logits = torch.randn(T, D, generator=g).cuda(), spread_logits(T, E, 33).cuda()
+    bias = (torch.randperm(E, generator=g).float() * 0.37 / E).cuda()
+    want = fp4.moe(x, logits, w13, w2, topk, bias=bias)
+    check_close(want, *ref_moe(x, logits, w13, w2, topk, bias=bias), torch.float32)
+    pool, graphs = torch.cuda.graph_pool_handle(), []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, pool=pool):
+            y = fp4.moe(x, logits, w13, w2, topk, bias=bias)
+        graphs.append((gr, y))
+    for gr, y in graphs * 3:
+        y.zero_()
+        gr.replay()
+        assert torch.equal(y, want)
+    fp4.check()
+
+
+@pytest.mark.parametrize("T", [7, 8, 9, 31])
+def test_the_same_token_many_times_gives_the_same_row(T):
+    from test_gpu_fp4_moe import experts
+    E, D, I, topk = 24, 640, 96, 5
+    w13, w2 = experts(E, D, I, 41)
+    g = torch.Generator().manual_seed(42)
+    x, logits = torch.randn(1, D, generator=g).cuda(), torch.randn(1, E, generator=g).cuda()
+    y = fp4.moe(x.repeat(T, 1), logits.repeat(T, 1), w13, w2, topk)
+    assert torch.equal(y, y[:1].expand(T, D)) and torch.equal(y[:1], fp4.moe(x, logits, w13, w2, topk)) or T > 8
