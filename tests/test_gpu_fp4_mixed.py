@@ -165,4 +165,4 @@ def test_the_same_token_many_times_gives_the_same_row(T):
     g = torch.Generator().manual_seed(42)
     x, logits = torch.randn(1, D, generator=g).cuda(), torch.randn(1, E, generator=g).cuda()
     y = fp4.moe(x.repeat(T, 1), logits.repeat(T, 1), w13, w2, topk)
-    assert torch.equal(y, y[:1].expand(T, D)) and torch.equal(y[:1], fp4.moe(x, logits, w13, w2, topk)) or T > 8
+    assert torch.equal(y, y[:1].expand(T, D)) and y.abs().max() > 0.1
