@@ -166,3 +166,75 @@ def test_the_same_token_many_times_gives_the_same_row(T):
     x, logits = torch.randn(1, D, generator=g).cuda(), torch.randn(1, E, generator=g).cuda()
     y = fp4.moe(x.repeat(T, 1), logits.repeat(T, 1), w13, w2, topk)
     assert torch.equal(y, y[:1].expand(T, D)) and y.abs().max() > 0.1
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_operands_made_on_another_stream(captured):
+    """Fork and join around every operator: one operand comes late from a second stream and the kernel before on the first one lets
+    its dependents start early; what the second stream wrote is what is read."""
+    from test_gpu_fp4_moe import experts
+    T, E, D, I, topk = 4, 8, 1024, 128, 2
+    g = torch.Generator().manual_seed(51)
+    w13, w2 = experts(E, D, I, 52)
+    w = fp4.quantize(torch.randn(1280, D, generator=g).cuda(), "nvfp4")
+    big = torch.randn(4096, 4096, generator=g).cuda()
+    xs = {m: torch.randn(m, D, generator=g).cuda() for m in (1, 20, 300)}
+    x, logits = torch.randn(T, D, generator=g).cuda(), torch.randn(T, E, generator=g).cuda()
+    bufs = {m: torch.empty_like(v) for m, v in xs.items()}
+    xb, lb = torch.empty_like(x), torch.empty_like(logits)
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    small = torch.randn(64, 128, device="cuda")
+
+    def late(dst, src):
+        """On the other stream: some work, then dst = src."""
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            dst.fill_(7.0)
+            a = big
+            for _ in range(3):
+                a = a @ big
+            dst.copy_(src)
+            dst.add_(a[:1, :1] * 0.0)
+        fp4.quantize(small)                      # on the main stream, ends long before
+        main.wait_stream(side)
+
+    def run():
+        out = []
+        for m in xs:
+            late(bufs[m], xs[m])
+            out.append(fp4.linear(bufs[m], w))
+            late(bufs[m], xs[m])
+            q = fp4.quantize(bufs[m], "nvfp4")
+            out.append(fp4.matmul(q, w))
+            out.append(fp4.dequantize(q))
+        late(xb, x), late(lb, logits)
+        out.append(fp4.moe(xb, lb, w13, w2, topk))
+        return out
+
+    big.mul_(4096 ** -0.5)
+    want = []
+    for m in xs:
+        q = fp4.quantize(xs[m], "nvfp4")
+        want += [fp4.linear(xs[m], w), fp4.matmul(q, w), fp4.dequantize(q)]
+    want.append(fp4.moe(x, logits, w13, w2, topk))
+    torch.cuda.synchronize()
+    if captured:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(main):
+            run()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(gr, stream=main):
+            got = run()
+        for _ in range(3):
+            [v.zero_() for v in got]
+            torch.cuda.synchronize()
+            gr.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    else:
+        for _ in range(3):
+            with torch.cuda.stream(main):
+                got = run()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    fp4.check()
