@@ -74,8 +74,6 @@ __device__ __forceinline__ void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uin
                      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(sfa), "r"(sfb) : "memory");
 }
 
-enum Stores : int { kByElement = 0, kTma = 1, kTmaButTheEnd = 2 };   // of P = X
-
 struct GemmArgs {
     const uint8_t *sfp, *sfq;
     const void* x;            // QX: the rows to quantise (row stride ldx, element type xdt; tensor scale xts if scaled)
@@ -86,7 +84,7 @@ struct GemmArgs {
     int64_t ldo;
     int64_t P, Q, K;
     float alpha;
-    int dtype, vec /* Stores */, tiles_p, tiles_q, splits;
+    int dtype, vec, tail, tiles_p, tiles_q, splits;   // vec: TMA can address out; tail: its rows end inside a 16-byte unit
     int behind;               // the kernel before this one is the quantiser of X, and everything before that is complete
     int* status;
 };
@@ -117,11 +115,12 @@ __device__ __forceinline__ void store_columns(const GemmArgs& a, uint32_t tmem, 
 // P = X: a lane holds a row's outputs side by side.  They go through two buffers of 32 rows x ROW bytes of this warp
 // (16-byte units swizzled as in TMA's 128- or 64-byte mode) and leave as TMA stores, which the tensor core does not wait
 // for: the accumulator is given back as soon as it is read.  Rows that TMA cannot address (base or row stride not a
-// multiple of 16 bytes) leave as stores of 32 neighbouring outputs, and so does the buffer in which a row ends inside a 16-byte
-// unit: TMA clips a box at whole units, and what is behind the row's end is not the output's.
+// multiple of 16 bytes) leave as stores of 32 neighbouring outputs, and so does a tile in which rows end inside a 16-byte unit: TMA
+// clips a box at whole units, and what is behind a row's end is not the output's.  (Decided per tile: a test per buffer, or the
+// last unit alone by element, cost all tiles 1.3 to 4 % of 1024 x 4096 x 24896.)
 template <typename T, int BN, int ROW, bool PAIR = false>
 __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap* tmap_o, uint32_t tmem, uint32_t buf0, int warp, int lane,
-                                           int64_t p0, int64_t q0, uint32_t acc_empty, int& turn) {
+                                           int64_t p0, int64_t q0, bool vec, uint32_t acc_empty, int& turn) {
     constexpr int kCols = ROW / (int)sizeof(T), kChunks = BN / 2 / kCols;   // columns of a buffer, buffers of this warp's half
     auto unit = [](int row, int u) { return (uint32_t)(row * ROW + ((u ^ (ROW == 128 ? row & 7 : row >> 1 & 3)) << 4)); };
     static_assert(kChunks >= 1, "a warp's half is a buffer at least");
@@ -155,7 +154,7 @@ __device__ __forceinline__ void store_rows(const GemmArgs& a, const CUtensorMap*
             }
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(buf + unit(lane, u)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
         }
-        if (a.vec == kTma || (a.vec == kTmaButTheEnd && (q + kCols <= a.Q || q >= a.Q))) {
+        if (vec) {
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
@@ -446,9 +445,10 @@ fp4_gemm_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_constan
                     else store_columns<float, BN>(a, tmem, quarter_warp, lane, p0, q0);
                 } else {
                     const uint32_t buf = staging + (uint32_t)w * 8192;
-                    if (a.dtype == kBf16) store_rows<__nv_bfloat16, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
-                    else if (a.dtype == kF16) store_rows<__half, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
-                    else store_rows<float, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, acc_empty, turn);
+                    const bool vec = a.vec && (!a.tail || q0 + BN <= a.Q);
+                    if (a.dtype == kBf16) store_rows<__nv_bfloat16, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, vec, acc_empty, turn);
+                    else if (a.dtype == kF16) store_rows<__half, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, vec, acc_empty, turn);
+                    else store_rows<float, BN, 128>(a, &tmap_o, tmem, buf, quarter_warp, lane, p0, q0, vec, acc_empty, turn);
                     continue;   // (store_rows gave the accumulator back)
                 }
             }
@@ -672,10 +672,11 @@ fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_p, const __grid_co
             const bool go = __shfl_sync(0xffffffffu, (done && *(volatile int*)&s_fail == 0) ? 1 : 0, 0) != 0;
             if (!go) break;
             const uint32_t buf = staging + (uint32_t)w * 4096;
+            const bool vec = a.vec && (!a.tail || q0 + 256 <= a.Q);
             const int64_t pr = p0 + 128 * rank;
-            if (a.dtype == kBf16) store_rows<__nv_bfloat16, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, peer_empty, turn);
-            else if (a.dtype == kF16) store_rows<__half, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, peer_empty, turn);
-            else store_rows<float, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, peer_empty, turn);
+            if (a.dtype == kBf16) store_rows<__nv_bfloat16, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, vec, peer_empty, turn);
+            else if (a.dtype == kF16) store_rows<__half, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, vec, peer_empty, turn);
+            else store_rows<float, 256, 64, true>(a, &tmap_o, tmem, buf, quarter_warp, lane, pr, q0, vec, peer_empty, turn);
         }
         if (lane == 0) bulk_wait<0>();
     }
@@ -834,7 +835,8 @@ static int fp4_matmul(const void* xc, const void* xs, const void* wc, const void
         (fmt != kMxFp4 && fmt != kNvFp4) || (((uintptr_t)xc | (uintptr_t)xs | (uintptr_t)wc | (uintptr_t)ws) & 15))
         return (int)cudaErrorInvalidValue;
     const int esz = a.dtype == kF32 ? 4 : 2;
-    a.vec = ((uintptr_t)a.out & 15) || a.ldo * esz % 16 ? kByElement : N * esz % 16 ? kTmaButTheEnd : kTma;
+    a.vec = ((uintptr_t)a.out & 15) == 0 && a.ldo * esz % 16 == 0;
+    a.tail = N * esz % 16 != 0;
     a.status = status ? status : fp4_status_ptr();
     if (!a.status) return (int)cudaErrorNotSupported;
     return fmt == kMxFp4 ? gemm_fmt<kMxFp4>(a, xc, (const uint8_t*)xs, wc, (const uint8_t*)ws, M, N, st)
