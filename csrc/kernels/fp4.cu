@@ -5,9 +5,11 @@
 //           code = e2m1(u / s), both quotients rounded to f32 first
 //
 // Both kernels are bound by HBM (2 + 17/32 bytes per bf16 value) but for the quantiser to nvfp4, whose instructions per
-// value weigh as much (83 % of the issue slots).  24896 x 4096, call after call: f32 to either format 68 us (6.8 TB/s), bf16 to
-// mxfp4 42.3 us (6.1 TB/s), to nvfp4 48.3 us (5.3 TB/s; 12 us more with scalar products, a division and a rounded reciprocal
-// per block), with a tensor scale 53 us; expanded to bf16 43.7 us (5.9 TB/s), to f32 76 us (6.1 TB/s).  A thread owns eight consecutive
+// value weigh as much (83 % of the issue slots).  24896 x 4096 in a graph of many: f32 to either format 68 us (6.8 TB/s), bf16 to
+// mxfp4 41.3 us (6.2 TB/s), to nvfp4 47 us (5.5 TB/s; 12 us more with scalar products, a division and a rounded reciprocal
+// per block), with a tensor scale 52 us; expanded to bf16 42.5 us (6.1 TB/s), to f32 74 us (6.3 TB/s).  A matrix whose base, row
+// stride or width is no multiple of eight values goes by element, in all of its tiles: 24896 x 4095 bf16 75 to 85 us and 289 us
+// back, f32 110 and 357 us.  A thread owns eight consecutive
 // columns (one 16-byte load of 16-bit values, one 4-byte store of codes), a block of 32 (16) columns is four (two)
 // lanes, and a warp takes the four rows i, 32 + i, 64 + i, 96 + i of a 128-row tile over 256 columns: four independent
 // loads in flight per thread, and the scales of those rows are 16 consecutive bytes of a chunk, so one lane writes them

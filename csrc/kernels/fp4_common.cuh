@@ -15,7 +15,7 @@
 enum Fp4Fmt : int { kMxFp4 = 0, kNvFp4 = 1 };
 enum Fp4Dtype : int { kF32 = 0, kBf16 = 1, kF16 = 2 };
 
-// fb_fp4_quantize (fp4.cu).  pdl: as above; without, the product behind it starts earlier (60 x 4096 x 4096: 10.4 us for both
+// fb_fp4_quantize (fp4.cu).  pdl: as for fp4_launch below; without, the product behind it starts earlier (60 x 4096 x 4096: 10.4 us for both
 // launches, 11.8 with).
 int fp4_quantize(const void* x, int64_t dtype, int64_t ld, int64_t bstride, void* codes, void* scales, int64_t batch, int64_t rows,
                  int64_t cols, int64_t fmt, float ts, bool pdl, cudaStream_t st);

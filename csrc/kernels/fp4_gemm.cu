@@ -11,15 +11,16 @@
 // weights fill the lanes whatever the number of rows, and the K axis is split over a cluster of S CTAs whose partial
 // tiles are summed in rank order through distributed shared memory: no workspace, no atomics, the same bits every run.
 //
-// Bounds.  Few rows: the weights' bytes from HBM; 1 x 129280 x 5120 mxfp4 58 us (6.1 TB/s), 1 x 8192 x 5120 8.6 us (3.4 for the
-// bytes), 16 x 4096 x 24896 nvfp4 14.4 us with its quantiser (8.9 for the bytes: the rest is the latency of two launches and of
-// the first tiles).  Many rows: the tensor cores and the operands' way from L2; 8192 x 8192 x 8192 mxfp4 187 us (5.9 PFLOP/s),
-// nvfp4 212 us, 8192 x 4096 x 24896 nvfp4 400 us, where repeated calls run into the power cap (about 1.55 GHz).
+// Bounds (times in graphs of many calls).  Few rows: the weights' bytes from HBM; 1 x 5120 x 129280 mxfp4 59 us (5.9 TB/s), 1 x 8192 x
+// 5120 8.8 us (3.4 for the bytes), 16 x 4096 x 24896 nvfp4 14.8 us with its quantiser (8.9 for the bytes: the rest is the latency of
+// two launches and of the first tiles).  Many rows: the tensor cores and the operands' way from L2; 8192 x 8192 x 8192 mxfp4 192 us
+// (5.7 PFLOP/s, twenty calls after a pause), nvfp4 217 us, 8192 x 4096 x 24896 nvfp4 404 us, where repeated calls run into the
+// power cap (about 1.55 GHz).
 //
 // Warps: 0 producer (TMA boxes of both operands, bulk copies of the scale chunks), 1 MMA issuer, 2..9 epilogue (two per
 // lane quarter).  Without a split the CTAs are persistent and walk the tiles; the accumulator is handed to the epilogue
 // and back through two barriers.  Every wait has a clock budget; on expiry the status words say so, the tile is not
-// stored and the tensor memory is released.
+// stored, the copies in flight are waited for and the tensor memory is released.
 #include "fp4_common.cuh"
 
 namespace {

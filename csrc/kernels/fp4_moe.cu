@@ -1,6 +1,6 @@
 // A whole layer of 4-bit experts for a few tokens (1..32) in two kernels.
 //
-//   p = score(logits), chosen = top-k of p + bias (ties to the lower index), w = scale * p / sum(chosen p)
+//   p = score(logits), chosen = top-k of p + bias (in f32; ties to the lower index), w = scale * p / sum(chosen p)
 //   g, u = W13[e] . e4m3(x)                            e4m3(.): power-of-two scale per 32 values
 //   h[e, t] = e4m3(silu(min(g, limit)) * clamp(u, -limit, limit) * w[t, e])
 //   y[t] = sum over chosen e of W2[e] . h[e, t]
@@ -26,7 +26,7 @@
 // Kernel 2 then reads the list of chosen experts, which kernel 1 leaves behind (routing again there cost 4 us at its head).
 // Experts of 5120 x 2304, a call among others: one token (6 experts, 113 MB, 17.2 us of HBM) 34 us: 7 until the first weight of kernel 1
 // (routing 5), 12.5 of weights, 5 until the first weight of kernel 2, 5 of weights, 2 for the sum; 5 tokens (15 experts, 43 us of HBM)
-// 58 us; 32 tokens (88 experts, 252 us of HBM) 313 us, 18 of them routing.  8 tokens of 44 experts of 5120 x 576 (32 us of HBM)
+// 59 us; 32 tokens (88 experts, 252 us of HBM) 320 us, 18 of them routing.  8 tokens of 44 experts of 5120 x 576 (32 us of HBM)
 // 60 us.  The first kernel's weights in flight decide at 32 tokens: six stages beside x and the receive slots 338 us, seven 317.
 #include "fp4_common.cuh"
 

@@ -41,7 +41,8 @@ class Fp4Tensor:
     """A 4-bit tensor ``[..., rows, cols]``: ``codes`` [..., rows, 64 * ceil(cols / 128)] uint8 (the even column in the low
     nibble, zero codes behind the last column) and ``scales`` [..., ceil(rows / 128), C, 512] uint8 with C =
     ceil(cols / 128) (mxfp4) or twice that (nvfp4): byte ``16 i + 4 g + s`` of a chunk is the scale of row ``32 g + i`` and
-    block ``s`` of the chunk's four.  Scale bytes of rows and blocks that do not exist are never NaN codes.
+    block ``s`` of the chunk's four.  Scales are not negative (an nvfp4 byte has no sign bit); scale bytes of rows and blocks that
+    do not exist are never NaN codes.
 
     ``tensor_scale`` (a float, nvfp4 only) multiplies every value."""
 
